@@ -48,8 +48,19 @@ enum {
 };
 
 /* KV storage types: GpuElement::{F32,Bf16} (src/decode_resident/arena.rs:26-41)
- * plus the u8 group-32 affine format (32 codes + bf16 scale + bf16 bias). */
-enum { SGK_KV_F32 = 0, SGK_KV_BF16 = 1, SGK_KV_U8G32 = 2 };
+ * plus the u8 group-32 affine format (32 codes + bf16 scale + bf16 bias) and the u4 one. */
+enum { SGK_KV_F32 = 0, SGK_KV_BF16 = 1, SGK_KV_U8G32 = 2, SGK_KV_U4G32 = 3 };
+/* SGK_KV_U4G32 (no counterpart in the reference, whose KV is f32 or bf16): per 32 contiguous values x of a head
+ * row at position r, with y = x for even r and y = -x for odd r,
+ *   bias = bf16(min y); step = bf16(max((max y - bias) / 15, 2^-40, 2^(e-16))) where 2^e is the power of two
+ *   at or below the largest (max y - bias) / 15 of the head row (2^-40 at least);
+ *   code = nearest((y - bias) / step) within 0..15, ties to even.
+ * Every rounding is of the exact value. scale = (-1)^r step and bias = (-1)^r bias are what is kept, and
+ * value = code * scale + bias is what the row reads back as: the affine formula of the u8 format, the scales
+ * of odd rows negative (sums of weighted values then lose no digits to a common offset). A group that
+ * holds an infinity or a NaN, or whose range overflows, reads back as NaN. head_dim: a multiple of 32. A row of a head
+ * takes head_dim * 10 / 16 + 1 bytes for K and as many for V. The tensor-core attention kernel takes
+ * head_dim 128 and 256 with up to 8 query heads per KV head; other shapes go to the generic kernel. */
 
 /* Tokens per page. The page is the unit of allocation, sharing and copy. */
 #define SGK_PAGE_TOKENS 16
@@ -136,6 +147,10 @@ int32_t sgk_seq_block_table(const sgk_seq* seq, int32_t* pages_out, int64_t cap,
 int32_t sgk_seq_reset(sgk_seq* seq, void* stream);
 /* Sliding-window layers: returns pages that lie wholly before `row` to the pool. */
 int32_t sgk_seq_release_before(sgk_seq* seq, int64_t row);
+/* The same where the first rows stay visible (attention sinks): returns the pages that lie wholly inside rows
+ * [first_row, row). What has been returned is one range of a sequence; a call extends it at either end
+ * (Dimension error when rows would be left between the two). */
+int32_t sgk_seq_release_between(sgk_seq* seq, int64_t first_row, int64_t row);
 /* FullAttentionMetalState view of (sequence, layer). Owned by the sequence. */
 int32_t sgk_seq_layer(sgk_seq* seq, int32_t layer, int32_t q_heads, sgk_kv** out);
 
@@ -159,6 +174,15 @@ int32_t sgk_kv_dtype(const sgk_kv* kv);
 int64_t sgk_kv_byte_len(const sgk_kv* kv); /* capacity * kv_dim * storage bytes, K or V */
 /* kv.truncate(len) (attention.rs:501-510): moves the cursor only. */
 int32_t sgk_kv_truncate(sgk_kv* kv, int64_t len);
+/* The same in stream order, without waiting: the cursor moves when `stream` gets there. Where len needs pages
+ * that the sequence does not hold yet, taking them is synchronous (sgk_seq_reserve). */
+int32_t sgk_kv_enqueue_truncate(sgk_kv* kv, void* stream, int64_t len);
+/* Attention sinks (no counterpart in the reference): the first `rows` rows stay visible to every attention over this
+ * KV state that has a window (window_start or sliding_window), beside the window's own rows: row r is seen when
+ * r < rows or r >= window start. 0 (the default): none. A property of the layer: a batch's members share it
+ * (Config error otherwise), a captured step keeps the number it was captured with. */
+int32_t sgk_kv_set_attention_sinks(sgk_kv* kv, int64_t rows);
+int64_t sgk_kv_attention_sinks(const sgk_kv* kv);
 /* kv.seed(keys_rows, values_rows, n_rows) (attention.rs:550-602) */
 int32_t sgk_kv_seed_f32(sgk_kv* kv, const float* k, size_t k_len, const float* v, size_t v_len,
                         int64_t n_rows);
@@ -231,12 +255,16 @@ int32_t sgk_kv_enqueue_append_attention(sgk_kv* kv, void* stream, const float* d
                                         float attn_scalar);
 /* kv.keys()/values() read-back used by the reference's tests (tests.rs:380-478):
  * the paged GATHER. Rows [row0,row0+n) as contiguous [n, kv_dim] in the storage
- * type (f32: float, bf16: uint16 bit patterns). For u8 use the _u8 form. */
+ * type (f32: float, bf16: uint16 bit patterns). For u8 and u4 use the _u8 and _u4 forms (a byte per code). */
 int32_t sgk_kv_gather_rows(sgk_kv* kv, int64_t row0, int64_t n, void* k_out, void* v_out);
 int32_t sgk_kv_gather_rows_u8(sgk_kv* kv, int64_t row0, int64_t n, uint8_t* k_codes, uint16_t* k_scale,
                               uint16_t* k_bias, uint8_t* v_codes, uint16_t* v_scale, uint16_t* v_bias);
-/* Same rows decoded to f32 (bf16 upcast, u8 q*scale+bias, src/quantization.rs:173-179). */
+int32_t sgk_kv_gather_rows_u4(sgk_kv* kv, int64_t row0, int64_t n, uint8_t* k_codes, uint16_t* k_scale,
+                              uint16_t* k_bias, uint8_t* v_codes, uint16_t* v_scale, uint16_t* v_bias);
+/* Same rows decoded to f32 (bf16 upcast, u8 and u4 q*scale+bias, src/quantization.rs:173-179). */
 int32_t sgk_kv_gather_rows_f32(sgk_kv* kv, int64_t row0, int64_t n, float* k_out, float* v_out);
+/* The decoded rows into device memory, [n][kv_dim] each, 16-byte aligned: enqueue only. */
+int32_t sgk_kv_enqueue_gather_rows_f32(sgk_kv* kv, void* stream, int64_t row0, int64_t n, float* d_k, float* d_v);
 int32_t sgk_kv_block_table(const sgk_kv* kv, int32_t* pages_out, int64_t cap, int64_t* n_out);
 /* Forces one attention kernel: 0 = automatic, 1 = generic CUDA-core kernel,
  * 2 = tensor-core paged kernel (errors if the shape does not qualify). */
@@ -257,6 +285,9 @@ int32_t sgk_batch_enqueue_attention(sgk_batch* batch, void* stream, const float*
 int32_t sgk_batch_enqueue_step(sgk_batch* batch, void* stream, const float* d_k, const float* d_v,
                                const float* d_q, float* d_out, int64_t sliding_window,
                                float attn_scalar);
+/* Moves the cursor of every member, in stream order (lens: [n], host memory; one launch per 512 members):
+ * drops the rejected tails of a batched verify, which differ from sequence to sequence. */
+int32_t sgk_batch_enqueue_truncate(sgk_batch* batch, void* stream, const int64_t* lens);
 /* Tuning hooks read by the benchmark: 0 = automatic. */
 /* Speculative-decoding verify (src/decode_resident/layers.rs:1295-1433; CPU twin
  * cached_attention_prefill_rows, src/decoder/attention_ops.rs:976-1017): n_rows draft rows

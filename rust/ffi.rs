@@ -19,6 +19,7 @@ pub const SGK_ERR_TIMEOUT: i32 = 6;
 pub const SGK_KV_F32: i32 = 0;
 pub const SGK_KV_BF16: i32 = 1;
 pub const SGK_KV_U8G32: i32 = 2;
+pub const SGK_KV_U4G32: i32 = 3;
 pub const SGK_PAGE_TOKENS: usize = 16;
 pub const SGK_NOALLOC_SCRATCH_BYTES: usize = 4 << 20;
 pub const SGK_NOALLOC_MAX_Q_DIM: usize = 16384;
@@ -147,6 +148,7 @@ extern "C" {
     pub fn sgk_seq_block_table(seq: *const SgkSeq, pages_out: *mut i32, cap: i64, n_out: *mut i64) -> i32;
     pub fn sgk_seq_reset(seq: *mut SgkSeq, stream: *mut std::ffi::c_void) -> i32;
     pub fn sgk_seq_release_before(seq: *mut SgkSeq, row: i64) -> i32;
+    pub fn sgk_seq_release_between(seq: *mut SgkSeq, first_row: i64, row: i64) -> i32;
     pub fn sgk_seq_layer(seq: *mut SgkSeq, layer: i32, q_heads: i32, out: *mut *mut SgkKv) -> i32;
     pub fn sgk_kv_create(state: *mut SgkState, capacity: i64, q_heads: i32, kv_heads: i32, head_dim: i32, dtype: i32, page_tokens: i32, out: *mut *mut SgkKv) -> i32;
     pub fn sgk_kv_create_shuffled(state: *mut SgkState, capacity: i64, q_heads: i32, kv_heads: i32, head_dim: i32, dtype: i32, seed: u64, out: *mut *mut SgkKv) -> i32;
@@ -160,6 +162,9 @@ extern "C" {
     pub fn sgk_kv_dtype(kv: *const SgkKv) -> i32;
     pub fn sgk_kv_byte_len(kv: *const SgkKv) -> i64;
     pub fn sgk_kv_truncate(kv: *mut SgkKv, len: i64) -> i32;
+    pub fn sgk_kv_enqueue_truncate(kv: *mut SgkKv, stream: *mut std::ffi::c_void, len: i64) -> i32;
+    pub fn sgk_kv_set_attention_sinks(kv: *mut SgkKv, rows: i64) -> i32;
+    pub fn sgk_kv_attention_sinks(kv: *const SgkKv) -> i64;
     pub fn sgk_kv_seed_f32(kv: *mut SgkKv, k: *const f32, k_len: usize, v: *const f32, v_len: usize, n_rows: i64) -> i32;
     pub fn sgk_kv_append_row_f32(kv: *mut SgkKv, k: *const f32, k_len: usize, v: *const f32, v_len: usize) -> i32;
     pub fn sgk_kv_append_rows_f32(kv: *mut SgkKv, k: *const f32, k_len: usize, v: *const f32, v_len: usize, n_rows: i64) -> i32;
@@ -175,7 +180,9 @@ extern "C" {
     pub fn sgk_kv_enqueue_append_attention(kv: *mut SgkKv, stream: *mut std::ffi::c_void, d_k: *const f32, d_v: *const f32, d_q: *const f32, d_out: *mut f32, sliding_window: i64, attn_scalar: f32) -> i32;
     pub fn sgk_kv_gather_rows(kv: *mut SgkKv, row0: i64, n: i64, k_out: *mut std::ffi::c_void, v_out: *mut std::ffi::c_void) -> i32;
     pub fn sgk_kv_gather_rows_u8(kv: *mut SgkKv, row0: i64, n: i64, k_codes: *mut u8, k_scale: *mut u16, k_bias: *mut u16, v_codes: *mut u8, v_scale: *mut u16, v_bias: *mut u16) -> i32;
+    pub fn sgk_kv_gather_rows_u4(kv: *mut SgkKv, row0: i64, n: i64, k_codes: *mut u8, k_scale: *mut u16, k_bias: *mut u16, v_codes: *mut u8, v_scale: *mut u16, v_bias: *mut u16) -> i32;
     pub fn sgk_kv_gather_rows_f32(kv: *mut SgkKv, row0: i64, n: i64, k_out: *mut f32, v_out: *mut f32) -> i32;
+    pub fn sgk_kv_enqueue_gather_rows_f32(kv: *mut SgkKv, stream: *mut std::ffi::c_void, row0: i64, n: i64, d_k: *mut f32, d_v: *mut f32) -> i32;
     pub fn sgk_kv_block_table(kv: *const SgkKv, pages_out: *mut i32, cap: i64, n_out: *mut i64) -> i32;
     pub fn sgk_kv_set_attention_kernel(kv: *mut SgkKv, which: i32) -> i32;
     pub fn sgk_batch_create(state: *mut SgkState, kvs: *mut *mut SgkKv, n: i32, out: *mut *mut SgkBatch) -> i32;
@@ -183,6 +190,7 @@ extern "C" {
     pub fn sgk_batch_enqueue_append(batch: *mut SgkBatch, stream: *mut std::ffi::c_void, d_k: *const f32, d_v: *const f32) -> i32;
     pub fn sgk_batch_enqueue_attention(batch: *mut SgkBatch, stream: *mut std::ffi::c_void, d_q: *const f32, d_out: *mut f32, sliding_window: i64, attn_scalar: f32) -> i32;
     pub fn sgk_batch_enqueue_step(batch: *mut SgkBatch, stream: *mut std::ffi::c_void, d_k: *const f32, d_v: *const f32, d_q: *const f32, d_out: *mut f32, sliding_window: i64, attn_scalar: f32) -> i32;
+    pub fn sgk_batch_enqueue_truncate(batch: *mut SgkBatch, stream: *mut std::ffi::c_void, lens: *const i64) -> i32;
     pub fn sgk_batch_enqueue_verify_rows(batch: *mut SgkBatch, stream: *mut std::ffi::c_void, d_k: *const f32, d_v: *const f32, d_q: *const f32, d_out: *mut f32, n_rows: i32, sliding_window: i64, attn_scalar: f32) -> i32;
     pub fn sgk_batch_set_splits(batch: *mut SgkBatch, splits: i32) -> i32;
     pub fn sgk_batch_get_splits(batch: *const SgkBatch, splits_out: *mut i32) -> i32;

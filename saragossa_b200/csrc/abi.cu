@@ -137,11 +137,12 @@ int32_t sgk_pool_create(sgk_state* st, int32_t layers, int32_t kv_heads, int32_t
   if (layers <= 0 || kv_heads <= 0 || head_dim <= 0 || num_pages <= 0 || max_seqs <= 0 || max_seq_tokens <= 0)
     return fail(SGK_ERR_CONFIG, "pool: zero dimension");
   if (page_tokens != SGK_PAGE_TOKENS) return fail(SGK_ERR_CONFIG, "pool: page_tokens must be %d", SGK_PAGE_TOKENS);
-  if (dtype < SGK_KV_F32 || dtype > SGK_KV_U8G32) return fail(SGK_ERR_BACKEND, "pool: unknown KV element type %d", dtype);
-  if (dtype == SGK_KV_U8G32 && head_dim % QGROUP != 0)
-    return fail(SGK_ERR_CONFIG, "u8 KV needs head_dim to be a multiple of %d", QGROUP);
+  if (dtype < SGK_KV_F32 || dtype > SGK_KV_U4G32) return fail(SGK_ERR_BACKEND, "pool: unknown KV element type %d", dtype);
+  const bool quantised = dtype == SGK_KV_U8G32 || dtype == SGK_KV_U4G32;
+  if (quantised && head_dim % QGROUP != 0)
+    return fail(SGK_ERR_CONFIG, "%s KV needs head_dim to be a multiple of %d", dtype == SGK_KV_U8G32 ? "u8" : "u4", QGROUP);
   if (head_dim > 512) return fail(SGK_ERR_CONFIG, "head_dim %d > 512 is not supported", head_dim);
-  if (dtype != SGK_KV_U8G32 && (int64_t(head_dim) * (dtype == SGK_KV_F32 ? 4 : 2) * PAGE_TOKENS) % 16 != 0)
+  if (!quantised && (int64_t(head_dim) * (dtype == SGK_KV_F32 ? 4 : 2) * PAGE_TOKENS) % 16 != 0)
     return fail(SGK_ERR_CONFIG, "head_dim %d gives tiles that are not 16-byte multiples", head_dim);
   auto p = std::make_unique<sgk_pool>();
   p->st = st;
@@ -294,15 +295,17 @@ int32_t sgk_seq_block_table(const sgk_seq* s, int32_t* pages_out, int64_t cap, i
   return SGK_OK;
 }
 
-int32_t sgk_seq_release_before(sgk_seq* s, int64_t row) {
+int32_t sgk_seq_release_between(sgk_seq* s, int64_t first_row, int64_t row) {
   if (!s) return fail(SGK_ERR_BACKEND, "null sequence");
-  if (row < 0) return fail(SGK_ERR_DIMENSION, "negative row");
+  if (first_row < 0 || row < 0) return fail(SGK_ERR_DIMENSION, "negative row");
   if (!s->pool->host_only()) {
     SGK_CUDA(s->pool->st->order_after_last_caller(s->pool->st->stream));
     SGK_CUDA(cudaStreamSynchronize(s->pool->st->stream));
   }
-  return s->release_before(row);
+  return s->release_between(first_row, row);
 }
+
+int32_t sgk_seq_release_before(sgk_seq* s, int64_t row) { return sgk_seq_release_between(s, 0, row); }
 
 int32_t sgk_seq_layer(sgk_seq* s, int32_t layer, int32_t q_heads, sgk_kv** out) {
   if (!s || !out) return fail(SGK_ERR_BACKEND, "null argument");
@@ -399,6 +402,23 @@ int32_t sgk_kv_truncate(sgk_kv* kv, int64_t len) {
   SGK_CUDA(cudaStreamSynchronize(kv->st->stream));
   return SGK_OK;
 }
+
+int32_t sgk_kv_enqueue_truncate(sgk_kv* kv, void* stream, int64_t len) {
+  if (!kv) return fail(SGK_ERR_BACKEND, "null KV state");
+  if (kv->pool()->host_only()) return fail(SGK_ERR_BACKEND, "enqueue over a bookkeeping-only pool");
+  if (len < 0 || len > kv->seq->capacity)
+    return fail(SGK_ERR_DIMENSION, "truncate KV %lld > capacity %lld", (long long)len, (long long)kv->seq->capacity);
+  SGK_TRY(kv->seq->reserve(len));
+  return kv->seq->set_len(kv->layer, len, kv->st->pick(stream));
+}
+
+int32_t sgk_kv_set_attention_sinks(sgk_kv* kv, int64_t rows) {
+  if (!kv) return fail(SGK_ERR_BACKEND, "null KV state");
+  if (rows < 0) return fail(SGK_ERR_DIMENSION, "negative number of attention sinks");
+  kv->sink_rows = rows;
+  return SGK_OK;
+}
+int64_t sgk_kv_attention_sinks(const sgk_kv* kv) { return kv ? kv->sink_rows : 0; }
 
 static int32_t append_rows_host(sgk_kv* kv, const float* k, size_t k_len, const float* v, size_t v_len, int64_t n_rows,
                                 bool reset) {
@@ -610,12 +630,12 @@ static int32_t gather_impl(sgk_kv* kv, int64_t row0, int64_t n, int mode, void* 
     return fail(SGK_ERR_DIMENSION, "gather rows [%lld,%lld) outside len %lld", (long long)row0, (long long)(row0 + n),
                 (long long)kv->len());
   if (n == 0) return SGK_OK;
-  if (row0 / PAGE_TOKENS < kv->seq->released_pages)
+  if (kv->seq->released(row0 / PAGE_TOKENS, (row0 + n + PAGE_TOKENS - 1) / PAGE_TOKENS))
     return fail(SGK_ERR_DIMENSION, "gather reaches rows released by the sliding window");
   Pool* pool = kv->pool();
   const size_t cells = static_cast<size_t>(n) * kv->kv_dim();
   size_t esz = mode == 1 ? 4 : (pool->dtype == KV_F32 ? 4 : pool->dtype == KV_BF16 ? 2 : 1);
-  const size_t groups = pool->dtype == KV_U8G32 && mode == 2 ? cells / QGROUP : 0;
+  const size_t groups = mode == 2 ? cells / QGROUP : 0;
   size_t bytes = 2 * cells * esz + 4 * groups * sizeof(uint16_t);
   uint8_t* d = nullptr;
   SGK_CUDA(cudaMalloc(&d, bytes));
@@ -655,6 +675,8 @@ static int32_t gather_impl(sgk_kv* kv, int64_t row0, int64_t n, int mode, void* 
 int32_t sgk_kv_gather_rows(sgk_kv* kv, int64_t row0, int64_t n, void* k_out, void* v_out) {
   if (kv && kv->pool()->dtype == KV_U8G32)
     return fail(SGK_ERR_BACKEND, "gather_rows on a u8 KV: use gather_rows_u8 or gather_rows_f32");
+  if (kv && kv->pool()->dtype == KV_U4G32)
+    return fail(SGK_ERR_BACKEND, "gather_rows on a u4 KV: use gather_rows_u4 or gather_rows_f32");
   return gather_impl(kv, row0, n, 0, k_out, v_out, nullptr, nullptr, nullptr, nullptr);
 }
 
@@ -663,6 +685,40 @@ int32_t sgk_kv_gather_rows_u8(sgk_kv* kv, int64_t row0, int64_t n, uint8_t* k_co
   if (kv && kv->pool()->dtype != KV_U8G32) return fail(SGK_ERR_BACKEND, "gather_rows_u8 on a KV that is not u8");
   if (!k_scale || !k_bias || !v_scale || !v_bias) return fail(SGK_ERR_BACKEND, "null host pointer");
   return gather_impl(kv, row0, n, 2, k_codes, v_codes, k_scale, k_bias, v_scale, v_bias);
+}
+
+int32_t sgk_kv_gather_rows_u4(sgk_kv* kv, int64_t row0, int64_t n, uint8_t* k_codes, uint16_t* k_scale,
+                              uint16_t* k_bias, uint8_t* v_codes, uint16_t* v_scale, uint16_t* v_bias) {
+  if (kv && kv->pool()->dtype != KV_U4G32) return fail(SGK_ERR_BACKEND, "gather_rows_u4 on a KV that is not u4");
+  if (!k_scale || !k_bias || !v_scale || !v_bias) return fail(SGK_ERR_BACKEND, "null host pointer");
+  return gather_impl(kv, row0, n, 2, k_codes, v_codes, k_scale, k_bias, v_scale, v_bias);
+}
+
+int32_t sgk_kv_enqueue_gather_rows_f32(sgk_kv* kv, void* stream, int64_t row0, int64_t n, float* d_k, float* d_v) {
+  if (!kv) return fail(SGK_ERR_BACKEND, "null KV state");
+  if (!d_k || !d_v) return fail(SGK_ERR_BACKEND, "gather: null device pointer");
+  Pool* pool = kv->pool();
+  if (pool->host_only()) return fail(SGK_ERR_BACKEND, "gather over a bookkeeping-only pool");
+  if (row0 < 0 || n < 0 || row0 > kv->len() || n > kv->len() - row0)
+    return fail(SGK_ERR_DIMENSION, "gather of %lld rows from row %lld outside len %lld", (long long)n, (long long)row0,
+                (long long)kv->len());
+  if (n == 0) return SGK_OK;
+  if (kv->seq->released(row0 / PAGE_TOKENS, (row0 + n + PAGE_TOKENS - 1) / PAGE_TOKENS))
+    return fail(SGK_ERR_DIMENSION, "gather reaches rows released by the sliding window");
+  GatherArgs a{};
+  a.pool = pool->view();
+  a.layer = kv->layer;
+  a.slot = kv->seq->slot;
+  a.row0 = row0;
+  a.n = n;
+  a.mode = 1;
+  a.k_out = d_k;
+  a.v_out = d_v;
+  a.num_pages = pool->num_pages;
+  a.status = kv->st->d_status;
+  SGK_CUDA(launch_gather(a, kv->st->pick(stream)));
+  kv->st->launches += 1;
+  return SGK_OK;
 }
 
 int32_t sgk_kv_gather_rows_f32(sgk_kv* kv, int64_t row0, int64_t n, float* k_out, float* v_out) {
@@ -713,6 +769,12 @@ int32_t sgk_batch_enqueue_attention(sgk_batch* b, void* stream, const float* d_q
   if (!b) return fail(SGK_ERR_BACKEND, "null batch");
   if (sliding_window < 0) return fail(SGK_ERR_DIMENSION, "negative sliding window");
   return b->enqueue_attention(b->st->pick(stream), d_q, d_out, 0, sliding_window, attn_scalar, nullptr, nullptr);
+}
+
+int32_t sgk_batch_enqueue_truncate(sgk_batch* b, void* stream, const int64_t* lens) {
+  if (!b) return fail(SGK_ERR_BACKEND, "null batch");
+  if (!lens) return fail(SGK_ERR_BACKEND, "truncate: null host pointer");
+  return b->enqueue_truncate(b->st->pick(stream), lens);
 }
 
 int32_t sgk_batch_enqueue_step(sgk_batch* b, void* stream, const float* d_k, const float* d_v, const float* d_q,

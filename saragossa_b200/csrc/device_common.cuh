@@ -2,6 +2,7 @@
 // reference's host code), element access through the page layout, and the
 // split-K partial merge.
 #pragma once
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -25,13 +26,29 @@ __device__ __forceinline__ float bf16_bits_to_f32(uint16_t b) {
   return __uint_as_float(static_cast<uint32_t>(b) << 16);
 }
 
+// Signed step of (row, group) of a u4 tile as f32. V steps are stored divided by their row's power of two.
+__device__ __forceinline__ float u4_step(const uint8_t* tile, int hd, int is_v, int row, int grp) {
+  const uint16_t bits = *reinterpret_cast<const uint16_t*>(tile + u4_step_offset(is_v, row, grp, hd));
+  if (!is_v) return bf16_bits_to_f32(bits);
+  const uint8_t* pow_tile = row < 8 ? tile - tile_bytes(KV_U4G32, hd) : tile;   // the K tile lies before the V tile
+  return __half2float(__ushort_as_half(bits)) *
+         bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(pow_tile + u4_pow_offset(row, hd)));
+}
+__device__ __forceinline__ int u4_code(const uint8_t* tile, int hd, int is_v, int row, int dim) {
+  return (tile[is_v ? u4_v_byte(row, dim, hd) : u4_k_byte(row, dim, hd)] >> (4 * u4_nibble(dim))) & 15;
+}
+
 // One stored element (row, dim) of a tile decoded to f32: f32 as is, bf16 upcast,
-// u8 q*scale+bias with separate roundings (src/quantization.rs:173-179).
+// u8 q*scale+bias with separate roundings (src/quantization.rs:173-179), u4 the same (there the
+// product is exact). A V tile is decoded where it lies, behind its K tile.
 __device__ __forceinline__ float load_tile_elem(const uint8_t* tile, int dtype, int hd, int is_v,
                                                 int row, int dim) {
   if (dtype == KV_F32) return reinterpret_cast<const float*>(tile)[row * hd + dim];
   if (dtype == KV_BF16)
     return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(tile)[bf16_elem_index(row, dim, hd)]);
+  if (dtype == KV_U4G32)
+    return __fadd_rn(__fmul_rn(static_cast<float>(u4_code(tile, hd, is_v, row, dim)), u4_step(tile, hd, is_v, row, dim / QGROUP)),
+                     bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u4_bias_offset(row, dim / QGROUP, hd))));
   int idx = is_v ? u8_v_code_index(row, dim, hd) : u8_k_code_index(row, dim, hd);
   float scale = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u8_scale_offset(row, dim / QGROUP, hd)));
   float bias = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u8_bias_offset(is_v, row, dim / QGROUP, hd)));

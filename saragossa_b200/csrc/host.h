@@ -37,6 +37,17 @@ const char* last_error_cstr();
   } while (0)
 
 struct Exchange;
+// What an attention over rows [0, len) with a window from row `start` sees beside the window: the pages
+// [0, pages) that hold the sinks (fewer where they reach the window's first page) and `rows` rows of them.
+struct SinkSpan {
+  int64_t rows, pages;
+  SinkSpan(int64_t sink_rows, int64_t start) {
+    rows = sink_rows < start ? sink_rows : start;
+    pages = (rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
+    if (pages > start / PAGE_TOKENS) pages = start / PAGE_TOKENS;
+  }
+};
+
 // Where the next attention launch of a batch also sends its outputs (set by the exchange entry point
 // for one enqueue): the peers' counterparts of d_out.
 struct PeerTarget {
@@ -160,7 +171,11 @@ struct Seq {
   int slot = -1;
   int64_t capacity = 0;
   std::vector<int32_t> pages;  // page id per page index, -1 once released
-  int64_t released_pages = 0;  // leading page indices already returned to the pool
+  // page indices [released_first, released_pages) have been returned to the pool; rows before
+  // released_first are sinks that stay
+  int64_t released_first = 0, released_pages = 0;
+  // whether any of the page indices [first, last) has been returned
+  bool released(int64_t first, int64_t last) const { return first < released_pages && last > released_first && first < last; }
   std::vector<int64_t> len;    // per layer, host mirror of the device cursor
   std::vector<std::unique_ptr<Kv>> views;
   // Changes whenever pages of the sequence are released or replaced (never when pages are only
@@ -169,7 +184,7 @@ struct Seq {
   void new_epoch();
 
   int reserve(int64_t tokens);
-  int release_before(int64_t row);
+  int release_between(int64_t first_row, int64_t row);
   int release_all();
   // Makes the page holding `row` exclusively owned (copy-on-write of a shared page).
   int ensure_writable(int64_t row, cudaStream_t stream);
@@ -185,6 +200,7 @@ struct Kv {
   Seq* seq = nullptr;
   int layer = 0;
   int q_heads = 0;
+  int64_t sink_rows = 0;   // first rows that a windowed attention still sees
   // standalone KV owns its pool and sequence
   std::unique_ptr<Pool> owned_pool;
   std::unique_ptr<Seq> owned_seq;
@@ -232,6 +248,7 @@ struct Batch {
   int choose_splits(int kernel, int64_t max_rows) const;
   int enqueue_append(cudaStream_t stream, const float* d_k, const float* d_v, int n_rows, const RopeArgs* rope,
                      const float* knorm_w);
+  int enqueue_truncate(cudaStream_t stream, const int64_t* lens);
   int enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out, int64_t window_start,
                         int64_t sliding_window, float attn_scalar, const float* d_k_new, const float* d_v_new);
   ~Batch();

@@ -184,15 +184,25 @@ void Seq::new_epoch() {
   epoch = ++counter;
 }
 
-int Seq::release_before(int64_t row) {
-  int64_t upto = std::min<int64_t>(row / PAGE_TOKENS, static_cast<int64_t>(pages.size()));
-  for (int64_t i = released_pages; i < upto; ++i) {
-    if (pages[i] >= 0) pool->release(pages[i]);
-    pages[i] = -1;
+int Seq::release_between(int64_t first_row, int64_t row) {
+  const int64_t have = static_cast<int64_t>(pages.size());
+  int64_t first = std::min((first_row + PAGE_TOKENS - 1) / PAGE_TOKENS, have);
+  int64_t upto = std::min<int64_t>(row / PAGE_TOKENS, have);
+  if (upto > first && released_pages > released_first) {
+    // what has been returned stays one range: it grows at either end
+    if (first > released_pages || upto < released_first)
+      return fail(SGK_ERR_DIMENSION, "release of rows [%lld,%lld) leaves rows between them and those already returned",
+                  (long long)first_row, (long long)row);
+    first = std::min(first, released_first);
+    upto = std::max(upto, released_pages);
   }
-  if (upto > released_pages) {
+  if (upto > first && (first != released_first || upto != released_pages)) {
+    for (int64_t i = first; i < upto; ++i) {
+      if (pages[i] >= 0) pool->release(pages[i]);
+      pages[i] = -1;
+    }
     new_epoch();
-    int64_t first = released_pages;
+    released_first = first;
     released_pages = upto;
     SGK_TRY(publish(first, upto - first));
   }
@@ -205,7 +215,7 @@ int Seq::release_all() {
   for (auto& p : pages)
     if (p >= 0) pool->release(p);
   pages.clear();
-  released_pages = 0;
+  released_first = released_pages = 0;
   return SGK_OK;
 }
 
@@ -459,6 +469,27 @@ int Batch::enqueue_append(cudaStream_t stream, const float* d_k, const float* d_
   return SGK_OK;
 }
 
+int Batch::enqueue_truncate(cudaStream_t stream, const int64_t* lens) {
+  for (int i = 0; i < n(); ++i)
+    if (lens[i] < 0 || lens[i] > kvs[i]->seq->capacity)
+      return fail(SGK_ERR_DIMENSION, "truncate KV %lld > capacity %lld", (long long)lens[i], (long long)kvs[i]->seq->capacity);
+  for (int i = 0; i < n(); ++i) SGK_TRY(kvs[i]->seq->reserve(lens[i]));
+  SetLensArgs a{};
+  a.lens = pool->d_lens;
+  a.layers = pool->layers;
+  a.layer = layer;
+  for (int done = 0; done < n(); done += SET_LENS_MAX) {
+    a.n = std::min(n() - done, SET_LENS_MAX);
+    a.slots = n() == 1 ? nullptr : d_slots + done;
+    a.slot0 = kvs[0]->seq->slot;
+    for (int i = 0; i < a.n; ++i) a.value[i] = static_cast<int32_t>(lens[done + i]);
+    SGK_CUDA(launch_set_lens(a, stream));
+    st->launches += 1;
+  }
+  for (int i = 0; i < n(); ++i) kvs[i]->seq->len[layer] = lens[i];
+  return SGK_OK;
+}
+
 int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out, int64_t window_start,
                              int64_t sliding_window, float attn_scalar, const float* d_k_new,
                              const float* d_v_new) {
@@ -467,6 +498,8 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   int kernel = choose_kernel();
   if (kernel < 0) return fail(SGK_ERR_BACKEND, "tensor-core attention kernel does not take this shape");
   int64_t max_rows = 0;
+  const int64_t sink_rows = kvs[0]->sink_rows;
+  if (sink_rows > 0 && (sliding_window > 0 || window_start > 0)) kernel = 1;
   for (Kv* kv : kvs) {
     int64_t len_after = kv->len() + (fused ? 1 : 0);
     if (fused && kv->len() >= kv->seq->capacity)
@@ -476,9 +509,11 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     if (ws < 0 || ws >= len_after)
       return fail(SGK_ERR_DIMENSION, "attention_decode empty window: start=%lld, len=%lld", (long long)ws,
                   (long long)len_after);
-    if (ws / PAGE_TOKENS < kv->seq->released_pages)
+    if (kv->sink_rows != sink_rows) return fail(SGK_ERR_CONFIG, "batch members must share the number of attention sinks");
+    const SinkSpan sinks(sink_rows, ws);
+    if (kv->seq->released(ws / PAGE_TOKENS, (len_after + PAGE_TOKENS - 1) / PAGE_TOKENS) || kv->seq->released(0, sinks.pages))
       return fail(SGK_ERR_DIMENSION, "attention window reaches rows released by the sliding window");
-    max_rows = std::max(max_rows, len_after - ws);
+    max_rows = std::max(max_rows, len_after - ws + sinks.pages * PAGE_TOKENS);
   }
   if (fused && kernel < 2) {
     SGK_TRY(enqueue_append(stream, d_k_new, d_v_new, 1, nullptr, nullptr));
@@ -498,6 +533,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   a.out = d_out;
   a.window_start = window_start;
   a.sliding_window = sliding_window;
+  a.sink_rows = sink_rows;
   float scalar = attn_scalar > 0.0f ? attn_scalar : static_cast<float>(pool->head_dim);
   a.scale_log2e = 1.4426950408889634f / std::sqrt(scalar);
   const bool chained = st->chain_member(stream) && kernel >= 2;
@@ -510,8 +546,8 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     int64_t lo = INT64_MAX, hi = 0, total = 0;
     for (Kv* kv : kvs) {
       int64_t rows = kv->len() + (fused ? 1 : 0);
-      if (sliding_window > 0) rows = std::min<int64_t>(rows, sliding_window + PAGE_TOKENS);
-      else rows -= std::min<int64_t>(rows, window_start);
+      if (sliding_window > 0) rows = std::min<int64_t>(rows, sliding_window + PAGE_TOKENS + sink_rows);
+      else rows -= std::min<int64_t>(rows, window_start) - SinkSpan(sink_rows, std::min<int64_t>(rows, window_start)).rows;
       const int64_t pages = (rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
       lo = std::min(lo, pages), hi = std::max(hi, pages), total += pages;
     }

@@ -54,6 +54,7 @@ struct AttnArgs {
   float* out;            // [n_seq][q_heads*head_dim]
   int64_t window_start;     // explicit start row when sliding_window == 0
   int64_t sliding_window;   // > 0: start = max(len - window, 0)
+  int64_t sink_rows;        // rows [0, sink_rows) stay visible beside [start, len)
   int32_t shared_merge;     // 1: every block of a (sequence, KV head) merges a slice once all have arrived
                             //    (a cooperative launch); 2: the same as an ordinary launch
   int32_t cluster_merge;    // 1: the splits of a (sequence, KV head) are one thread-block cluster and merge through
@@ -103,6 +104,16 @@ cudaError_t launch_append_rows(const AppendArgs& a, int n_seq, cudaStream_t stre
 // Writes `value` into n consecutive int32 words (cursors, block-table entries), in stream order.
 cudaError_t launch_set_len(int32_t* ptr, int32_t value, cudaStream_t stream, int n = 1);
 
+// The cursors of several sequences at once: lens[slots[i]][layer] = value[i].
+constexpr int SET_LENS_MAX = 512;
+struct SetLensArgs {
+  int32_t* lens;
+  const int32_t* slots;   // NULL: slot0
+  int32_t slot0, layers, layer, n;
+  int32_t value[SET_LENS_MAX];
+};
+cudaError_t launch_set_lens(const SetLensArgs& a, cudaStream_t stream);
+
 cudaError_t launch_attention_generic(const AttnArgs& a, int n_seq, cudaStream_t stream);
 // Tensor-core paged kernel: bf16 pages, head_dim 128 or 256, q_heads/kv_heads <= 8.
 bool attention_mma_supported(int dtype, int head_dim, int gqa);
@@ -123,7 +134,7 @@ int attention_u8_resident_blocks(int head_dim, int n_stages);
 int attention_u8_max_clusters(int head_dim, int n_stages, int splits);
 
 // Gather rows [row0, row0+n) of one layer into contiguous [n, kv_dim] arrays.
-// mode 0: storage type (f32 / bf16 bits), 1: decoded f32, 2: u8 codes + scale + bias.
+// mode 0: storage type (f32 / bf16 bits), 1: decoded f32, 2: u8 or u4 codes (a byte each) + scale + bias.
 struct GatherArgs {
   PoolView pool;
   int32_t layer;

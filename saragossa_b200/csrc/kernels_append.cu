@@ -1,10 +1,11 @@
 // KV append: f32 K/V rows -> (optional RMSNorm + RoPE on K) -> storage type
-// (f32 / bf16 RNE / u8 group-32) -> scattered into the page the block table
+// (f32 / bf16 RNE / u8 or u4 group-32) -> scattered into the page the block table
 // names. One block per (kv head, row, sequence). Replaces the reference's
 // copy_at_f32 / copy_at_f32_to_bf16 dispatches (src/decode_resident/kernels.rs:1026-1044),
 // the host f32->bf16 loop of seed/append_row (src/decode_resident/utils.rs:76-110)
 // and, when fused, rms_norm_rope_heads_decode_f32 (kernels.rs:975-1024).
 #include "kernels.h"
+#include "u4_quant.cuh"
 
 namespace sgk {
 
@@ -141,8 +142,13 @@ __global__ void __launch_bounds__(128) append_rows_kernel(AppendArgs a) {
     const int rin = static_cast<int>(row % PAGE_TOKENS);
     uint8_t* ktile = a.pool.base + tile_offset(a.pool, page, a.layer, head, 0);
     uint8_t* vtile = a.pool.base + tile_offset(a.pool, page, a.layer, head, 1);
-    store_head_row(ktile, a.pool.dtype, hd, 0, rin, ks, a.pool.scale_max);
-    store_head_row(vtile, a.pool.dtype, hd, 1, rin, vs, a.pool.scale_max);
+    if (a.pool.dtype == KV_U4G32) {
+      // a warp per head row: the step of a group depends on the widest group of its row
+      if (tid < 64) u4_store_row(ktile, vtile, hd, tid >> 5, rin, tid < 32 ? ks : vs, tid & 31);
+    } else {
+      store_head_row(ktile, a.pool.dtype, hd, 0, rin, ks, a.pool.scale_max);
+      store_head_row(vtile, a.pool.dtype, hd, 1, rin, vs, a.pool.scale_max);
+    }
   } else if (tid == 0) {
     atomicExch(a.status, DEV_ERR_BAD_PAGE);
   }
@@ -515,7 +521,7 @@ cudaError_t launch_rope_table(float2* table, int64_t row0, int n_rows, const Rop
 
 cudaError_t launch_append_rows(const AppendArgs& a, int n_seq, cudaStream_t stream) {
   const int hd = a.pool.head_dim;
-  if (a.n_rows >= 4 && a.out_k == nullptr && (hd == 64 || hd == 128 || hd == 256)) {
+  if (a.n_rows >= 4 && a.out_k == nullptr && (hd == 64 || hd == 128 || hd == 256) && a.pool.dtype != KV_U4G32) {
     // bulk: one block per page tile; the first row may sit anywhere in its page, so one tile more
     dim3 grid(a.pool.kv_heads, (a.n_rows + PAGE_TOKENS - 1) / PAGE_TOKENS + 1, n_seq);
     // the kernel's carve-up: K rows, 1/rms per row, rope denominators (<= 128 pairs); V rows and a
@@ -529,6 +535,17 @@ cudaError_t launch_append_rows(const AppendArgs& a, int n_seq, cudaStream_t stre
   dim3 grid(a.pool.kv_heads, a.n_rows, n_seq);
   size_t smem = (2 * size_t(a.pool.head_dim) + 4) * sizeof(float);
   append_rows_kernel<<<grid, 128, smem, stream>>>(a);
+  return cudaGetLastError();
+}
+
+// lens[slots[i]][layer] = value[i]: the cursors of a batch, in stream order
+__global__ void set_lens_kernel(SetLensArgs a) {
+  const int i = threadIdx.x;
+  if (i < a.n) a.lens[int64_t(a.slots ? a.slots[i] : a.slot0) * a.layers + a.layer] = a.value[i];
+}
+
+cudaError_t launch_set_lens(const SetLensArgs& a, cudaStream_t stream) {
+  set_lens_kernel<<<1, SET_LENS_MAX, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

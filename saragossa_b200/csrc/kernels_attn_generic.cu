@@ -29,9 +29,12 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
   const int64_t len = a.pool.lens[int64_t(slot) * a.pool.layers + a.layer];
   int64_t ws = a.sliding_window > 0 ? (len > a.sliding_window ? len - a.sliding_window : 0) : a.window_start;
   if (ws > len) ws = len;
-  const int64_t n = len - ws;
-  const int64_t r0 = ws + (n * split) / a.splits;
-  const int64_t r1 = ws + (n * (split + 1)) / a.splits;
+  // visible rows: `sinks` at the head, then [ws, len); i counts them, row i + (i < sinks ? 0 : gap)
+  const int64_t sinks = a.sink_rows < ws ? a.sink_rows : ws;
+  const int64_t gap = ws - sinks;
+  const int64_t n = len - gap;
+  const int64_t i0 = (n * split) / a.splits;
+  const int64_t i1 = (n * (split + 1)) / a.splits;
   const int32_t* table = a.pool.tables + int64_t(slot) * a.pool.table_stride;
 
   const float* q = a.q + (int64_t(seq) * a.q_heads + qh) * hd;
@@ -43,7 +46,8 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
 #pragma unroll
   for (int j = 0; j < GEN_MAXJ; ++j) acc[j] = 0.0f;
 
-  for (int64_t r = r0 + warp; r < r1; r += GEN_WARPS) {
+  for (int64_t i = i0 + warp; i < i1; i += GEN_WARPS) {
+    const int64_t r = i < sinks ? i : i + gap;
     int32_t page = table[r / PAGE_TOKENS];
     if (page < 0 || page >= a.num_pages) {
       if (lane == 0) atomicExch(a.status, DEV_ERR_BAD_PAGE);

@@ -50,6 +50,18 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(GatherArgs a) {
       int e = bf16_elem_index(rin, dim, hd);
       reinterpret_cast<uint16_t*>(a.k_out)[i] = reinterpret_cast<const uint16_t*>(kt)[e];
       reinterpret_cast<uint16_t*>(a.v_out)[i] = reinterpret_cast<const uint16_t*>(vt)[e];
+    } else if (a.pool.dtype == KV_U4G32) {
+      reinterpret_cast<uint8_t*>(a.k_out)[i] = static_cast<uint8_t>(u4_code(kt, hd, 0, rin, dim));
+      reinterpret_cast<uint8_t*>(a.v_out)[i] = static_cast<uint8_t>(u4_code(vt, hd, 1, rin, dim));
+      if (dim % QGROUP == 0) {
+        const int64_t gi = r * (kv_dim / QGROUP) + col / QGROUP;
+        const int grp = dim / QGROUP;
+        // steps are bf16 values, V steps once they are multiplied by their row's power of two again
+        a.k_scale[gi] = static_cast<uint16_t>(__float_as_uint(u4_step(kt, hd, 0, rin, grp)) >> 16);
+        a.k_bias[gi] = *reinterpret_cast<const uint16_t*>(kt + u4_bias_offset(rin, grp, hd));
+        a.v_scale[gi] = static_cast<uint16_t>(__float_as_uint(u4_step(vt, hd, 1, rin, grp)) >> 16);
+        a.v_bias[gi] = *reinterpret_cast<const uint16_t*>(vt + u4_bias_offset(rin, grp, hd));
+      }
     } else {
       reinterpret_cast<uint8_t*>(a.k_out)[i] = kt[u8_k_code_index(rin, dim, hd)];
       reinterpret_cast<uint8_t*>(a.v_out)[i] = vt[u8_v_code_index(rin, dim, hd)];

@@ -23,6 +23,13 @@
 //          consecutive 16-dim steps are two 16-byte loads, see u8_v_code_index. After the
 //          codes: the bf16 scales [row][group], then the bf16 biases, [row][group] for K
 //          and [group][row] for V (the order the tensor-core bias products read them in).
+//   u4   : one byte holds the codes of dims p (low nibble) and p + 16 (high nibble) of one row and
+//          group, p = 0 .. 15. K bytes lie row by row in the order a lane of the tensor-core kernel
+//          reads them (u4_k_byte), V bytes dim by dim, four rows of a lane in one word (u4_v_byte).
+//          Then 2 bytes per (row, group) of step: for K the bf16 step [row][group], for V the step
+//          divided by the row's power of two, as fp16, ordered [row / 8][row / 2 % 4][group][row % 2];
+//          then the bf16 biases [row][group]; then 16 bytes with eight bf16 powers of two: those of
+//          V rows 0-7 end the K tile, those of rows 8-15 end the V tile.
 #pragma once
 #include <stdint.h>
 
@@ -36,15 +43,18 @@ namespace sgk {
 
 constexpr int PAGE_TOKENS = 16;
 constexpr int QGROUP = 32;
-enum : int32_t { KV_F32 = 0, KV_BF16 = 1, KV_U8G32 = 2 };
+enum : int32_t { KV_F32 = 0, KV_BF16 = 1, KV_U8G32 = 2, KV_U4G32 = 3 };
 
 SGK_HD int64_t tile_code_bytes(int dtype, int hd) {
   return dtype == KV_F32 ? int64_t(PAGE_TOKENS) * hd * 4
          : dtype == KV_BF16 ? int64_t(PAGE_TOKENS) * hd * 2
-                            : int64_t(PAGE_TOKENS) * hd;
+         : dtype == KV_U8G32 ? int64_t(PAGE_TOKENS) * hd
+                             : int64_t(PAGE_TOKENS) * hd / 2;
 }
 SGK_HD int64_t tile_bytes(int dtype, int hd) {
-  int64_t meta = dtype == KV_U8G32 ? int64_t(PAGE_TOKENS) * (hd / QGROUP) * 4 : 0;
+  int64_t meta = dtype == KV_U8G32   ? int64_t(PAGE_TOKENS) * (hd / QGROUP) * 4
+                 : dtype == KV_U4G32 ? int64_t(PAGE_TOKENS) * (hd / QGROUP) * 4 + PAGE_TOKENS
+                                     : 0;
   return tile_code_bytes(dtype, hd) + meta;
 }
 // Bytes one stored row of one head occupies (reported as the storage size).
@@ -110,6 +120,45 @@ SGK_HD int u8_bias_offset(int is_v, int row, int group, int hd) {
   const int groups = hd / QGROUP;
   return PAGE_TOKENS * hd + PAGE_TOKENS * groups * 2 +
          (is_v ? group * PAGE_TOKENS + row : row * groups + group) * 2;
+}
+
+// ---- u4 tiles --------------------------------------------------------------------------------
+// Byte that holds the K code of (row, dim); the nibble is u4_nibble(dim). A lane (g, t) of the matrix
+// instruction reads, for row g, the bytes p = 4t .. 4t+3 of four groups with one 16-byte load; with
+// more than one set of four groups the sets of odd rows change places, so that the eight lanes a
+// shared-memory pass serves touch different banks.
+SGK_HD int u4_nibble(int dim) { return (dim >> 4) & 1; }
+SGK_HD int u4_k_byte(int row, int dim, int hd) {
+  const int grp = dim >> 5, p = dim & 15;
+  if (hd % 128 != 0) return row * (hd / 2) + grp * 16 + p;
+  int set = grp >> 2;
+  if (hd % 256 == 0) set ^= row & 1;
+  return row * (hd / 2) + set * 64 + (p >> 2) * 16 + (grp & 3) * 4 + (p & 3);
+}
+// Byte that holds the V code of (row, dim). The word of lane (g, t) for (group, half): dims p = g +
+// 8 * half (and p + 16), its bytes rows 2t, 2t+8, 2t+1, 2t+9: the low bytes of its two 16-bit halves
+// are one register of the matrix instruction's A fragment, the high bytes another. A lane's four
+// words of two groups are one 16-byte load.
+SGK_HD int u4_v_byte(int row, int dim, int hd) {
+  const int grp = dim >> 5, p = dim & 15;
+  if (hd % 64 != 0) return (grp * 16 + p) * PAGE_TOKENS + row;
+  const int lane = (p & 7) * 4 + ((row & 7) >> 1);
+  const int word = ((grp >> 1) * 32 + lane) * 4 + (grp & 1) * 2 + (p >> 3);
+  return word * 4 + (row & 1) * 2 + (row >> 3);
+}
+// Byte offsets inside a u4 tile.
+SGK_HD int u4_step_offset(int is_v, int row, int group, int hd) {
+  const int groups = hd / QGROUP;
+  return PAGE_TOKENS * hd / 2 +
+         (is_v ? (((row >> 3) * 4 + ((row & 7) >> 1)) * groups + group) * 2 + (row & 1) : row * groups + group) * 2;
+}
+SGK_HD int u4_bias_offset(int row, int group, int hd) {
+  const int groups = hd / QGROUP;
+  return PAGE_TOKENS * hd / 2 + (PAGE_TOKENS * groups + row * groups + group) * 2;
+}
+// Power of two of V row `row`, relative to the tile that holds it: the K tile (row < 8) or the V tile.
+SGK_HD int u4_pow_offset(int row, int hd) {
+  return PAGE_TOKENS * hd / 2 + PAGE_TOKENS * (hd / QGROUP) * 4 + (row & 7) * 2;
 }
 
 }  // namespace sgk

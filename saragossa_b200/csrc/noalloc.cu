@@ -118,7 +118,8 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   if (window_start < 0 || window_start >= len)
     return fail(SGK_ERR_DIMENSION, "attention_decode empty window: start=%lld, len=%lld", (long long)window_start,
                 (long long)len);
-  if (window_start / PAGE_TOKENS < kv->seq->released_pages)
+  const SinkSpan sinks(kv->sink_rows, window_start);
+  if (kv->seq->released(window_start / PAGE_TOKENS, (len + PAGE_TOKENS - 1) / PAGE_TOKENS) || kv->seq->released(0, sinks.pages))
     return fail(SGK_ERR_DIMENSION, "attention window reaches rows released by the sliding window");
 
   // The state's device is current for every call (not only for the first one, which resolves the
@@ -130,11 +131,11 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
 
   // the same kernel selection as the allocating entry point: tensor-core kernels over bf16 and over
   // u8 group-32 pages, the generic kernel for everything else
-  const bool u8 = attention_u8_supported(pool->dtype, hd, qh / kvh);
-  const bool mma = u8 || attention_mma_supported(pool->dtype, hd, qh / kvh);
+  const bool u8 = sinks.rows == 0 && attention_u8_supported(pool->dtype, hd, qh / kvh);
+  const bool mma = u8 || (sinks.rows == 0 && attention_mma_supported(pool->dtype, hd, qh / kvh));
   // split count: fill the SMs (two blocks each for the tensor-core kernel, eight for the
   // generic one), keep a few pages per split, and stay inside the static workspace
-  const int64_t pages = (len - window_start + PAGE_TOKENS - 1) / PAGE_TOKENS;
+  const int64_t pages = (len - window_start + PAGE_TOKENS - 1) / PAGE_TOKENS + sinks.pages;
   const int64_t units = mma ? kvh : qh;
   const int64_t slots = int64_t(st->sm_count) * (mma ? 2 : 8);
   int64_t splits = std::max<int64_t>(1, slots / units);
@@ -166,6 +167,7 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   a.out = d_out;
   a.window_start = window_start;
   a.sliding_window = 0;
+  a.sink_rows = kv->sink_rows;
   const float scalar = attn_scalar > 0.0f ? attn_scalar : static_cast<float>(hd);
   a.scale_log2e = 1.4426950408889634f / std::sqrt(scalar);
   a.splits = static_cast<int>(splits);

@@ -1,0 +1,131 @@
+// The 4-bit quantiser shared by the append kernels and the fused append of the attention kernel.
+//
+// A head row is cut into groups of 32 values. Rows at odd positions are quantised negated (y = -x): V
+// rows are summed with weights p, and codes that all count up from a minimum would make that sum a
+// large number minus a large number; with the sign alternating from row to row neighbouring rows
+// cancel inside one matrix instruction and the f32 accumulator keeps its digits.
+//   bias = bf16(min y),  step = bf16(max((max y - bias) / 15, 2^-40, 2^(e-16))),
+//   2^e = the power of two at or below the largest (max y - bias) / 15 of the head row (at least 2^-40),
+//   code = nearest((y - bias) / step), ties to even, kept within 0..15;
+//   stored: the codes, (-1)^row * step and (-1)^row * bias.
+// The floor 2^(e-16) lets V keep step / 2^e as an fp16 number without loss.
+//
+// Each rounding is of the exact value, although everything runs in f32: a difference a - b comes with
+// its rounding error (two-difference), multiples of a bf16 step by a number below 16 and of a 9-bit
+// midpoint by 15 are exact, and so are the remainders they leave. A division that is rounded to f32
+// first and to bf16 afterwards picks the wrong neighbour about once in 2^15 groups.
+//
+// A group that holds an infinity or a NaN, or whose bias or step is not finite, reads back as NaN.
+#pragma once
+#include "device_common.cuh"
+
+namespace sgk {
+
+constexpr int U4_EXP_MIN = -40;   // smallest step 2^-40
+
+// a - b = d + err exactly
+__device__ __forceinline__ float two_diff(float a, float b, float& err) {
+  const float d = __fsub_rn(a, b);
+  const float z = __fsub_rn(d, a);
+  err = __fsub_rn(__fsub_rn(a, __fsub_rn(d, z)), __fadd_rn(b, z));
+  return d;
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // -126..127
+
+// What the values of one group say of it: bias, width = max y - bias as a pair, exponent of width / 15.
+struct U4Range {
+  float bias, width, err;
+  int exponent;   // U4_EXP_MIN .. 127
+  bool finite;
+};
+__device__ __forceinline__ U4Range u4_range(float lo, float hi) {
+  U4Range r;
+  r.bias = bf16_bits_to_f32(f32_to_bf16_bits(lo));
+  r.width = two_diff(hi, r.bias, r.err);
+  r.finite = fabsf(r.bias) < INFINITY && r.width < INFINITY;
+  r.exponent = U4_EXP_MIN;
+  if (r.finite && r.width > 0x1p-37f) {   // 15 * 2^-40 < 2^-36: below that the floor of the exponent stands
+    int e = static_cast<int>(__float_as_uint(r.width * (1.0f / 15.0f)) >> 23) - 127;
+    const float at = 15.0f * pow2f(e);
+    if (r.width < at || (r.width == at && r.err < 0.0f)) e -= 1;
+    else if (r.width > 2.0f * at || (r.width == 2.0f * at && r.err >= 0.0f)) e += 1;
+    r.exponent = max(e, U4_EXP_MIN);
+  }
+  return r;
+}
+// bf16 bits of the (positive) step of a group; row_exponent = the largest exponent of the head row.
+__device__ __forceinline__ uint16_t u4_step_bits(const U4Range& r, int row_exponent) {
+  if (!r.finite) return 0x7fc0;
+  const float floor_step = pow2f(max(row_exponent - 16, U4_EXP_MIN));
+  const float at = 15.0f * floor_step;
+  if (r.width < at || (r.width == at && r.err <= 0.0f)) return static_cast<uint16_t>(__float_as_uint(floor_step) >> 16);
+  const uint32_t low = __float_as_uint(r.width * (1.0f / 15.0f)) & 0xffff0000u;
+  const float mid = 15.0f * __uint_as_float(low | 0x8000u);   // the border to the next bf16 value, times 15
+  const bool up = r.width > mid || (r.width == mid && (r.err > 0.0f || (r.err == 0.0f && (low & 0x10000u))));
+  return static_cast<uint16_t>((low >> 16) + (up ? 1u : 0u));
+}
+// Code of y; inv ~ 1 / step (an error of a few units in the last place is mended below).
+__device__ __forceinline__ uint32_t u4_code_of(float y, float bias, float step, float inv) {
+  const float t = __fsub_rn(y, bias);
+  const float guess = fminf(fmaxf(t * inv, 0.0f), 15.0f) + 12582912.0f;   // 1.5 * 2^23: rounds to a whole number
+  int code = static_cast<int>(__float_as_uint(guess) & 15u);
+  const float rest = fmaf(-(guess - 12582912.0f), step, t);   // exact
+  const float half = 0.5f * step;
+  if (fabsf(rest) >= half) {   // at a border, or past it: rare
+    float err;
+    two_diff(y, bias, err);
+    const bool tie_moves = err == 0.0f && (code & 1);
+    if (rest > half || (rest == half && (err > 0.0f || tie_moves))) code += 1;
+    else if (rest < -half || (rest == -half && (err < 0.0f || tie_moves))) code -= 1;
+    code = min(max(code, 0), 15);
+  }
+  return static_cast<uint32_t>(code);
+}
+// fp16 bits of step / 2^row_exponent, with the row's sign: exact (8 significant bits, >= 2^-16).
+__device__ __forceinline__ uint16_t u4_v_factor_bits(uint16_t step_bits, int row_exponent, uint32_t odd) {
+  if (step_bits == 0x7fc0) return 0x7e00;
+  const float f = bf16_bits_to_f32(step_bits) * pow2f(-row_exponent);
+  return static_cast<uint16_t>(__half_as_ushort(__float2half_rn(f)) | (odd << 15));
+}
+__device__ __forceinline__ void warp_min_max(float x, float& lo, float& hi) {
+  asm("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(x));
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(x));
+}
+
+// Quantises and stores one head row of `hd` values (xs, shared memory) as row `row` of a u4 tile; one
+// whole warp. ktile / vtile: the K tile and the V tile behind it.
+__device__ __forceinline__ void u4_store_row(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, const float* xs, int lane) {
+  uint8_t* tile = is_v ? vtile : ktile;
+  const uint32_t odd = row & 1;
+  const float sign = odd ? -1.0f : 1.0f;
+  const int groups = hd / QGROUP;
+  int row_exponent = U4_EXP_MIN;
+  for (int g = 0; g < groups; ++g) {
+    float lo, hi;
+    warp_min_max(sign * xs[g * QGROUP + lane], lo, hi);
+    row_exponent = max(row_exponent, u4_range(lo, hi).exponent);
+  }
+  for (int g = 0; g < groups; ++g) {
+    const float y = sign * xs[g * QGROUP + lane];
+    float lo, hi;
+    warp_min_max(y, lo, hi);
+    const U4Range r = u4_range(lo, hi);
+    const uint16_t step_bits = u4_step_bits(r, row_exponent);
+    const float step = bf16_bits_to_f32(step_bits);
+    const uint32_t code = r.finite ? u4_code_of(y, r.bias, step, 1.0f / step) : 0u;
+    const uint32_t high = __shfl_down_sync(0xffffffffu, code, 16);
+    const int dim = g * QGROUP + lane;
+    if (lane < 16) tile[is_v ? u4_v_byte(row, dim, hd) : u4_k_byte(row, dim, hd)] = static_cast<uint8_t>(code | (high << 4));
+    if (lane == 0) {
+      *reinterpret_cast<uint16_t*>(tile + u4_step_offset(is_v, row, g, hd)) =
+          is_v ? u4_v_factor_bits(step_bits, row_exponent, odd) : static_cast<uint16_t>(step_bits ^ (odd << 15));
+      *reinterpret_cast<uint16_t*>(tile + u4_bias_offset(row, g, hd)) =
+          static_cast<uint16_t>(r.finite ? (__float_as_uint(sign * r.bias) >> 16) : 0u);
+    }
+  }
+  if (is_v && lane == 0)
+    *reinterpret_cast<uint16_t*>((row < 8 ? ktile : vtile) + u4_pow_offset(row, hd)) =
+        static_cast<uint16_t>(__float_as_uint(pow2f(row_exponent)) >> 16);
+}
+
+}  // namespace sgk

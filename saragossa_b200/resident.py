@@ -17,7 +17,7 @@ import numpy as np
 
 from . import _ffi
 
-KV_F32, KV_BF16, KV_U8G32 = 0, 1, 2
+KV_F32, KV_BF16, KV_U8G32, KV_U4G32 = 0, 1, 2, 3
 PAGE_TOKENS = 16
 _KINDS = {1: "Dimension", 2: "Config", 3: "Backend", 4: "MemoryGuard", 5: "Shape", 6: "Timeout"}
 
@@ -469,6 +469,10 @@ class Sequence:
     def release_before(self, row):
         check(self.L.sgk_seq_release_before(self.h, row))
 
+    def release_between(self, first_row, row):
+        """Returns the pages wholly inside rows [first_row, row): the rows between the attention sinks and a window."""
+        check(self.L.sgk_seq_release_between(self.h, first_row, row))
+
     def layer(self, layer, q_heads):
         h = C.c_void_p()
         check(self.L.sgk_seq_layer(self.h, layer, q_heads, C.byref(h)))
@@ -523,6 +527,17 @@ class FullAttentionState:
 
     def truncate(self, n):
         check(self.L.sgk_kv_truncate(self.h, n))
+
+    def encode_truncate(self, n, stream=None):
+        """truncate in stream order, without waiting."""
+        check(self.L.sgk_kv_enqueue_truncate(self.h, stream, n))
+
+    def set_attention_sinks(self, rows):
+        """The first `rows` rows stay visible to every windowed attention over this state."""
+        check(self.L.sgk_kv_set_attention_sinks(self.h, rows))
+
+    def attention_sinks(self):
+        return self.L.sgk_kv_attention_sinks(self.h)
 
     def seed(self, keys_rows, values_rows, n_rows):
         k, v = _f32(keys_rows).ravel(), _f32(values_rows).ravel()
@@ -582,7 +597,7 @@ class FullAttentionState:
 
     def _gather(self, row0, n):
         n = self.len() - row0 if n is None else n
-        dt = {KV_F32: np.float32, KV_BF16: np.uint16}[self.dtype()]
+        dt = {KV_F32: np.float32, KV_BF16: np.uint16}.get(self.dtype(), np.uint8)   # refused below
         k = np.empty((n, self.kv_dim()), dt)
         v = np.empty((n, self.kv_dim()), dt)
         check(self.L.sgk_kv_gather_rows(self.h, row0, n, _ptr(k), _ptr(v)))
@@ -605,12 +620,25 @@ class FullAttentionState:
         check(self.L.sgk_kv_gather_rows_f32(self.h, row0, n, _ptr(k), _ptr(v)))
         return k, v
 
+    def encode_gather_rows_f32(self, d_k: DeviceBuffer, d_v: DeviceBuffer, row0=0, n=None, stream=None):
+        """The decoded rows [row0, row0 + n) into device buffers, [n][kv_dim] f32 each; enqueue only."""
+        n = self.len() - row0 if n is None else n
+        check(self.L.sgk_kv_enqueue_gather_rows_f32(self.h, stream, row0, n, d_k.ptr, d_v.ptr))
+
     def gather_rows_u8(self, row0=0, n=None):
+        """K codes, scales, biases and the same of V of u8 group-32 pages (scales and biases as bf16 bit patterns)."""
+        return self._gather_codes(self.L.sgk_kv_gather_rows_u8, row0, n)
+
+    def gather_rows_u4(self, row0=0, n=None):
+        """The same of u4 group-32 pages, one code per byte; the scales of rows at odd positions are negative."""
+        return self._gather_codes(self.L.sgk_kv_gather_rows_u4, row0, n)
+
+    def _gather_codes(self, gather, row0, n):
         n = self.len() - row0 if n is None else n
         d, g = self.kv_dim(), self.kv_dim() // 32
         out = [np.empty((n, d), np.uint8), np.empty((n, g), np.uint16), np.empty((n, g), np.uint16),
                np.empty((n, d), np.uint8), np.empty((n, g), np.uint16), np.empty((n, g), np.uint16)]
-        check(self.L.sgk_kv_gather_rows_u8(self.h, row0, n, *[_ptr(a) for a in out]))
+        check(gather(self.h, row0, n, *[_ptr(a) for a in out]))
         return out
 
     def block_table(self):
@@ -642,6 +670,13 @@ class Batch:
 
     def enqueue_append(self, d_k, d_v, stream=None):
         check(self.L.sgk_batch_enqueue_append(self.h, stream, d_k.ptr, d_v.ptr))
+
+    def enqueue_truncate(self, lens, stream=None):
+        """Moves every member's cursor, in stream order: lens[i] rows stay of sequence i."""
+        arr = np.ascontiguousarray(lens, dtype=np.int64)
+        if arr.shape != (len(self.kvs),):
+            raise InferError(1, f"truncate: {arr.shape} lengths for {len(self.kvs)} sequences")
+        check(self.L.sgk_batch_enqueue_truncate(self.h, stream, _ptr(arr)))
 
     def enqueue_attention(self, d_q, d_out, sliding_window=0, attn_scalar=0.0, stream=None):
         check(self.L.sgk_batch_enqueue_attention(self.h, stream, d_q.ptr, d_out.ptr, sliding_window, attn_scalar))
