@@ -56,6 +56,7 @@ int32_t sgk_state_create(int32_t device, sgk_state** out) {
   SGK_CUDA(cudaMemset(st->d_lm_ws, 0, 9 * sizeof(unsigned long long)));
   SGK_CUDA(attention_mma_configure());
   SGK_CUDA(attention_u8_configure());
+  SGK_CUDA(attention_u4_configure());
   *out = st.release();
   return SGK_OK;
 }

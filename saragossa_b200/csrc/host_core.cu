@@ -337,9 +337,10 @@ int create_batch(State* st, Kv** kvs, int n, Batch** out) {
 
 int Batch::choose_kernel() const {
   int gqa = q_heads / pool->kv_heads;
-  // 1 = generic CUDA-core kernel, 2 = tensor-core kernel over bf16 pages, 3 = over u8 pages
+  // 1 = generic CUDA-core kernel, 2 = tensor-core kernel over bf16 pages, 3 = over u8 pages, 4 = over u4 pages
   int tensor = attention_mma_supported(pool->dtype, pool->head_dim, gqa)  ? 2
                : attention_u8_supported(pool->dtype, pool->head_dim, gqa) ? 3
+               : attention_u4_supported(pool->dtype, pool->head_dim, gqa) ? 4
                                                                           : 0;
   if (kernel_override == 2 && tensor == 0) return -1;
   if (kernel_override == 1) return 1;
@@ -499,7 +500,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   if (kernel < 0) return fail(SGK_ERR_BACKEND, "tensor-core attention kernel does not take this shape");
   int64_t max_rows = 0;
   const int64_t sink_rows = kvs[0]->sink_rows;
-  if (sink_rows > 0 && (sliding_window > 0 || window_start > 0)) kernel = 1;
+  if (kernel != 4 && sink_rows > 0 && (sliding_window > 0 || window_start > 0)) kernel = 1;
   for (Kv* kv : kvs) {
     int64_t len_after = kv->len() + (fused ? 1 : 0);
     if (fused && kv->len() >= kv->seq->capacity)
@@ -587,6 +588,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       return e ? std::atoi(e) : 0;
     }();
     if (kernel == 3) a.n_stages = attention_u8_max_stages(pool->head_dim);
+    if (kernel == 4) a.n_stages = attention_u4_max_stages(pool->head_dim);
     if (env_stages >= 4 && env_stages <= a.n_stages) a.n_stages = env_stages / 4 * 4;
 #ifdef SGK_TRACE
     a.trace = g_trace;
@@ -603,7 +605,8 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     static const bool shared_merge_off = std::getenv("SGK_NO_SHARED_MERGE") != nullptr;
     if (!shared_merge_off && a.pages_per_split == 0 && a.splits > 12 && a.splits <= 160) {
       if (resident_per_sm < 0 || resident_stages != a.n_stages)   // asked once per batch
-        resident_per_sm = kernel == 3 ? attention_u8_resident_blocks(pool->head_dim, a.n_stages)
+        resident_per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim, a.n_stages)
+                          : kernel == 3 ? attention_u8_resident_blocks(pool->head_dim, a.n_stages)
                                       : attention_mma_resident_blocks(pool->head_dim, a.n_stages),
         resident_stages = a.n_stages;
       const int per_sm = resident_per_sm;
@@ -633,7 +636,8 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
         cluster_stages = a.n_stages;
       }
       if (max_clusters[a.splits] < 0)
-        max_clusters[a.splits] = kernel == 3 ? attention_u8_max_clusters(pool->head_dim, a.n_stages, a.splits)
+        max_clusters[a.splits] = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, a.n_stages, a.splits)
+                                 : kernel == 3 ? attention_u8_max_clusters(pool->head_dim, a.n_stages, a.splits)
                                              : attention_mma_max_clusters(pool->head_dim, a.n_stages, a.splits);
       a.cluster_merge = int64_t(pool->kv_heads) * n() <= max_clusters[a.splits];
     }
@@ -657,7 +661,9 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       a.exit_counter = ex->d_flags + ex->n_ranks + 1;
       peer_target_fused = true;
     }
-    if (kernel == 3) {
+    if (kernel == 4) {
+      SGK_CUDA(launch_attention_u4(a, n(), stream));
+    } else if (kernel == 3) {
       SGK_CUDA(launch_attention_u8(a, n(), stream));
     } else {
       SGK_CUDA(launch_attention_mma(a, n(), stream));

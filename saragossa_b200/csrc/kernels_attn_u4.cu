@@ -1,0 +1,690 @@
+// Paged split-K flash-decoding over u4 group-32 pages (head_dim 128 / 256, GQA group <= 8), with the
+// per-token append (quantisation included) fused in and with attention sinks beside the window.
+//
+// Same pipeline as the other paged kernels (producer warp, one bulk async copy per page into a
+// shared-memory ring, consumer warps, merge of the splits); a page is worth 5/16 of its bf16 bytes and
+// nearly the same products, so here the instructions count. What a page costs a warp:
+//
+//   codes    A byte holds two codes, n0 + 16 n1. Both go to the matrix instruction as fp16 subnormals:
+//            u = the byte (16 n1 + n0) * 2^-24 and r = (byte & 15) * 2^-24, one byte permute or mask each,
+//            four registers from a word with four instructions. Never separated further:
+//   scores   q_x n0 + q_y n1 = r (q_x - q_y / 16) + u (q_y / 16): the two dims of a byte share a k-slot and the
+//            query is prepared once per launch. Products per group of 32 dims, then in f32
+//              z[row][h] = 2^24 sum_g step_k[row][g] (sum_d codes q) + sum_g bias_k[row][g] qsum[h][g] + e[row],
+//            the bias sum as one bf16 product with qsum in three bf16 parts (24 bits);
+//   outputs  U[d][h] = sum_row u w, R[d][h] = sum_row r w; the low dim of a byte is R, the high one (U - R) / 16,
+//            taken once at the end. w = p * step_v as fp16 hi + lo (22 bits).
+//   softmax  a V row's steps are stored as f * 2^e with fp16 f (layout.h); 2^e joins the score, so the weight
+//            p'' = exp2(z - M) is bounded whatever the row's range, and w = p'' f needs no scaling. p = p'' 2^-e
+//            feeds the sum of the weights and the bias part of V. M is a reference, not the maximum: it moves only
+//            when a z exceeds it by more than 14 (then to 6 below the largest z), so a page costs one vote
+//            instead of the shuffles of a maximum, and p'' stays inside fp16.
+//
+// Rows of odd position are stored negated (u4_quant.cuh): without it U and R would be sums of codes that
+// all count up from a minimum, hundreds of times larger than the result under flat attention, and f32
+// would lose those digits.
+// q is scaled to a largest magnitude of 2^12..2^13 per head by a power of two, so any size of query keeps its 22 bits.
+//
+// The reference's KV has no 4-bit form; this kernel computes cached_attention_one
+// (src/decoder/attention_ops.rs:889-974) over the rows' values code * scale + bias.
+#include "mma_common.cuh"
+#include "u4_quant.cuh"
+
+namespace sgk {
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float x0, float x1) {  // x0 in the low half
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(x1), "f"(x0));
+  return r;
+}
+__device__ __forceinline__ float bf16_lo_f32(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float bf16_hi_f32(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_f16(float x0, float x1) {
+  __half2 v = __floats2half2_rn(x0, x1);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+__device__ __forceinline__ uint32_t hmul2_u32(uint32_t a, uint32_t b) {
+  __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hfma2_u32(uint32_t a, uint32_t b, uint32_t c) {
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+// The four A registers' worth of a word: bytes 0, 2 and bytes 1, 3 as fp16 subnormals (u), their low nibbles (r).
+struct U4Word {
+  uint32_t ua, ub, ra, rb;
+  __device__ __forceinline__ explicit U4Word(uint32_t w) {
+    ua = w & 0x00ff00ffu;
+    ub = __byte_perm(w, 0u, 0x4341);
+    ra = w & 0x000f000fu;
+    rb = ub & 0x000f000fu;
+  }
+};
+
+constexpr float U4_LIMIT = 14.0f;   // p'' <= 2^14
+constexpr float U4_LEVEL = 6.0f;    // p'' of the largest z when the reference moves
+
+template <int HD>
+struct U4Smem {
+  static constexpr int G = HD / QGROUP;
+  static constexpr int STEPS = PAGE_TOKENS * HD / 2;          // 2 bytes per (row, group)
+  static constexpr int BIASES = STEPS + PAGE_TOKENS * G * 2;  // bf16 [row][group]
+  static constexpr int POWERS = BIASES + PAGE_TOKENS * G * 2; // 8 x bf16
+  static constexpr int TILE = POWERS + 16;
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int OPAD = HD + 4;
+  static constexpr int Q_BYTES = G * 2 * 32 * 16;             // B fragments: [group][u | r][lane]{hi, lo}
+  static constexpr int QROWS_BYTES = 8 * HD * 4;              // q in f32 while the fragments are made
+  static constexpr int QSUM_BYTES = 8 * 8 * 4 + 8 * 4;        // [head][8 groups], absent groups zero; power of two per head
+  static constexpr int O_BYTES = MMA_CONSUMERS * 8 * OPAD * 4;
+  static constexpr int ML_BYTES = 512;
+  static constexpr int BAR_BYTES = 2 * MMA_MAX_STAGES * 8;
+  // the row of a fused append: f32 K and V, afterwards its bytes (codes K | V, then 4 G + 1 half words)
+  static constexpr int NEW_BYTES = 2 * HD * 4;
+  static constexpr int RECV_BYTES = ClusterRecv<HD>::BYTES;
+  static constexpr int FIXED = Q_BYTES + QROWS_BYTES + QSUM_BYTES + ML_BYTES + BAR_BYTES + 64 + NEW_BYTES + RECV_BYTES;
+  __host__ __device__ static size_t ring_bytes(int stages) {
+    size_t r = size_t(stages) * STAGE;
+    r = r > size_t(O_BYTES) ? r : size_t(O_BYTES);
+    return (r + 15) / 16 * 16;
+  }
+  static size_t total(int stages) { return ring_bytes(stages) + FIXED + 128; }
+  static_assert(STAGE % 16 == 0 && TILE % 16 == 0 && QSUM_BYTES % 16 == 0, "16-byte pieces");
+};
+
+// Writes the row that a fused append has quantised (`park`) into a tile pair in global or shared memory; one warp.
+template <int HD>
+__device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park, int rin, int lane) {
+  using S = U4Smem<HD>;
+  uint8_t* vtile = ktile + S::TILE;
+  const uint16_t* meta = reinterpret_cast<const uint16_t*>(park + HD);   // K step, K bias, V factor, V bias [G] each, power
+  const int p = lane & 15;
+#pragma unroll
+  for (int grp = 0; grp < S::G; ++grp) {
+    const int dim = grp * QGROUP + p;
+    if (lane < 16) ktile[u4_k_byte(rin, dim, HD)] = park[grp * 16 + p];
+    else vtile[u4_v_byte(rin, dim, HD)] = park[HD / 2 + grp * 16 + p];
+  }
+  if (lane < S::G) {
+    *reinterpret_cast<uint16_t*>(ktile + u4_step_offset(0, rin, lane, HD)) = meta[lane];
+    *reinterpret_cast<uint16_t*>(ktile + u4_bias_offset(rin, lane, HD)) = meta[S::G + lane];
+    *reinterpret_cast<uint16_t*>(vtile + u4_step_offset(1, rin, lane, HD)) = meta[2 * S::G + lane];
+    *reinterpret_cast<uint16_t*>(vtile + u4_bias_offset(rin, lane, HD)) = meta[3 * S::G + lane];
+  }
+  if (lane == 0) *reinterpret_cast<uint16_t*>((rin < 8 ? ktile : vtile) + u4_pow_offset(rin, HD)) = meta[4 * S::G];
+}
+
+// PP: pages a warp works on at once. Two (head_dim 128) give the chains of matrix instructions twice
+// the independent work and share the query's fragments; with head_dim 256 one page fills the registers.
+template <int HD, bool CLUSTER, bool PEERS>
+__global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a) {
+  using S = U4Smem<HD>;
+  constexpr int G = S::G;
+  constexpr int PP = HD == 128 ? 2 : 1;
+  constexpr int SETS = G / 4;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  const int nst = a.n_stages;
+  uint8_t* q_frag = ring + S::ring_bytes(nst);
+  float* q_rows = reinterpret_cast<float*>(q_frag + S::Q_BYTES);          // [8][HD]
+  float* qsum_s = q_rows + 8 * HD;                                        // [8][8]
+  float* qpow_s = qsum_s + 64;                                            // [8]
+  float* o_s = reinterpret_cast<float*>(ring);    // aliases the ring once it has drained
+  float* ml_s = qpow_s + 8;                                               // [warps][8][2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(ml_s) + S::ML_BYTES);
+  int* flags = reinterpret_cast<int*>(bars + 2 * MMA_MAX_STAGES);
+  float* new_s = reinterpret_cast<float*>(flags + 16);
+  float* recv_s = new_s + 2 * HD;
+  volatile int* abort_flag = flags;
+
+  const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int gqa = a.q_heads / a.pool.kv_heads;
+  const int slot = a.slots ? a.slots[seq] : a.slot0;
+  int32_t* len_ptr = a.pool.lens + int64_t(slot) * a.pool.layers + a.layer;
+  const bool do_append = a.k_new != nullptr;
+  if (a.pdl_trigger) pdl_launch_dependents();
+
+  const int len_old = *reinterpret_cast<const volatile int32_t*>(len_ptr);
+  const int len = len_old + (do_append ? 1 : 0);
+  int64_t start = a.sliding_window > 0 ? (len > a.sliding_window ? len - a.sliding_window : 0) : a.window_start;
+  if (start >= len) start = len > 0 ? len - 1 : 0;
+  const int ws = static_cast<int>(start);
+  const int sinks = static_cast<int>(a.sink_rows < ws ? a.sink_rows : ws);   // rows [0, sinks) and [ws, len) are seen
+  const int p_first = ws / PAGE_TOKENS;
+  const int sink_pages = min((sinks + PAGE_TOKENS - 1) / PAGE_TOKENS, p_first);
+  const PageMap map{sink_pages, p_first - sink_pages};
+  const int n_pages = sink_pages + (len - 1) / PAGE_TOKENS - p_first + 1;
+  int splits = a.splits;
+  if (a.pages_per_split > 0) {
+    const int want = (n_pages + a.pages_per_split - 1) / a.pages_per_split;
+    splits = want < 1 ? 1 : min(want, a.splits);
+  }
+  if (split >= splits) return;
+  const int pb = static_cast<int>(int64_t(n_pages) * split / splits);
+  const int pe = static_cast<int>(int64_t(n_pages) * (split + 1) / splits);
+  const int my_pages = pe - pb;
+  const int32_t* table = a.pool.tables + int64_t(slot) * a.pool.table_stride;
+  const int64_t head_off = int64_t(a.layer) * a.pool.layer_bytes + int64_t(kvh) * 2 * a.pool.tile_bytes;
+  const bool owns_append = do_append && pe == n_pages && my_pages > 0;   // the new row lies in the last page
+
+  int32_t first_entry = -1;
+  if (warp == MMA_CONSUMERS) {
+    if (lane == 0) {
+      flags[0] = 0;
+      flags[1] = 0;
+      flags[5] = 0;   // set once the quantised row of a fused append is parked in shared memory
+      for (int s = 0; s < nst; ++s) {
+        mbar_init(smem_u32(bars + s), 1);
+        mbar_init(smem_u32(bars + MMA_MAX_STAGES + s), 1);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (lane < my_pages) first_entry = table[map.page(pb + lane)];
+    __syncwarp();
+    asm volatile("bar.arrive 3, %0;" ::"r"(MMA_THREADS) : "memory");
+    // ---------------- producer warp ----------------
+    produce_pages<S::STAGE>(a, table, pb, my_pages, first_entry, ring, bars, nst, head_off, abort_flag, lane, map);
+    if (a.pdl_wait) pdl_wait();   // the tail writes to memory the earlier launch may still be using
+  } else {
+    // ---------------- consumer warps: the query first ----------------
+    constexpr int NV = HD / 64;
+    const float* q = a.q + (int64_t(seq) * a.q_heads + int64_t(kvh) * gqa) * HD;
+    // q and the row to append come from the launch before this one; the cursor, the block table and
+    // the pages the producer starts to copy do not
+    if (a.pdl_wait) pdl_wait();
+    float4 v[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int f = (tid + k * MMA_CONSUMERS * 32) * 4;
+      v[k] = (f / HD < gqa) ? __ldg(reinterpret_cast<const float4*>(q + f)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (owns_append && tid * 4 < 2 * HD) {
+      const int64_t row_off = int64_t(seq) * a.pool.kv_heads * HD + kvh * HD;
+      const float* src = tid * 4 < HD ? a.k_new + row_off + tid * 4 : a.v_new + row_off + (tid * 4 - HD);
+      *reinterpret_cast<float4*>(new_s + tid * 4) = __ldg(reinterpret_cast<const float4*>(src));
+    }
+    if (owns_append && tid == 0) flags[2] = table[len_old / PAGE_TOKENS];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int f = (tid + k * MMA_CONSUMERS * 32) * 4;
+      v[k].x *= a.scale_log2e, v[k].y *= a.scale_log2e, v[k].z *= a.scale_log2e, v[k].w *= a.scale_log2e;
+      *reinterpret_cast<float4*>(q_rows + f) = v[k];
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(MMA_CONSUMERS * 32) : "memory");
+    // Two heads per warp: sums of the groups, and the power of two that brings the largest |q| to 2^12..2^13.
+#pragma unroll
+    for (int h = 2 * warp; h < 2 * warp + 2; ++h) {
+      float big = 0.0f;
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) {
+        const float x = q_rows[h * HD + grp * QGROUP + lane];
+        big = fmaxf(big, fabsf(x));
+        float sum = x;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == grp) qsum_s[h * 8 + grp] = sum;
+      }
+      if (G < 8 && lane >= G && lane < 8) qsum_s[h * 8 + lane] = 0.0f;
+      asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(big) : "f"(big));
+      if (lane == 0) {
+        const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+        qpow_s[h] = pow2f(max(-90, min(90, e - 12)));   // q = qpow * (what the fragments hold)
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"r"(MMA_CONSUMERS * 32) : "memory");
+    for (int i = tid; i < G * 32; i += MMA_CONSUMERS * 32) {
+      const int grp = i >> 5, h = (i & 31) >> 2, t = i & 3;
+      const float inv = 1.0f / qpow_s[h];
+      const float* row = q_rows + h * HD + grp * QGROUP + 4 * t;
+      const float4 x = *reinterpret_cast<const float4*>(row), y = *reinterpret_cast<const float4*>(row + 16);
+      const float u[4] = {y.x * inv * 0.0625f, y.y * inv * 0.0625f, y.z * inv * 0.0625f, y.w * inv * 0.0625f};
+      const float r[4] = {x.x * inv - u[0], x.y * inv - u[1], x.z * inv - u[2], x.w * inv - u[3]};
+      // k-slots (2t, 2t+1) are the bytes 0 and 2 of a word, (2t+8, 2t+9) the bytes 1 and 3
+      uint4 fu, fr;
+      fu.x = pack_f16(u[0], u[2]), fu.y = pack_f16(u[1], u[3]);
+      fr.x = pack_f16(r[0], r[2]), fr.y = pack_f16(r[1], r[3]);
+      const float2 u0 = unpack_f16(fu.x), u1 = unpack_f16(fu.y), r0 = unpack_f16(fr.x), r1 = unpack_f16(fr.y);
+      fu.z = pack_f16(u[0] - u0.x, u[2] - u0.y), fu.w = pack_f16(u[1] - u1.x, u[3] - u1.y);
+      fr.z = pack_f16(r[0] - r0.x, r[2] - r0.y), fr.w = pack_f16(r[1] - r1.x, r[3] - r1.y);
+      *reinterpret_cast<uint4*>(q_frag + ((grp * 2) * 32 + (i & 31)) * 16) = fu;
+      *reinterpret_cast<uint4*>(q_frag + ((grp * 2 + 1) * 32 + (i & 31)) * 16) = fr;
+    }
+    // The bias product's B fragment: group sums as three bf16 parts. With four groups the sixteen k-slots
+    // take {hi, mid, lo, nothing}; with eight, {hi, mid}, and lo goes through a k = 8 product.
+    uint32_t qs0, qs1, qs2 = 0;
+    {
+      const int g = lane >> 2, t = lane & 3;
+      const int pair = G == 4 ? (t & 1) : t;
+      const float2 x = *reinterpret_cast<const float2*>(qsum_s + g * 8 + 2 * pair);
+      const uint32_t hi = pack_bf16(x.x, x.y);
+      const float2 r = make_float2(x.x - bf16_lo_f32(hi), x.y - bf16_hi_f32(hi));
+      const uint32_t mid = pack_bf16(r.x, r.y);
+      const uint32_t lo = pack_bf16(r.x - bf16_lo_f32(mid), r.y - bf16_hi_f32(mid));
+      if (G == 4) qs0 = t < 2 ? hi : mid, qs1 = t < 2 ? lo : 0u;
+      else qs0 = hi, qs1 = mid, qs2 = lo;
+    }
+    const int g = lane >> 2, t = lane & 3;
+    const float ch0 = qpow_s[2 * t] * 16777216.0f, ch1 = qpow_s[2 * t + 1] * 16777216.0f;   // codes are in units of 2^-24
+    asm volatile("bar.sync 3, %0;" ::"r"(MMA_THREADS) : "memory");   // fragments written; barriers initialised
+
+    // The row of a fused append is quantised now, by the warp with the fewest pages, while the first pages are
+    // on their way; its bytes go to the page in global memory and stay parked in shared memory for the warp
+    // that will meet the page in the ring.
+    uint8_t* park = reinterpret_cast<uint8_t*>(new_s);
+    if (owns_append && warp == MMA_CONSUMERS - 1) {
+      const int rin = len_old % PAGE_TOKENS;
+      const uint32_t odd = rin & 1;
+      const int32_t page = flags[2];
+      float x[2 * G];
+#pragma unroll
+      for (int i = 0; i < 2 * G; ++i) x[i] = new_s[i * QGROUP + lane];
+      __syncwarp();
+      uint32_t code[2 * G];
+      uint16_t* meta = reinterpret_cast<uint16_t*>(park + HD);
+#pragma unroll
+      for (int is_v = 0; is_v < 2; ++is_v) {
+        U4Row<G> row;
+        row.quantize(*reinterpret_cast<float(*)[G]>(x + is_v * G), odd);
+#pragma unroll
+        for (int grp = 0; grp < G; ++grp) {
+          code[is_v * G + grp] = row.code[grp];
+          if (lane == grp) {
+            meta[is_v * 2 * G + grp] = is_v ? u4_v_factor_bits(row.step[grp], row.exponent, odd) : static_cast<uint16_t>(row.step[grp] ^ (odd << 15));
+            meta[is_v * 2 * G + G + grp] = row.bias[grp];
+          }
+        }
+        if (is_v && lane == 0) meta[4 * G] = static_cast<uint16_t>(__float_as_uint(pow2f(row.exponent)) >> 16);
+      }
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) {
+        // lanes 0-15 put the K byte together, lanes 16-31 the V byte
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, lane < 16 ? code[G + grp] : code[grp], 16);
+        park[(lane < 16 ? 0 : HD / 2) + grp * 16 + (lane & 15)] =
+            static_cast<uint8_t>(lane < 16 ? code[grp] | (other << 4) : other | (code[G + grp] << 4));
+      }
+      __syncwarp();
+      // a bad table entry is reported by the producer, which meets it too
+      if (page >= 0 && page < a.num_pages) u4_place_row<HD>(a.pool.base + int64_t(page) * a.pool.page_bytes + head_off, park, rin, lane);
+      __syncwarp();
+      if (lane == 0) {
+        __threadfence_block();
+        *reinterpret_cast<volatile int*>(flags + 5) = 1;
+      }
+    }
+
+    // ---------------- the pages ----------------
+    float o_u[G][4], o_r[G][4], o_b[G][2];
+#pragma unroll
+    for (int grp = 0; grp < G; ++grp) {
+      o_u[grp][0] = o_u[grp][1] = o_u[grp][2] = o_u[grp][3] = 0.0f;
+      o_r[grp][0] = o_r[grp][1] = o_r[grp][2] = o_r[grp][3] = 0.0f;
+      o_b[grp][0] = o_b[grp][1] = 0.0f;
+    }
+    float m0 = -1.0e30f, m1 = -1.0e30f, l0 = 0.0f, l1 = 0.0f;
+    const int k_off = g * (HD / 2) + t * 16;                                  // + (set ^ odd row) * 64; row g + 8: + 4 * HD
+    const int kb_off = S::BIASES + g * G * 2 + (G == 4 ? (t & 1) : t) * 4;    // K biases of row g
+    const int vs_off = S::TILE + S::STEPS + t * G * 4;                        // V factors of rows 2t, 2t+1; rows + 8: + 16 * G
+    const int vb_off = S::TILE + S::BIASES + g * G * 2;                       // V biases of row g; row g + 8: + 16 * G
+    int stage = warp;
+    uint32_t parity = 0;
+    for (int i = warp; i < my_pages; i += MMA_CONSUMERS * PP) {
+      uint8_t* tile[PP];
+      int stages[PP];
+      bool ok = true;
+      bool whole = true;   // every row of the pages is seen
+      int row_base[PP];
+#pragma unroll
+      for (int u = 0; u < PP; ++u) {
+        stages[u] = stage;
+        tile[u] = ring + stage * S::STAGE;
+        const int v = pb + i + u * MMA_CONSUMERS;
+        const bool there = u == 0 || i + u * MMA_CONSUMERS < my_pages;
+        row_base[u] = there ? static_cast<int>(map.page(v)) * PAGE_TOKENS : 0x40000000;   // past every length
+        whole = whole && row_base[u] <= len - PAGE_TOKENS && (row_base[u] >= ws || row_base[u] <= sinks - PAGE_TOKENS);
+        if (there) {
+          ok = mbar_wait(smem_u32(bars + stage), parity, abort_flag, a.status) && ok;
+          stage += MMA_CONSUMERS;   // the stage count is a multiple of the consumer count
+          if (stage >= nst) {
+            stage -= nst;
+            parity ^= 1;
+          }
+        }
+        if (there && owns_append && v == n_pages - 1 && ok) {
+          // the new row joins the staged copy
+          uint32_t spins = 0;
+          while (*reinterpret_cast<volatile int*>(flags + 5) == 0) {
+            if (++spins > WAIT_SPINS) {
+              *abort_flag = 1;
+              atomicExch(a.status, DEV_ERR_WAIT_TIMEOUT);
+              break;
+            }
+          }
+          __syncwarp();
+          u4_place_row<HD>(tile[u], park, len_old % PAGE_TOKENS, lane);
+          __syncwarp();
+        }
+      }
+      if (ok) {
+        // ---- scores ----
+        float z[PP][4];   // (row g; heads 2t, 2t+1), (row g + 8; ...)
+        float acc[PP][4][4];
+#pragma unroll
+        for (int u = 0; u < PP; ++u) z[u][0] = z[u][1] = z[u][2] = z[u][3] = 0.0f;
+#pragma unroll
+        for (int set = 0; set < SETS; ++set) {
+          uint4 w0[PP], w1[PP];
+#pragma unroll
+          for (int u = 0; u < PP; ++u) {
+            const int at = k_off + (SETS > 1 ? (set ^ (g & 1)) : 0) * 64;
+            w0[u] = *reinterpret_cast<const uint4*>(tile[u] + at);
+            w1[u] = *reinterpret_cast<const uint4*>(tile[u] + at + 4 * HD);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.0f;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 fu = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2) * 32 + lane) * 16);
+            const uint4 fr = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2 + 1) * 32 + lane) * 16);
+#pragma unroll
+            for (int u = 0; u < PP; ++u) {
+              const uint32_t x0 = j == 0 ? w0[u].x : j == 1 ? w0[u].y : j == 2 ? w0[u].z : w0[u].w;
+              const uint32_t x1 = j == 0 ? w1[u].x : j == 1 ? w1[u].y : j == 2 ? w1[u].z : w1[u].w;
+              const U4Word c0(x0), c1(x1);
+              mma_f16(acc[u][j], c0.ua, c1.ua, c0.ub, c1.ub, fu.x, fu.y);
+              mma_f16(acc[u][j], c0.ra, c1.ra, c0.rb, c1.rb, fr.x, fr.y);
+              mma_f16(acc[u][j], c0.ua, c1.ua, c0.ub, c1.ub, fu.z, fu.w);
+              mma_f16(acc[u][j], c0.ra, c1.ra, c0.rb, c1.rb, fr.z, fr.w);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < PP; ++u) {
+            const uint2 s0 = *reinterpret_cast<const uint2*>(tile[u] + S::STEPS + g * G * 2 + set * 8);
+            const uint2 s1 = *reinterpret_cast<const uint2*>(tile[u] + S::STEPS + (g + 8) * G * 2 + set * 8);
+            const float a0[4] = {bf16_lo_f32(s0.x), bf16_hi_f32(s0.x), bf16_lo_f32(s0.y), bf16_hi_f32(s0.y)};
+            const float a1[4] = {bf16_lo_f32(s1.x), bf16_hi_f32(s1.x), bf16_lo_f32(s1.y), bf16_hi_f32(s1.y)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              z[u][0] = fmaf(a0[j], acc[u][j][0], z[u][0]);
+              z[u][1] = fmaf(a0[j], acc[u][j][1], z[u][1]);
+              z[u][2] = fmaf(a1[j], acc[u][j][2], z[u][2]);
+              z[u][3] = fmaf(a1[j], acc[u][j][3], z[u][3]);
+            }
+          }
+        }
+        float back[PP][2];   // 2^-e of rows g, g + 8
+        bool over = false;
+#pragma unroll
+        for (int u = 0; u < PP; ++u) {
+          const uint32_t e0 = *reinterpret_cast<const uint16_t*>(tile[u] + S::POWERS + 2 * g);
+          const uint32_t e1 = *reinterpret_cast<const uint16_t*>(tile[u] + S::TILE + S::POWERS + 2 * g);
+          back[u][0] = __uint_as_float(0x7f000000u - (e0 << 16));
+          back[u][1] = __uint_as_float(0x7f000000u - (e1 << 16));
+          const float x0 = __uint_as_float(0x4b000000u | (e0 >> 7)) - 8388735.0f;   // e = exponent field - 127
+          const float x1 = __uint_as_float(0x4b000000u | (e1 >> 7)) - 8388735.0f;
+          float sb[4] = {x0, x0, x1, x1};
+          const uint32_t b0 = *reinterpret_cast<const uint32_t*>(tile[u] + kb_off);
+          const uint32_t b1 = *reinterpret_cast<const uint32_t*>(tile[u] + kb_off + 16 * G);
+          mma_bf16(sb, b0, b1, b0, b1, qs0, qs1);
+          if (G == 8) mma_bf16_k8(sb, b0, b1, qs2);
+          z[u][0] = fmaf(z[u][0], ch0, sb[0]);
+          z[u][1] = fmaf(z[u][1], ch1, sb[1]);
+          z[u][2] = fmaf(z[u][2], ch0, sb[2]);
+          z[u][3] = fmaf(z[u][3], ch1, sb[3]);
+        }
+        uint4 vs0[PP][SETS], vs1[PP][SETS];   // V factors: rows (2t, 2t+1) and (2t+8, 2t+9)
+        uint2 vb0[PP][SETS], vb1[PP][SETS];   // V biases: rows g and g + 8
+#pragma unroll
+        for (int u = 0; u < PP; ++u)
+#pragma unroll
+          for (int set = 0; set < SETS; ++set) {
+            vs0[u][set] = *reinterpret_cast<const uint4*>(tile[u] + vs_off + set * 16);
+            vs1[u][set] = *reinterpret_cast<const uint4*>(tile[u] + vs_off + 16 * G + set * 16);
+            vb0[u][set] = *reinterpret_cast<const uint2*>(tile[u] + vb_off + set * 8);
+            vb1[u][set] = *reinterpret_cast<const uint2*>(tile[u] + vb_off + 16 * G + set * 8);
+          }
+        if (!whole) {
+          // A row that is not seen weighs nothing, whatever its bytes say.
+#pragma unroll
+          for (int u = 0; u < PP; ++u) {
+            const auto seen = [&](int r) {
+              const int row = row_base[u] + r;
+              return row < len && (row < sinks || row >= ws);
+            };
+            const bool s0 = seen(g), s1 = seen(g + 8);
+            if (!s0) z[u][0] = z[u][1] = -INFINITY, back[u][0] = 0.0f;
+            if (!s1) z[u][2] = z[u][3] = -INFINITY, back[u][1] = 0.0f;
+            const uint32_t k0 = (seen(2 * t) ? 0x0000ffffu : 0u) | (seen(2 * t + 1) ? 0xffff0000u : 0u);
+            const uint32_t k1 = (seen(2 * t + 8) ? 0x0000ffffu : 0u) | (seen(2 * t + 9) ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int set = 0; set < SETS; ++set) {
+              vs0[u][set] = make_uint4(vs0[u][set].x & k0, vs0[u][set].y & k0, vs0[u][set].z & k0, vs0[u][set].w & k0);
+              vs1[u][set] = make_uint4(vs1[u][set].x & k1, vs1[u][set].y & k1, vs1[u][set].z & k1, vs1[u][set].w & k1);
+              if (!s0) vb0[u][set] = make_uint2(0u, 0u);
+              if (!s1) vb1[u][set] = make_uint2(0u, 0u);
+            }
+          }
+        }
+        float mx0 = fmaxf(z[0][0], z[0][2]), mx1 = fmaxf(z[0][1], z[0][3]);
+        if (PP == 2) mx0 = fmaxf(mx0, fmaxf(z[PP - 1][0], z[PP - 1][2])), mx1 = fmaxf(mx1, fmaxf(z[PP - 1][1], z[PP - 1][3]));
+        over = mx0 > m0 + U4_LIMIT || mx1 > m1 + U4_LIMIT;
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+          }
+          const float mn0 = mx0 > m0 + U4_LIMIT ? mx0 - U4_LEVEL : m0, mn1 = mx1 > m1 + U4_LIMIT ? mx1 - U4_LEVEL : m1;
+          const float al0 = exp2f(m0 - mn0), al1 = exp2f(m1 - mn1);
+          l0 *= al0;
+          l1 *= al1;
+#pragma unroll
+          for (int grp = 0; grp < G; ++grp) {
+            o_u[grp][0] *= al0, o_u[grp][2] *= al0, o_r[grp][0] *= al0, o_r[grp][2] *= al0, o_b[grp][0] *= al0;
+            o_u[grp][1] *= al1, o_u[grp][3] *= al1, o_r[grp][1] *= al1, o_r[grp][3] *= al1, o_b[grp][1] *= al1;
+          }
+          m0 = mn0;
+          m1 = mn1;
+        }
+        // ---- weights and outputs ----
+#pragma unroll
+        for (int u = 0; u < PP; ++u) {
+          float p[4];
+          p[0] = exp2f(z[u][0] - m0);
+          p[1] = exp2f(z[u][1] - m1);
+          p[2] = exp2f(z[u][2] - m0);
+          p[3] = exp2f(z[u][3] - m1);
+          const uint32_t h0 = pack_f16(p[0], p[1]), h1 = pack_f16(p[2], p[3]);
+          const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
+          const uint32_t d0 = pack_f16(p[0] - f0.x, p[1] - f0.y), d1 = pack_f16(p[2] - f1.x, p[3] - f1.y);
+          // (row g; heads 2t, 2t+1) -> (rows 2t, 2t+1; head g)
+          const uint32_t ph0 = movmatrix_trans(h0), ph1 = movmatrix_trans(h1);
+          const uint32_t pl0 = movmatrix_trans(d0), pl1 = movmatrix_trans(d1);
+          p[0] *= back[u][0], p[1] *= back[u][0], p[2] *= back[u][1], p[3] *= back[u][1];
+          l0 += p[0] + p[2];
+          l1 += p[1] + p[3];
+#pragma unroll
+          for (int set = 0; set < SETS; ++set) {
+            const float b0[4] = {bf16_lo_f32(vb0[u][set].x), bf16_hi_f32(vb0[u][set].x), bf16_lo_f32(vb0[u][set].y), bf16_hi_f32(vb0[u][set].y)};
+            const float b1[4] = {bf16_lo_f32(vb1[u][set].x), bf16_hi_f32(vb1[u][set].x), bf16_lo_f32(vb1[u][set].y), bf16_hi_f32(vb1[u][set].y)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              o_b[set * 4 + j][0] = fmaf(b0[j], p[0], fmaf(b1[j], p[2], o_b[set * 4 + j][0]));
+              o_b[set * 4 + j][1] = fmaf(b0[j], p[1], fmaf(b1[j], p[3], o_b[set * 4 + j][1]));
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {   // two groups: one 16-byte load of codes
+              const int grp = set * 4 + half * 2;
+              const uint4 w = *reinterpret_cast<const uint4*>(tile[u] + S::TILE + ((grp >> 1) * 32 + lane) * 16);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t s0 = half ? (j ? vs0[u][set].w : vs0[u][set].z) : (j ? vs0[u][set].y : vs0[u][set].x);
+                const uint32_t s1 = half ? (j ? vs1[u][set].w : vs1[u][set].z) : (j ? vs1[u][set].y : vs1[u][set].x);
+                const uint32_t wh0 = hmul2_u32(ph0, s0), wh1 = hmul2_u32(ph1, s1);
+                const uint32_t wl0 = hfma2_u32(pl0, s0, hfma2_u32(ph0, s0, wh0 ^ 0x80008000u));
+                const uint32_t wl1 = hfma2_u32(pl1, s1, hfma2_u32(ph1, s1, wh1 ^ 0x80008000u));
+                const U4Word c0(j ? w.z : w.x), c1(j ? w.w : w.y);
+                mma_f16(o_u[grp + j], c0.ua, c1.ua, c0.ub, c1.ub, wh0, wh1);
+                mma_f16(o_r[grp + j], c0.ra, c1.ra, c0.rb, c1.rb, wh0, wh1);
+                mma_f16(o_u[grp + j], c0.ua, c1.ua, c0.ub, c1.ub, wl0, wl1);
+                mma_f16(o_r[grp + j], c0.ra, c1.ra, c0.rb, c1.rb, wl0, wl1);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < PP; ++u)
+          if (u == 0 || i + u * MMA_CONSUMERS < my_pages) mbar_arrive(smem_u32(bars + MMA_MAX_STAGES + stages[u]));
+      }
+    }
+
+    // ---- hand this warp's state to the merge buffer (it aliases the ring) ----
+    asm volatile("bar.sync 1, %0;" ::"r"(MMA_CONSUMERS * 32) : "memory");
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp) {
+        o_b[grp][0] += __shfl_xor_sync(0xffffffffu, o_b[grp][0], off);
+        o_b[grp][1] += __shfl_xor_sync(0xffffffffu, o_b[grp][1], off);
+      }
+    }
+    float* ow = o_s + warp * 8 * S::OPAD;
+#pragma unroll
+    for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {   // (dim g + 8 * (c / 2); head 2t + c % 2)
+        float* to = ow + (2 * t + (c & 1)) * S::OPAD + grp * QGROUP + g + 8 * (c >> 1);
+        to[0] = fmaf(o_r[grp][c], 16777216.0f, o_b[grp][c & 1]);
+        to[16] = fmaf(o_u[grp][c] - o_r[grp][c], 1048576.0f, o_b[grp][c & 1]);   // 2^24 / 16
+      }
+    if (g == 0) {
+      ml_s[(warp * 8 + 2 * t) * 2] = m0;
+      ml_s[(warp * 8 + 2 * t) * 2 + 1] = l0;
+      ml_s[(warp * 8 + 2 * t + 1) * 2] = m1;
+      ml_s[(warp * 8 + 2 * t + 1) * 2 + 1] = l1;
+    }
+  }
+  __syncthreads();
+  finish_block<HD, CLUSTER, PEERS>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
+                                   splits, recv_s);
+  if (PEERS) peers_finish(a, tid, flags);
+}
+
+bool attention_u4_supported(int dtype, int head_dim, int gqa) {
+  return dtype == KV_U4G32 && (head_dim == 128 || head_dim == 256) && gqa >= 1 && gqa <= 8;
+}
+
+int attention_u4_max_stages(int head_dim) {
+  size_t budget = 113 * 1024;  // two blocks per SM
+  size_t fixed = head_dim == 128 ? U4Smem<128>::FIXED : U4Smem<256>::FIXED;
+  size_t stage = head_dim == 128 ? U4Smem<128>::STAGE : U4Smem<256>::STAGE;
+  int n = static_cast<int>((budget - fixed - 128) / stage);
+  if (n > MMA_MAX_STAGES) n = MMA_MAX_STAGES;
+  return n / MMA_CONSUMERS * MMA_CONSUMERS;  // a stage always belongs to the same warp
+}
+
+static const void* u4_kernel(int head_dim, bool cluster, bool peers) {
+  if (head_dim == 128)
+    return peers     ? reinterpret_cast<const void*>(attention_u4_kernel<128, false, true>)
+           : cluster ? reinterpret_cast<const void*>(attention_u4_kernel<128, true, false>)
+                     : reinterpret_cast<const void*>(attention_u4_kernel<128, false, false>);
+  return peers     ? reinterpret_cast<const void*>(attention_u4_kernel<256, false, true>)
+         : cluster ? reinterpret_cast<const void*>(attention_u4_kernel<256, true, false>)
+                   : reinterpret_cast<const void*>(attention_u4_kernel<256, false, false>);
+}
+static size_t u4_smem(int head_dim, int n_stages) {
+  return head_dim == 128 ? U4Smem<128>::total(n_stages) : U4Smem<256>::total(n_stages);
+}
+
+int attention_u4_resident_blocks(int head_dim, int n_stages) {
+  int blocks = 0;
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, u4_kernel(head_dim, false, false), MMA_THREADS,
+                                                                u4_smem(head_dim, n_stages));
+  return e == cudaSuccess ? blocks : 0;
+}
+
+// How many clusters of `splits` blocks the device can hold at once (0: such a launch would fail).
+int attention_u4_max_clusters(int head_dim, int n_stages, int splits) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(splits, 1, 1);
+  cfg.blockDim = dim3(MMA_THREADS);
+  cfg.dynamicSmemBytes = u4_smem(head_dim, n_stages);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, u4_kernel(head_dim, true, false), &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
+cudaError_t attention_u4_configure() {
+  for (int hd : {128, 256})
+    for (int kind = 0; kind < 3; ++kind) {
+      const void* kernel = u4_kernel(hd, kind == 1, kind == 2);
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+      // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
+      if (e == cudaSuccess && kind == 1) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+    }
+  return cudaSuccess;
+}
+
+cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.splits, a.pool.kv_heads, n_seq);
+  cfg.blockDim = dim3(MMA_THREADS);
+  cfg.dynamicSmemBytes = u4_smem(a.pool.head_dim, a.n_stages);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n_attr = 0;
+  if (a.cluster_merge && a.n_peers == 0) {
+    // the splits of a (sequence, KV head) are the x extent of the grid and of the cluster
+    attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+    attr[n_attr].val.clusterDim.x = a.splits;
+    attr[n_attr].val.clusterDim.y = 1;
+    attr[n_attr].val.clusterDim.z = 1;
+    n_attr += 1;
+  } else if (a.shared_merge == 1) {
+    // blocks that wait for one another next to launches of other streams
+    attr[n_attr].id = cudaLaunchAttributeCooperative;
+    attr[n_attr].val.cooperative = 1;
+    n_attr += 1;
+  }
+  if (a.pdl_wait) {
+    attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+    n_attr += 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n_attr;
+  void* args[1] = {const_cast<AttnArgs*>(&a)};
+  return cudaLaunchKernelExC(&cfg, u4_kernel(a.pool.head_dim, a.cluster_merge != 0, a.n_peers > 0), args);
+}
+
+}  // namespace sgk

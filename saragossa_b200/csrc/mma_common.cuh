@@ -102,17 +102,26 @@ __device__ __forceinline__ unsigned long long sgk_trace_now(int gt) {
 // no-ops in a launch without such a neighbour.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Which pages a windowed attention with sinks reads: the page with ordinal v (0 .. n_pages) is page v
+// while v < sinks, page v + gap from there on. Without sinks: sinks = 0, gap = the window's first page.
+struct PageMap {
+  int64_t sinks, gap;
+  __device__ __forceinline__ int64_t page(int64_t v) const { return v + (v >= sinks ? gap : 0); }
+};
+struct PageIdentity {
+  __device__ __forceinline__ int64_t page(int64_t v) const { return v; }
+};
 // The producer warp's walk over the block's pages [pb, pb + my_pages): one bulk copy of
 // STAGE_BYTES per page into stage (page index % nst), completion on the stage's "full" barrier
 // (bars[stage]); a stage is refilled once its "empty" barrier (bars[MMA_MAX_STAGES + stage]) has
 // completed. The first min(my_pages, nst) copies find fresh stages and wait for nothing: lane j
 // starts page j, so one pass of the warp puts them all in flight (issued one after the other by
 // one lane, each costs that lane a round trip to its barrier first). first_entry: lane l holds
-// table[pb + l] for l < my_pages.
-template <int STAGE_BYTES>
+// the table's entry of page pb + l for l < my_pages.
+template <int STAGE_BYTES, typename MAP = PageIdentity>
 __device__ __forceinline__ void produce_pages(const AttnArgs& a, const int32_t* table, int64_t pb, int my_pages,
                                               int32_t first_entry, uint8_t* ring, uint64_t* bars, int nst,
-                                              int64_t head_off, volatile int* abort_flag, int lane) {
+                                              int64_t head_off, volatile int* abort_flag, int lane, MAP map = MAP()) {
   const uint64_t policy = l2_policy_evict_first();
   const int first = my_pages < nst ? my_pages : nst;
   if (lane < first) {
@@ -133,7 +142,7 @@ __device__ __forceinline__ void produce_pages(const AttnArgs& a, const int32_t* 
   uint32_t parity = 0;    // second use of a stage: wait for the consumers' first release
   for (int base = 0; base < my_pages; base += 32) {
     const int idx = base + lane;
-    const int32_t entry = base == 0 ? first_entry : (idx < my_pages ? table[pb + idx] : -1);
+    const int32_t entry = base == 0 ? first_entry : (idx < my_pages ? table[map.page(pb + idx)] : -1);
     const int cnt = min(32, my_pages - base);
     for (int j = base == 0 ? nst : 0; j < cnt; ++j) {
       const int32_t page = __shfl_sync(0xffffffffu, entry, j);

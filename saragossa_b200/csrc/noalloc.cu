@@ -129,10 +129,11 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   unsigned char* scratch = nullptr;
   SGK_TRY(noalloc_scratch(st->device, &scratch));
 
-  // the same kernel selection as the allocating entry point: tensor-core kernels over bf16 and over
-  // u8 group-32 pages, the generic kernel for everything else
+  // the same kernel selection as the allocating entry point: tensor-core kernels over bf16, u8 and
+  // u4 group-32 pages, the generic kernel for everything else
+  const bool u4 = attention_u4_supported(pool->dtype, hd, qh / kvh);
   const bool u8 = sinks.rows == 0 && attention_u8_supported(pool->dtype, hd, qh / kvh);
-  const bool mma = u8 || (sinks.rows == 0 && attention_mma_supported(pool->dtype, hd, qh / kvh));
+  const bool mma = u4 || u8 || (sinks.rows == 0 && attention_mma_supported(pool->dtype, hd, qh / kvh));
   // split count: fill the SMs (two blocks each for the tensor-core kernel, eight for the
   // generic one), keep a few pages per split, and stay inside the static workspace
   const int64_t pages = (len - window_start + PAGE_TOKENS - 1) / PAGE_TOKENS + sinks.pages;
@@ -186,7 +187,10 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   a.num_pages = pool->num_pages;
   a.k_new = nullptr;
   a.v_new = nullptr;
-  if (u8) {
+  if (u4) {
+    a.n_stages = attention_u4_max_stages(hd);
+    SGK_CUDA(launch_attention_u4(a, 1, cs));
+  } else if (u8) {
     a.n_stages = attention_u8_max_stages(hd);
     SGK_CUDA(launch_attention_u8(a, 1, cs));
   } else if (mma) {

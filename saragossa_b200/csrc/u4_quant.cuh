@@ -92,6 +92,33 @@ __device__ __forceinline__ void warp_min_max(float x, float& lo, float& hi) {
   asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(x));
 }
 
+// One head row of G groups held by a warp, lane l with element l of every group.
+template <int G>
+struct U4Row {
+  uint32_t code[G];
+  uint16_t step[G], bias[G];   // step positive, bias signed (bf16 bits)
+  int exponent;
+  __device__ __forceinline__ void quantize(const float (&x)[G], uint32_t odd) {
+    const float sign = odd ? -1.0f : 1.0f;
+    U4Range r[G];
+    exponent = U4_EXP_MIN;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float lo, hi;
+      warp_min_max(sign * x[g], lo, hi);
+      r[g] = u4_range(lo, hi);
+      exponent = max(exponent, r[g].exponent);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      step[g] = u4_step_bits(r[g], exponent);
+      const float s = bf16_bits_to_f32(step[g]);
+      code[g] = r[g].finite ? u4_code_of(sign * x[g], r[g].bias, s, 1.0f / s) : 0u;
+      bias[g] = static_cast<uint16_t>(r[g].finite ? (__float_as_uint(sign * r[g].bias) >> 16) : 0u);
+    }
+  }
+};
+
 // Quantises and stores one head row of `hd` values (xs, shared memory) as row `row` of a u4 tile; one
 // whole warp. ktile / vtile: the K tile and the V tile behind it.
 __device__ __forceinline__ void u4_store_row(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, const float* xs, int lane) {

@@ -303,7 +303,7 @@ def test_attention_over_u4_pages_takes_any_size_of_query(state, hd, scale):
 def test_generic_and_tensor_core_kernel_agree(state):
     kv, k, v = filled(state, 900, 16, 2, 128)
     q = np.random.default_rng(3).standard_normal((16, 128)).astype(np.float32)
-    for which in (1,):
+    for which in (1, 2):
         kv.set_attention_kernel(which)
         assert ref.close(kv.attention_decode(q, attn_scalar=50.0), ref.attention(q, k, v, 2, scalar=50.0))[0], which
     kv.close()
