@@ -5,22 +5,21 @@
 // shared-memory ring, consumer warps, merge of the splits); a page is worth 5/16 of its bf16 bytes and
 // nearly the same products, so here the instructions count. What a page costs a warp:
 //
-//   codes    A byte holds two codes, n0 + 16 n1. Both go to the matrix instruction as fp16 subnormals:
-//            u = the byte (16 n1 + n0) * 2^-24 and r = (byte & 15) * 2^-24, one byte permute or mask each,
-//            four registers from a word with four instructions. Never separated further:
-//   scores   q_x n0 + q_y n1 = r (q_x - q_y / 16) + u (q_y / 16): the two dims of a byte share a k-slot and the
-//            query is prepared once per launch. Products per group of 32 dims, then in f32
-//              z[row][h] = 2^24 sum_g step_k[row][g] (sum_d codes q) + sum_g bias_k[row][g] qsum[h][g] + e[row],
+//   codes    a byte holds two codes, n0 + 16 n1; a word becomes four registers of exact fp16 numbers n0 and
+//            16 n1 with eight instructions (U4Word);
+//   scores   the two dims of a byte share a k-slot, and the query is prepared once per launch (q and q / 16, as fp16
+//            hi + lo parts, 22 bits). Products per group of 32 dims, then in f32
+//              z[row][h] = sum_g step_k[row][g] (sum_d codes q) + sum_g bias_k[row][g] qsum[h][g] + e[row],
 //            the bias sum as one bf16 product with qsum in three bf16 parts (24 bits);
-//   outputs  U[d][h] = sum_row u w, R[d][h] = sum_row r w; the low dim of a byte is R, the high one (U - R) / 16,
-//            taken once at the end. w = p * step_v as fp16 hi + lo (22 bits).
+//   outputs  O[d][h] = sum_row code w, the high dims of the bytes times 16 until the end; w = p * step_v as fp16
+//            hi + lo (22 bits).
 //   softmax  a V row's steps are stored as f * 2^e with fp16 f (layout.h); 2^e joins the score, so the weight
 //            p'' = exp2(z - M) is bounded whatever the row's range, and w = p'' f needs no scaling. p = p'' 2^-e
 //            feeds the sum of the weights and the bias part of V. M is a reference, not the maximum: it moves only
 //            when a z exceeds it by more than 14 (then to 6 below the largest z), so a page costs one vote
 //            instead of the shuffles of a maximum, and p'' stays inside fp16.
 //
-// Rows of odd position are stored negated (u4_quant.cuh): without it U and R would be sums of codes that
+// Rows of odd position are stored negated (u4_quant.cuh): without it O would be a sum of codes that
 // all count up from a minimum, hundreds of times larger than the result under flat attention, and f32
 // would lose those digits.
 // q is scaled to a largest magnitude of 2^12..2^13 per head by a power of two, so any size of query keeps its 22 bits.
@@ -59,18 +58,28 @@ __device__ __forceinline__ uint32_t hmul2_u32(uint32_t a, uint32_t b) {
   __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
+  __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
 __device__ __forceinline__ uint32_t hfma2_u32(uint32_t a, uint32_t b, uint32_t c) {
   __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// The four A registers' worth of a word: bytes 0, 2 and bytes 1, 3 as fp16 subnormals (u), their low nibbles (r).
+// A word's eight codes as four A registers: bytes 0, 2 and bytes 1, 3, their low codes n0 and 16 times their high
+// ones, as fp16 numbers. (0x6400 | byte) is 1024 + byte, so n0 = (1024 + n0) - 1024 and 16 n1 = (1024 + byte) - (1024 + n0),
+// both exact. (As fp16 subnormals, without the subtraction, the codes would cost half the instructions and most of the
+// accumulator's digits: the matrix unit aligns its products by their exponent fields, and a subnormal's field
+// lies up to ten bits above its value. Scores were off by 1e-5.)
 struct U4Word {
-  uint32_t ua, ub, ra, rb;
+  uint32_t a_lo, b_lo, a_hi, b_hi;
   __device__ __forceinline__ explicit U4Word(uint32_t w) {
-    ua = w & 0x00ff00ffu;
-    ub = __byte_perm(w, 0u, 0x4341);
-    ra = w & 0x000f000fu;
-    rb = ub & 0x000f000fu;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4240), b = __byte_perm(w, 0x64646464u, 0x4341);
+    const uint32_t a0 = a & 0xff0fff0fu, b0 = b & 0xff0fff0fu;
+    a_lo = hsub2_u32(a0, 0x64006400u);
+    b_lo = hsub2_u32(b0, 0x64006400u);
+    a_hi = hsub2_u32(a, a0);
+    b_hi = hsub2_u32(b, b0);
   }
 };
 
@@ -86,7 +95,7 @@ struct U4Smem {
   static constexpr int TILE = POWERS + 16;
   static constexpr int STAGE = 2 * TILE;
   static constexpr int OPAD = HD + 4;
-  static constexpr int Q_BYTES = G * 2 * 32 * 16;             // B fragments: [group][u | r][lane]{hi, lo}
+  static constexpr int Q_BYTES = G * 2 * 32 * 16;             // B fragments: [group][high | low dims][lane]{hi, lo}
   static constexpr int QROWS_BYTES = 8 * HD * 4;              // q in f32 while the fragments are made
   static constexpr int QSUM_BYTES = 8 * 8 * 4 + 8 * 4;        // [head][8 groups], absent groups zero; power of two per head
   static constexpr int O_BYTES = MMA_CONSUMERS * 8 * OPAD * 4;
@@ -253,7 +262,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
       const float* row = q_rows + h * HD + grp * QGROUP + 4 * t;
       const float4 x = *reinterpret_cast<const float4*>(row), y = *reinterpret_cast<const float4*>(row + 16);
       const float u[4] = {y.x * inv * 0.0625f, y.y * inv * 0.0625f, y.z * inv * 0.0625f, y.w * inv * 0.0625f};
-      const float r[4] = {x.x * inv - u[0], x.y * inv - u[1], x.z * inv - u[2], x.w * inv - u[3]};
+      const float r[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
       // k-slots (2t, 2t+1) are the bytes 0 and 2 of a word, (2t+8, 2t+9) the bytes 1 and 3
       uint4 fu, fr;
       fu.x = pack_f16(u[0], u[2]), fu.y = pack_f16(u[1], u[3]);
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
       else qs0 = hi, qs1 = mid, qs2 = lo;
     }
     const int g = lane >> 2, t = lane & 3;
-    const float ch0 = qpow_s[2 * t] * 16777216.0f, ch1 = qpow_s[2 * t + 1] * 16777216.0f;   // codes are in units of 2^-24
+    const float ch0 = qpow_s[2 * t], ch1 = qpow_s[2 * t + 1];
     asm volatile("bar.sync 3, %0;" ::"r"(MMA_THREADS) : "memory");   // fragments written; barriers initialised
 
     // The row of a fused append is quantised now, by the warp with the fewest pages, while the first pages are
@@ -328,11 +337,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
     }
 
     // ---------------- the pages ----------------
-    float o_u[G][4], o_r[G][4], o_b[G][2];
+    float o_hi[G][4], o_lo[G][4], o_b[G][2];
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
-      o_u[grp][0] = o_u[grp][1] = o_u[grp][2] = o_u[grp][3] = 0.0f;
-      o_r[grp][0] = o_r[grp][1] = o_r[grp][2] = o_r[grp][3] = 0.0f;
+      o_hi[grp][0] = o_hi[grp][1] = o_hi[grp][2] = o_hi[grp][3] = 0.0f;
+      o_lo[grp][0] = o_lo[grp][1] = o_lo[grp][2] = o_lo[grp][3] = 0.0f;
       o_b[grp][0] = o_b[grp][1] = 0.0f;
     }
     float m0 = -1.0e30f, m1 = -1.0e30f, l0 = 0.0f, l1 = 0.0f;
@@ -405,10 +414,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
               const uint32_t x0 = j == 0 ? w0[u].x : j == 1 ? w0[u].y : j == 2 ? w0[u].z : w0[u].w;
               const uint32_t x1 = j == 0 ? w1[u].x : j == 1 ? w1[u].y : j == 2 ? w1[u].z : w1[u].w;
               const U4Word c0(x0), c1(x1);
-              mma_f16(acc[u][j], c0.ua, c1.ua, c0.ub, c1.ub, fu.x, fu.y);
-              mma_f16(acc[u][j], c0.ra, c1.ra, c0.rb, c1.rb, fr.x, fr.y);
-              mma_f16(acc[u][j], c0.ua, c1.ua, c0.ub, c1.ub, fu.z, fu.w);
-              mma_f16(acc[u][j], c0.ra, c1.ra, c0.rb, c1.rb, fr.z, fr.w);
+              mma_f16(acc[u][j], c0.a_hi, c1.a_hi, c0.b_hi, c1.b_hi, fu.z, fu.w);   // the small parts first: the
+              mma_f16(acc[u][j], c0.a_lo, c1.a_lo, c0.b_lo, c1.b_lo, fr.z, fr.w);   // accumulator is truncated after
+              mma_f16(acc[u][j], c0.a_lo, c1.a_lo, c0.b_lo, c1.b_lo, fr.x, fr.y);   // every product
+              mma_f16(acc[u][j], c0.a_hi, c1.a_hi, c0.b_hi, c1.b_hi, fu.x, fu.y);
             }
           }
 #pragma unroll
@@ -494,13 +503,14 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
           l1 *= al1;
 #pragma unroll
           for (int grp = 0; grp < G; ++grp) {
-            o_u[grp][0] *= al0, o_u[grp][2] *= al0, o_r[grp][0] *= al0, o_r[grp][2] *= al0, o_b[grp][0] *= al0;
-            o_u[grp][1] *= al1, o_u[grp][3] *= al1, o_r[grp][1] *= al1, o_r[grp][3] *= al1, o_b[grp][1] *= al1;
+            o_hi[grp][0] *= al0, o_hi[grp][2] *= al0, o_lo[grp][0] *= al0, o_lo[grp][2] *= al0, o_b[grp][0] *= al0;
+            o_hi[grp][1] *= al1, o_hi[grp][3] *= al1, o_lo[grp][1] *= al1, o_lo[grp][3] *= al1, o_b[grp][1] *= al1;
           }
           m0 = mn0;
           m1 = mn1;
         }
-        // ---- weights and outputs ----
+        // ---- weights ----
+        uint32_t ph[PP][2], pl[PP][2];
 #pragma unroll
         for (int u = 0; u < PP; ++u) {
           float p[4];
@@ -512,8 +522,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
           const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
           const uint32_t d0 = pack_f16(p[0] - f0.x, p[1] - f0.y), d1 = pack_f16(p[2] - f1.x, p[3] - f1.y);
           // (row g; heads 2t, 2t+1) -> (rows 2t, 2t+1; head g)
-          const uint32_t ph0 = movmatrix_trans(h0), ph1 = movmatrix_trans(h1);
-          const uint32_t pl0 = movmatrix_trans(d0), pl1 = movmatrix_trans(d1);
+          ph[u][0] = movmatrix_trans(h0), ph[u][1] = movmatrix_trans(h1);
+          pl[u][0] = movmatrix_trans(d0), pl[u][1] = movmatrix_trans(d1);
           p[0] *= back[u][0], p[1] *= back[u][0], p[2] *= back[u][1], p[3] *= back[u][1];
           l0 += p[0] + p[2];
           l1 += p[1] + p[3];
@@ -526,25 +536,52 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
               o_b[set * 4 + j][0] = fmaf(b0[j], p[0], fmaf(b1[j], p[2], o_b[set * 4 + j][0]));
               o_b[set * 4 + j][1] = fmaf(b0[j], p[1], fmaf(b1[j], p[3], o_b[set * 4 + j][1]));
             }
+          }
+        }
+        // ---- outputs. The matrix instruction truncates its f32 sum: hundreds of them in one accumulator shrink it
+        //      by a few parts in 10^6. So each iteration sums its own pages, small parts first, and the running
+        //      totals take that sum with a rounding addition. ----
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {   // two groups: one 16-byte load of codes
-              const int grp = set * 4 + half * 2;
-              const uint4 w = *reinterpret_cast<const uint4*>(tile[u] + S::TILE + ((grp >> 1) * 32 + lane) * 16);
+        for (int pair = 0; pair < G / 2; ++pair) {   // two groups: one 16-byte load of codes
+          float cu[2][4], cr[2][4];
+          uint32_t wh[PP][2][2], wl[PP][2][2];
+          uint4 w[PP];
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const uint32_t s0 = half ? (j ? vs0[u][set].w : vs0[u][set].z) : (j ? vs0[u][set].y : vs0[u][set].x);
-                const uint32_t s1 = half ? (j ? vs1[u][set].w : vs1[u][set].z) : (j ? vs1[u][set].y : vs1[u][set].x);
-                const uint32_t wh0 = hmul2_u32(ph0, s0), wh1 = hmul2_u32(ph1, s1);
-                const uint32_t wl0 = hfma2_u32(pl0, s0, hfma2_u32(ph0, s0, wh0 ^ 0x80008000u));
-                const uint32_t wl1 = hfma2_u32(pl1, s1, hfma2_u32(ph1, s1, wh1 ^ 0x80008000u));
-                const U4Word c0(j ? w.z : w.x), c1(j ? w.w : w.y);
-                mma_f16(o_u[grp + j], c0.ua, c1.ua, c0.ub, c1.ub, wh0, wh1);
-                mma_f16(o_r[grp + j], c0.ra, c1.ra, c0.rb, c1.rb, wh0, wh1);
-                mma_f16(o_u[grp + j], c0.ua, c1.ua, c0.ub, c1.ub, wl0, wl1);
-                mma_f16(o_r[grp + j], c0.ra, c1.ra, c0.rb, c1.rb, wl0, wl1);
-              }
+          for (int u = 0; u < PP; ++u) {
+            w[u] = *reinterpret_cast<const uint4*>(tile[u] + S::TILE + (pair * 32 + lane) * 16);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint4 f0 = vs0[u][pair >> 1], f1 = vs1[u][pair >> 1];
+              const uint32_t s0 = (pair & 1) ? (j ? f0.w : f0.z) : (j ? f0.y : f0.x);
+              const uint32_t s1 = (pair & 1) ? (j ? f1.w : f1.z) : (j ? f1.y : f1.x);
+              wh[u][j][0] = hmul2_u32(ph[u][0], s0), wh[u][j][1] = hmul2_u32(ph[u][1], s1);
+              wl[u][j][0] = hfma2_u32(pl[u][0], s0, hfma2_u32(ph[u][0], s0, wh[u][j][0] ^ 0x80008000u));
+              wl[u][j][1] = hfma2_u32(pl[u][1], s1, hfma2_u32(ph[u][1], s1, wh[u][j][1] ^ 0x80008000u));
             }
           }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            cu[j][0] = cu[j][1] = cu[j][2] = cu[j][3] = 0.0f;
+            cr[j][0] = cr[j][1] = cr[j][2] = cr[j][3] = 0.0f;
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int u = 0; u < PP; ++u)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const U4Word c0(j ? w[u].z : w[u].x), c1(j ? w[u].w : w[u].y);
+                const uint32_t b0 = part ? wh[u][j][0] : wl[u][j][0], b1 = part ? wh[u][j][1] : wl[u][j][1];
+                mma_f16(cu[j], c0.a_hi, c1.a_hi, c0.b_hi, c1.b_hi, b0, b1);
+                mma_f16(cr[j], c0.a_lo, c1.a_lo, c0.b_lo, c1.b_lo, b0, b1);
+              }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              o_hi[pair * 2 + j][c] += cu[j][c];
+              o_lo[pair * 2 + j][c] += cr[j][c];
+            }
         }
       }
       __syncwarp();
@@ -573,8 +610,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
 #pragma unroll
       for (int c = 0; c < 4; ++c) {   // (dim g + 8 * (c / 2); head 2t + c % 2)
         float* to = ow + (2 * t + (c & 1)) * S::OPAD + grp * QGROUP + g + 8 * (c >> 1);
-        to[0] = fmaf(o_r[grp][c], 16777216.0f, o_b[grp][c & 1]);
-        to[16] = fmaf(o_u[grp][c] - o_r[grp][c], 1048576.0f, o_b[grp][c & 1]);   // 2^24 / 16
+        to[0] = o_lo[grp][c] + o_b[grp][c & 1];
+        to[16] = fmaf(o_hi[grp][c], 0.0625f, o_b[grp][c & 1]);
       }
     if (g == 0) {
       ml_s[(warp * 8 + 2 * t) * 2] = m0;
