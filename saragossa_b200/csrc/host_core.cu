@@ -311,8 +311,11 @@ int create_batch(State* st, Kv** kvs, int n, Batch** out) {
     slots.push_back(kvs[i]->seq->slot);
   }
   const int heads = std::max(b->q_heads, b->pool->kv_heads);
-  // Splits never need to exceed about two blocks per SM for the whole launch.
-  int by_sm = (2 * st->sm_count) / (n * b->pool->kv_heads);
+  // Splits never need to exceed the blocks that are resident at once.
+  const int blocks_per_sm = attention_u4_supported(b->pool->dtype, b->pool->head_dim, b->q_heads / b->pool->kv_heads)
+                                ? attention_u4_blocks_per_sm(b->pool->head_dim)
+                                : 2;
+  int by_sm = (blocks_per_sm * st->sm_count) / (n * b->pool->kv_heads);
   b->uniform_splits = std::min(144, std::max(1, by_sm));  // two merge levels of at most 12 partials each
   // an uneven batch cuts its long sequences finer than that (the workspace is sized for it)
   b->max_splits = n > 1 ? std::max(b->uniform_splits, 16) : b->uniform_splits;
@@ -361,7 +364,7 @@ int Batch::choose_splits(int kernel, int64_t max_rows) const {
     // with the best whole-wave fill (first one above 98.5%), while every split
     // keeps a few pages of work.
     const int heads = kernel >= 2 ? pool->kv_heads : q_heads;
-    const int64_t slots = int64_t(st->sm_count) * (kernel >= 2 ? 2 : 8);
+    const int64_t slots = int64_t(st->sm_count) * (kernel == 4 ? attention_u4_blocks_per_sm(pool->head_dim) : kernel >= 2 ? 2 : 8);
     const int64_t units = int64_t(heads) * n();
     const int64_t pages = (max_rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
     const int min_pages = kernel >= 2 ? 8 : 2;
@@ -553,7 +556,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       lo = std::min(lo, pages), hi = std::max(hi, pages), total += pages;
     }
     if (hi * 4 > lo * 5 && hi >= 32) {
-      const int64_t slots = int64_t(st->sm_count) * 2;
+      const int64_t slots = int64_t(st->sm_count) * (kernel == 4 ? attention_u4_blocks_per_sm(pool->head_dim) : 2);
       int64_t pps = (total * pool->kv_heads + slots * 3 - 1) / (slots * 3);
       pps = std::max<int64_t>(pps, 8);
       const int64_t need = (hi + pps - 1) / pps + 1;   // one spare: lengths grow while a graph is replayed
@@ -588,8 +591,8 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       return e ? std::atoi(e) : 0;
     }();
     if (kernel == 3) a.n_stages = attention_u8_max_stages(pool->head_dim);
-    if (kernel == 4) a.n_stages = attention_u4_max_stages(pool->head_dim);
     if (env_stages >= 4 && env_stages <= a.n_stages) a.n_stages = env_stages / 4 * 4;
+    if (kernel == 4) a.n_stages = attention_u4_stages(pool->head_dim);   // fixed
 #ifdef SGK_TRACE
     a.trace = g_trace;
     if (g_trace && g_trace_timeline) {
@@ -605,7 +608,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     static const bool shared_merge_off = std::getenv("SGK_NO_SHARED_MERGE") != nullptr;
     if (!shared_merge_off && a.pages_per_split == 0 && a.splits > 12 && a.splits <= 160) {
       if (resident_per_sm < 0 || resident_stages != a.n_stages)   // asked once per batch
-        resident_per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim, a.n_stages)
+        resident_per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim)
                           : kernel == 3 ? attention_u8_resident_blocks(pool->head_dim, a.n_stages)
                                       : attention_mma_resident_blocks(pool->head_dim, a.n_stages),
         resident_stages = a.n_stages;
@@ -636,7 +639,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
         cluster_stages = a.n_stages;
       }
       if (max_clusters[a.splits] < 0)
-        max_clusters[a.splits] = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, a.n_stages, a.splits)
+        max_clusters[a.splits] = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, a.splits)
                                  : kernel == 3 ? attention_u8_max_clusters(pool->head_dim, a.n_stages, a.splits)
                                              : attention_mma_max_clusters(pool->head_dim, a.n_stages, a.splits);
       a.cluster_merge = int64_t(pool->kv_heads) * n() <= max_clusters[a.splits];

@@ -136,9 +136,10 @@ int attention_u8_max_clusters(int head_dim, int n_stages, int splits);
 bool attention_u4_supported(int dtype, int head_dim, int gqa);
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream);
 cudaError_t attention_u4_configure();
-int attention_u4_max_stages(int head_dim);
-int attention_u4_resident_blocks(int head_dim, int n_stages);
-int attention_u4_max_clusters(int head_dim, int n_stages, int splits);
+int attention_u4_blocks_per_sm(int head_dim);
+int attention_u4_stages(int head_dim);
+int attention_u4_resident_blocks(int head_dim);
+int attention_u4_max_clusters(int head_dim, int splits);
 
 // Gather rows [row0, row0+n) of one layer into contiguous [n, kv_dim] arrays.
 // mode 0: storage type (f32 / bf16 bits), 1: decoded f32, 2: u8 or u4 codes (a byte each) + scale + bias.

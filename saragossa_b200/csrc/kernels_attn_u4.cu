@@ -37,6 +37,41 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same onto nothing: c = a b
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // (x, y) += (a, b)
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(x, y)), "l"(pair_of(a, b)));
+  unpair(r, x, y);
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float c, float d) {   // (x, y) += (a, b) * (c, d)
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a, b)), "l"(pair_of(c, d)), "l"(pair_of(x, y)));
+  unpair(r, x, y);
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x, y) *= (a, b)
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(x, y)), "l"(pair_of(a, b)));
+  unpair(r, x, y);
+}
+// 2^x; results below 2^-126 are zero
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void mma_bf16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -62,27 +97,52 @@ __device__ __forceinline__ uint32_t hsub2_u32(uint32_t a, uint32_t b) {
   __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t hfma2_u32(uint32_t a, uint32_t b, uint32_t c) {
+__device__ __forceinline__ uint32_t hfma2_u32(uint32_t a, uint32_t b, uint32_t c) {   // a b + c
   __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// A word's eight codes as four A registers: bytes 0, 2 and bytes 1, 3, their low codes n0 and 16 times their high
-// ones, as fp16 numbers. (0x6400 | byte) is 1024 + byte, so n0 = (1024 + n0) - 1024 and 16 n1 = (1024 + byte) - (1024 + n0),
-// both exact. (As fp16 subnormals, without the subtraction, the codes would cost half the instructions and most of the
-// accumulator's digits: the matrix unit aligns its products by their exponent fields, and a subnormal's field
-// lies up to ten bits above its value. Scores were off by 1e-5.)
+__device__ __forceinline__ uint32_t hfms2_u32(uint32_t a, uint32_t b, uint32_t c) {   // a b - c
+  __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), __hneg2(*reinterpret_cast<__half2*>(&c)));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {   // (a & b) | c as one instruction
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// A word's eight codes as four A registers: bytes 0, 2 and bytes 1, 3, as whole bytes u = 16 n1 + n0 and as low codes n0.
+// u goes to the matrix unit as the fp16 subnormal u * 2^-24: one mask or permute. n0 must be a normal number,
+// (1024 + n0) - 1024: the unit aligns its products by their exponent fields, and a subnormal's field lies up to ten
+// bits above its value, digits that the accumulator loses. u is largest in the field and its share of the result is
+// divided by 16, so there it does not matter (with n0 a subnormal too, scores were off by 1e-5).
+// BASE: the fp16 number whose mantissa takes n0: 0x6400 (1024) gives n0, 0x2c00 gives n0 * 2^-14.
+template <uint32_t BASE>
 struct U4Word {
-  uint32_t a_lo, b_lo, a_hi, b_hi;
+  uint32_t a_u, b_u, a_n, b_n;
   __device__ __forceinline__ explicit U4Word(uint32_t w) {
-    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4240), b = __byte_perm(w, 0x64646464u, 0x4341);
-    const uint32_t a0 = a & 0xff0fff0fu, b0 = b & 0xff0fff0fu;
-    a_lo = hsub2_u32(a0, 0x64006400u);
-    b_lo = hsub2_u32(b0, 0x64006400u);
-    a_hi = hsub2_u32(a, a0);
-    b_hi = hsub2_u32(b, b0);
+    constexpr uint32_t base = BASE * 0x10001u;
+    a_u = w & 0x00ff00ffu;
+    b_u = __byte_perm(w, 0u, 0x4341);
+    a_n = hsub2_u32(and_or(w, 0x000f000fu, base), base);
+    b_n = hsub2_u32(and_or(b_u, 0x000f000fu, base), base);
   }
 };
 
+constexpr int U4_WARPS = MMA_CONSUMERS;
+constexpr int U4_THREADS = U4_WARPS * 32;
+// Launch shape by head size; registers and shared memory are split evenly among the resident blocks.
+template <int HD>
+struct U4Shape;
+template <>
+struct U4Shape<128> {
+  static constexpr int BLOCKS = 3;   // resident per SM
+  static constexpr int PAGES = 2;    // a warp works on at once
+  static constexpr int SLOTS = 4;    // stages of a warp, a multiple of PAGES
+};
+template <>
+struct U4Shape<256> {
+  static constexpr int BLOCKS = 2, PAGES = 1, SLOTS = 4;
+};
 constexpr float U4_LIMIT = 14.0f;   // p'' <= 2^14
 constexpr float U4_LEVEL = 6.0f;    // p'' of the largest z when the reference moves
 
@@ -94,24 +154,22 @@ struct U4Smem {
   static constexpr int POWERS = BIASES + PAGE_TOKENS * G * 2; // 8 x bf16
   static constexpr int TILE = POWERS + 16;
   static constexpr int STAGE = 2 * TILE;
+  static constexpr int SLOTS = U4Shape<HD>::SLOTS;
   static constexpr int OPAD = HD + 4;
   static constexpr int Q_BYTES = G * 2 * 32 * 16;             // B fragments: [group][high | low dims][lane]{hi, lo}
   static constexpr int QROWS_BYTES = 8 * HD * 4;              // q in f32 while the fragments are made
   static constexpr int QSUM_BYTES = 8 * 8 * 4 + 8 * 4;        // [head][8 groups], absent groups zero; power of two per head
-  static constexpr int O_BYTES = MMA_CONSUMERS * 8 * OPAD * 4;
+  static constexpr int O_BYTES = U4_WARPS * 8 * OPAD * 4;
   static constexpr int ML_BYTES = 512;
-  static constexpr int BAR_BYTES = 2 * MMA_MAX_STAGES * 8;
+  static constexpr int BAR_BYTES = U4_WARPS * SLOTS * 8;
   // the row of a fused append: f32 K and V, afterwards its bytes (codes K | V, then 4 G + 1 half words)
   static constexpr int NEW_BYTES = 2 * HD * 4;
   static constexpr int RECV_BYTES = ClusterRecv<HD>::BYTES;
   static constexpr int FIXED = Q_BYTES + QROWS_BYTES + QSUM_BYTES + ML_BYTES + BAR_BYTES + 64 + NEW_BYTES + RECV_BYTES;
-  __host__ __device__ static size_t ring_bytes(int stages) {
-    size_t r = size_t(stages) * STAGE;
-    r = r > size_t(O_BYTES) ? r : size_t(O_BYTES);
-    return (r + 15) / 16 * 16;
-  }
-  static size_t total(int stages) { return ring_bytes(stages) + FIXED + 128; }
+  static constexpr int RING_BYTES = U4_WARPS * SLOTS * STAGE > O_BYTES ? U4_WARPS * SLOTS * STAGE : O_BYTES;
+  static constexpr int TOTAL = RING_BYTES + FIXED;
   static_assert(STAGE % 16 == 0 && TILE % 16 == 0 && QSUM_BYTES % 16 == 0, "16-byte pieces");
+  static_assert(RING_BYTES % 16 == 0 && BAR_BYTES % 16 == 0, "16-byte pieces");
 };
 
 // Writes the row that a fused append has quantised (`park`) into a tile pair in global or shared memory; one warp.
@@ -136,31 +194,32 @@ __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park
   if (lane == 0) *reinterpret_cast<uint16_t*>((rin < 8 ? ktile : vtile) + u4_pow_offset(rin, HD)) = meta[4 * S::G];
 }
 
-// PP: pages a warp works on at once. Two (head_dim 128) give the chains of matrix instructions twice
-// the independent work and share the query's fragments; with head_dim 256 one page fills the registers.
+// PP: pages a warp works on at once. Two (head_dim 128) give the chains of matrix instructions twice the
+// independent work and share the query's fragments and the bookkeeping; with head_dim 256 one page fills the registers.
 template <int HD, bool CLUSTER, bool PEERS>
-__global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_kernel(AttnArgs a) {
   using S = U4Smem<HD>;
   constexpr int G = S::G;
-  constexpr int PP = HD == 128 ? 2 : 1;
+    constexpr int PP = U4Shape<HD>::PAGES;
   constexpr int SETS = G / 4;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-  const int nst = a.n_stages;
-  uint8_t* q_frag = ring + S::ring_bytes(nst);
+  // (not rounded up by hand: an address that went through an integer is a generic one to the compiler, and its loads too)
+  extern __shared__ __align__(128) uint8_t u4_smem[];
+  uint8_t* ring = u4_smem;
+  uint8_t* q_frag = ring + S::RING_BYTES;
   float* q_rows = reinterpret_cast<float*>(q_frag + S::Q_BYTES);          // [8][HD]
   float* qsum_s = q_rows + 8 * HD;                                        // [8][8]
   float* qpow_s = qsum_s + 64;                                            // [8]
   float* o_s = reinterpret_cast<float*>(ring);    // aliases the ring once it has drained
   float* ml_s = qpow_s + 8;                                               // [warps][8][2]
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(ml_s) + S::ML_BYTES);
-  int* flags = reinterpret_cast<int*>(bars + 2 * MMA_MAX_STAGES);
+  int* flags = reinterpret_cast<int*>(bars + U4_WARPS * S::SLOTS);
   float* new_s = reinterpret_cast<float*>(flags + 16);
   float* recv_s = new_s + 2 * HD;
   volatile int* abort_flag = flags;
 
   const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform over the warp, and known to be
   const int gqa = a.q_heads / a.pool.kv_heads;
   const int slot = a.slots ? a.slots[seq] : a.slot0;
   int32_t* len_ptr = a.pool.lens + int64_t(slot) * a.pool.layers + a.layer;
@@ -190,27 +249,40 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
   const int64_t head_off = int64_t(a.layer) * a.pool.layer_bytes + int64_t(kvh) * 2 * a.pool.tile_bytes;
   const bool owns_append = do_append && pe == n_pages && my_pages > 0;   // the new row lies in the last page
 
-  int32_t first_entry = -1;
-  if (warp == MMA_CONSUMERS) {
-    if (lane == 0) {
-      flags[0] = 0;
-      flags[1] = 0;
-      flags[5] = 0;   // set once the quantised row of a fused append is parked in shared memory
-      for (int s = 0; s < nst; ++s) {
-        mbar_init(smem_u32(bars + s), 1);
-        mbar_init(smem_u32(bars + MMA_MAX_STAGES + s), 1);
-      }
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  // Every warp owns every fourth stage of the ring and fetches its own pages: its n-th page has ordinal pb + warp + 4 n
+  // and goes to its stage n % SLOTS, one bulk copy per page, completion on the stage's barrier. A stage is refilled by the
+  // warp itself as soon as it has used it up, so no second barrier and no producer stand between the two (a producer warp
+  // needed about 640 cycles per page, waiting for the consumers' releases one by one).
+  // Lane l holds the block-table entries of the warp's pages 32 k + l: batch k and the one after it.
+  constexpr int SLOTS = S::SLOTS;
+  const int count = (my_pages - warp + U4_WARPS - 1) / U4_WARPS;   // this warp's pages
+  const auto entry_of = [&](int n) { return n < count ? table[map.page(pb + warp + U4_WARPS * n)] : -1; };
+  int32_t entries = entry_of(lane), entries_next = entry_of(32 + lane);
+  uint64_t* my_bars = bars + warp * SLOTS;
+  uint8_t* my_ring = ring + warp * SLOTS * S::STAGE;
+  const uint64_t policy = l2_policy_evict_first();
+  const auto fetch = [&](int slot_at, int32_t page) {   // one lane
+    if (page < 0 || page >= a.num_pages) {
+      atomicExch(a.status, DEV_ERR_BAD_PAGE);
+      *abort_flag = 1;
+      return;
     }
-    if (lane < my_pages) first_entry = table[map.page(pb + lane)];
-    __syncwarp();
-    asm volatile("bar.arrive 3, %0;" ::"r"(MMA_THREADS) : "memory");
-    // ---------------- producer warp ----------------
-    produce_pages<S::STAGE>(a, table, pb, my_pages, first_entry, ring, bars, nst, head_off, abort_flag, lane, map);
-    if (a.pdl_wait) pdl_wait();   // the tail writes to memory the earlier launch may still be using
-  } else {
-    // ---------------- consumer warps: the query first ----------------
+    const uint32_t bar = smem_u32(my_bars + slot_at);
+    mbar_expect_tx(bar, S::STAGE);
+    bulk_copy_g2s(smem_u32(my_ring + slot_at * S::STAGE), a.pool.base + int64_t(page) * a.pool.page_bytes + head_off, S::STAGE, bar, policy);
+  };
+  if (tid == 0) {
+    flags[0] = 0;   // a wait ran out, or a bad table entry
+    flags[1] = 0;
+    flags[5] = 0;   // set once the quantised row of a fused append is parked in shared memory
+  }
+  if (lane < SLOTS) mbar_init(smem_u32(my_bars + lane), 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  if (lane < SLOTS && lane < count) fetch(lane, entries);
+  {
+    // ---------------- the query ----------------
     constexpr int NV = HD / 64;
     const float* q = a.q + (int64_t(seq) * a.q_heads + int64_t(kvh) * gqa) * HD;
     // q and the row to append come from the launch before this one; the cursor, the block table and
@@ -219,7 +291,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
     float4 v[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int f = (tid + k * MMA_CONSUMERS * 32) * 4;
+      const int f = (tid + k * U4_THREADS) * 4;
       v[k] = (f / HD < gqa) ? __ldg(reinterpret_cast<const float4*>(q + f)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (owns_append && tid * 4 < 2 * HD) {
@@ -230,12 +302,12 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
     if (owns_append && tid == 0) flags[2] = table[len_old / PAGE_TOKENS];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int f = (tid + k * MMA_CONSUMERS * 32) * 4;
+      const int f = (tid + k * U4_THREADS) * 4;
       v[k].x *= a.scale_log2e, v[k].y *= a.scale_log2e, v[k].z *= a.scale_log2e, v[k].w *= a.scale_log2e;
       *reinterpret_cast<float4*>(q_rows + f) = v[k];
     }
-    asm volatile("bar.sync 1, %0;" ::"r"(MMA_CONSUMERS * 32) : "memory");
-    // Two heads per warp: sums of the groups, and the power of two that brings the largest |q| to 2^12..2^13.
+    __syncthreads();
+    // Two heads per warp: sums of the groups, and the power of two that brings the largest |q| to 2^15..2^16.
 #pragma unroll
     for (int h = 2 * warp; h < 2 * warp + 2; ++h) {
       float big = 0.0f;
@@ -252,17 +324,19 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
       asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(big) : "f"(big));
       if (lane == 0) {
         const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
-        qpow_s[h] = pow2f(max(-90, min(90, e - 12)));   // q = qpow * (what the fragments hold)
+        qpow_s[h] = pow2f(max(-90, min(90, e - 15)));   // q = qpow * (what the fragments hold)
       }
     }
-    asm volatile("bar.sync 1, %0;" ::"r"(MMA_CONSUMERS * 32) : "memory");
-    for (int i = tid; i < G * 32; i += MMA_CONSUMERS * 32) {
+    __syncthreads();
+    for (int i = tid; i < G * 32; i += U4_THREADS) {
       const int grp = i >> 5, h = (i & 31) >> 2, t = i & 3;
       const float inv = 1.0f / qpow_s[h];
       const float* row = q_rows + h * HD + grp * QGROUP + 4 * t;
       const float4 x = *reinterpret_cast<const float4*>(row), y = *reinterpret_cast<const float4*>(row + 16);
-      const float u[4] = {y.x * inv * 0.0625f, y.y * inv * 0.0625f, y.z * inv * 0.0625f, y.w * inv * 0.0625f};
-      const float r[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+      // n0 x + n1 y = n0 (x - y / 16) + u (y / 16), with u in units of 2^-24 and n0 in units of 2^-14
+      const float s = inv * 0.0625f, d = 0x1p-10f;
+      const float u[4] = {y.x * s, y.y * s, y.z * s, y.w * s};
+      const float r[4] = {fmaf(x.x, inv, -u[0]) * d, fmaf(x.y, inv, -u[1]) * d, fmaf(x.z, inv, -u[2]) * d, fmaf(x.w, inv, -u[3]) * d};
       // k-slots (2t, 2t+1) are the bytes 0 and 2 of a word, (2t+8, 2t+9) the bytes 1 and 3
       uint4 fu, fr;
       fu.x = pack_f16(u[0], u[2]), fu.y = pack_f16(u[1], u[3]);
@@ -288,14 +362,14 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
       else qs0 = hi, qs1 = mid, qs2 = lo;
     }
     const int g = lane >> 2, t = lane & 3;
-    const float ch0 = qpow_s[2 * t], ch1 = qpow_s[2 * t + 1];
-    asm volatile("bar.sync 3, %0;" ::"r"(MMA_THREADS) : "memory");   // fragments written; barriers initialised
+    const float ch0 = qpow_s[2 * t] * 16777216.0f, ch1 = qpow_s[2 * t + 1] * 16777216.0f;   // products are in units of 2^-24
+    __syncthreads();   // fragments written
 
     // The row of a fused append is quantised now, by the warp with the fewest pages, while the first pages are
     // on their way; its bytes go to the page in global memory and stay parked in shared memory for the warp
     // that will meet the page in the ring.
     uint8_t* park = reinterpret_cast<uint8_t*>(new_s);
-    if (owns_append && warp == MMA_CONSUMERS - 1) {
+    if (owns_append && warp == U4_WARPS - 1) {
       const int rin = len_old % PAGE_TOKENS;
       const uint32_t odd = rin & 1;
       const int32_t page = flags[2];
@@ -337,43 +411,62 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
     }
 
     // ---------------- the pages ----------------
-    float o_hi[G][4], o_lo[G][4], o_b[G][2];
+    float o_hi[G][4], o_lo[G][4], o_b[2][G];   // o_b: V biases, [head 2t, 2t + 1][group]
 #pragma unroll
     for (int grp = 0; grp < G; ++grp) {
       o_hi[grp][0] = o_hi[grp][1] = o_hi[grp][2] = o_hi[grp][3] = 0.0f;
       o_lo[grp][0] = o_lo[grp][1] = o_lo[grp][2] = o_lo[grp][3] = 0.0f;
-      o_b[grp][0] = o_b[grp][1] = 0.0f;
+      o_b[0][grp] = o_b[1][grp] = 0.0f;
     }
     float m0 = -1.0e30f, m1 = -1.0e30f, l0 = 0.0f, l1 = 0.0f;
     const int k_off = g * (HD / 2) + t * 16;                                  // + (set ^ odd row) * 64; row g + 8: + 4 * HD
     const int kb_off = S::BIASES + g * G * 2 + (G == 4 ? (t & 1) : t) * 4;    // K biases of row g
     const int vs_off = S::TILE + S::STEPS + t * G * 4;                        // V factors of rows 2t, 2t+1; rows + 8: + 16 * G
     const int vb_off = S::TILE + S::BIASES + g * G * 2;                       // V biases of row g; row g + 8: + 16 * G
-    int stage = warp;
-    uint32_t parity = 0;
-    for (int i = warp; i < my_pages; i += MMA_CONSUMERS * PP) {
-      uint8_t* tile[PP];
-      int stages[PP];
+    // Iterations that are not like the others: a page is not seen whole (the last of the sinks, the window's first, the
+    // last), takes the appended row, or is missing because the warp's pages are an odd number.
+    const auto next_special = [&](int from) {
+      int best = INT32_MAX;
+      const auto consider = [&](int v) {   // ordinal of a page
+        const int k = v - pb - warp;
+        if (k >= 0 && k % U4_WARPS == 0 && k / U4_WARPS < count) {
+          const int at = k / U4_WARPS / PP * PP;
+          if (at >= from) best = min(best, at);
+        }
+      };
+      if (sinks % PAGE_TOKENS) consider(sink_pages - 1);
+      if (ws % PAGE_TOKENS) consider(sink_pages);
+      if (len % PAGE_TOKENS || do_append) consider(n_pages - 1);
+      if (count % PP && count - count % PP >= from) best = min(best, count - count % PP);
+      return best;
+    };
+    int special_at = next_special(0);
+    int at = 0, phase = 0;   // stage of the iteration's first page
+    int batch = 0;           // first page of the entries held
+    for (int n = 0; n < count; n += PP) {
+      const uint8_t* tile[PP];
       bool ok = true;
-      bool whole = true;   // every row of the pages is seen
-      int row_base[PP];
 #pragma unroll
       for (int u = 0; u < PP; ++u) {
-        stages[u] = stage;
-        tile[u] = ring + stage * S::STAGE;
-        const int v = pb + i + u * MMA_CONSUMERS;
-        const bool there = u == 0 || i + u * MMA_CONSUMERS < my_pages;
-        row_base[u] = there ? static_cast<int>(map.page(v)) * PAGE_TOKENS : 0x40000000;   // past every length
-        whole = whole && row_base[u] <= len - PAGE_TOKENS && (row_base[u] >= ws || row_base[u] <= sinks - PAGE_TOKENS);
-        if (there) {
-          ok = mbar_wait(smem_u32(bars + stage), parity, abort_flag, a.status) && ok;
-          stage += MMA_CONSUMERS;   // the stage count is a multiple of the consumer count
-          if (stage >= nst) {
-            stage -= nst;
-            parity ^= 1;
-          }
+        const int slot_at = at + (u > 0 && n + u >= count ? 0 : u);   // a missing page stands in for itself by the first one
+        tile[u] = my_ring + slot_at * S::STAGE;
+        const uint32_t bar = smem_u32(my_bars + slot_at);
+        if (!mbar_try_wait(bar, phase)) ok = mbar_wait(bar, phase, abort_flag, a.status) && ok;
+      }
+      if (!ok) {
+        // gave up (reported): the copies still on their way are waited for, with the short bound, before the block leaves
+        for (int k = n; k < count && k < n + SLOTS; ++k) {
+          int slot_at = at + (k - n), ph = phase;
+          if (slot_at >= SLOTS) slot_at -= SLOTS, ph ^= 1;
+          mbar_wait(smem_u32(my_bars + slot_at), ph, abort_flag, a.status);
         }
-        if (there && owns_append && v == n_pages - 1 && ok) {
+        break;
+      }
+      const bool special = n == special_at;
+      if (special) {
+        special_at = next_special(n + PP);
+        const int k = n_pages - 1 - pb - warp - n * U4_WARPS;   // the last page is the iteration's page k / 4
+        if (owns_append && k >= 0 && k < PP * U4_WARPS && k % U4_WARPS == 0) {
           // the new row joins the staged copy
           uint32_t spins = 0;
           while (*reinterpret_cast<volatile int*>(flags + 5) == 0) {
@@ -384,11 +477,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
             }
           }
           __syncwarp();
-          u4_place_row<HD>(tile[u], park, len_old % PAGE_TOKENS, lane);
+          u4_place_row<HD>(my_ring + (at + k / U4_WARPS) * S::STAGE, park, len_old % PAGE_TOKENS, lane);
           __syncwarp();
         }
       }
-      if (ok) {
+      {
         // ---- scores ----
         float z[PP][4];   // (row g; heads 2t, 2t+1), (row g + 8; ...)
         float acc[PP][4][4];
@@ -402,8 +495,6 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
             const int at = k_off + (SETS > 1 ? (set ^ (g & 1)) : 0) * 64;
             w0[u] = *reinterpret_cast<const uint4*>(tile[u] + at);
             w1[u] = *reinterpret_cast<const uint4*>(tile[u] + at + 4 * HD);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.0f;
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -413,11 +504,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
             for (int u = 0; u < PP; ++u) {
               const uint32_t x0 = j == 0 ? w0[u].x : j == 1 ? w0[u].y : j == 2 ? w0[u].z : w0[u].w;
               const uint32_t x1 = j == 0 ? w1[u].x : j == 1 ? w1[u].y : j == 2 ? w1[u].z : w1[u].w;
-              const U4Word c0(x0), c1(x1);
-              mma_f16(acc[u][j], c0.a_hi, c1.a_hi, c0.b_hi, c1.b_hi, fu.z, fu.w);   // the small parts first: the
-              mma_f16(acc[u][j], c0.a_lo, c1.a_lo, c0.b_lo, c1.b_lo, fr.z, fr.w);   // accumulator is truncated after
-              mma_f16(acc[u][j], c0.a_lo, c1.a_lo, c0.b_lo, c1.b_lo, fr.x, fr.y);   // every product
-              mma_f16(acc[u][j], c0.a_hi, c1.a_hi, c0.b_hi, c1.b_hi, fu.x, fu.y);
+              const U4Word<0x2c00> c0(x0), c1(x1);
+              mma_f16_zero(acc[u][j], c0.a_u, c1.a_u, c0.b_u, c1.b_u, fu.z, fu.w);   // the small parts first: the
+              mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.z, fr.w);   // accumulator is truncated after
+              mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.x, fr.y);   // every product
+              mma_f16(acc[u][j], c0.a_u, c1.a_u, c0.b_u, c1.b_u, fu.x, fu.y);
             }
           }
 #pragma unroll
@@ -450,10 +541,9 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
           const uint32_t b1 = *reinterpret_cast<const uint32_t*>(tile[u] + kb_off + 16 * G);
           mma_bf16(sb, b0, b1, b0, b1, qs0, qs1);
           if (G == 8) mma_bf16_k8(sb, b0, b1, qs2);
-          z[u][0] = fmaf(z[u][0], ch0, sb[0]);
-          z[u][1] = fmaf(z[u][1], ch1, sb[1]);
-          z[u][2] = fmaf(z[u][2], ch0, sb[2]);
-          z[u][3] = fmaf(z[u][3], ch1, sb[3]);
+          fma2(sb[0], sb[1], z[u][0], z[u][1], ch0, ch1);
+          fma2(sb[2], sb[3], z[u][2], z[u][3], ch0, ch1);
+          z[u][0] = sb[0], z[u][1] = sb[1], z[u][2] = sb[2], z[u][3] = sb[3];
         }
         uint4 vs0[PP][SETS], vs1[PP][SETS];   // V factors: rows (2t, 2t+1) and (2t+8, 2t+9)
         uint2 vb0[PP][SETS], vb1[PP][SETS];   // V biases: rows g and g + 8
@@ -466,12 +556,14 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
             vb0[u][set] = *reinterpret_cast<const uint2*>(tile[u] + vb_off + set * 8);
             vb1[u][set] = *reinterpret_cast<const uint2*>(tile[u] + vb_off + 16 * G + set * 8);
           }
-        if (!whole) {
+        if (special) {
           // A row that is not seen weighs nothing, whatever its bytes say.
 #pragma unroll
           for (int u = 0; u < PP; ++u) {
+            const int v = pb + warp + U4_WARPS * (n + u);
+            const int base = u == 0 || n + u < count ? (v + (v >= sink_pages ? p_first - sink_pages : 0)) * PAGE_TOKENS : len;
             const auto seen = [&](int r) {
-              const int row = row_base[u] + r;
+              const int row = base + r;
               return row < len && (row < sinks || row >= ws);
             };
             const bool s0 = seen(g), s1 = seen(g + 8);
@@ -503,8 +595,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
           l1 *= al1;
 #pragma unroll
           for (int grp = 0; grp < G; ++grp) {
-            o_hi[grp][0] *= al0, o_hi[grp][2] *= al0, o_lo[grp][0] *= al0, o_lo[grp][2] *= al0, o_b[grp][0] *= al0;
-            o_hi[grp][1] *= al1, o_hi[grp][3] *= al1, o_lo[grp][1] *= al1, o_lo[grp][3] *= al1, o_b[grp][1] *= al1;
+            o_hi[grp][0] *= al0, o_hi[grp][2] *= al0, o_lo[grp][0] *= al0, o_lo[grp][2] *= al0, o_b[0][grp] *= al0;
+            o_hi[grp][1] *= al1, o_hi[grp][3] *= al1, o_lo[grp][1] *= al1, o_lo[grp][3] *= al1, o_b[1][grp] *= al1;
           }
           m0 = mn0;
           m1 = mn1;
@@ -513,29 +605,33 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
         uint32_t ph[PP][2], pl[PP][2];
 #pragma unroll
         for (int u = 0; u < PP; ++u) {
-          float p[4];
-          p[0] = exp2f(z[u][0] - m0);
-          p[1] = exp2f(z[u][1] - m1);
-          p[2] = exp2f(z[u][2] - m0);
-          p[3] = exp2f(z[u][3] - m1);
+          add2(z[u][0], z[u][1], -m0, -m1);
+          add2(z[u][2], z[u][3], -m0, -m1);
+          float p[4] = {exp2_ftz(z[u][0]), exp2_ftz(z[u][1]), exp2_ftz(z[u][2]), exp2_ftz(z[u][3])};
           const uint32_t h0 = pack_f16(p[0], p[1]), h1 = pack_f16(p[2], p[3]);
           const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
-          const uint32_t d0 = pack_f16(p[0] - f0.x, p[1] - f0.y), d1 = pack_f16(p[2] - f1.x, p[3] - f1.y);
+          float d[4] = {p[0], p[1], p[2], p[3]};
+          add2(d[0], d[1], -f0.x, -f0.y);
+          add2(d[2], d[3], -f1.x, -f1.y);
+          const uint32_t d0 = pack_f16(d[0], d[1]), d1 = pack_f16(d[2], d[3]);
           // (row g; heads 2t, 2t+1) -> (rows 2t, 2t+1; head g)
           ph[u][0] = movmatrix_trans(h0), ph[u][1] = movmatrix_trans(h1);
           pl[u][0] = movmatrix_trans(d0), pl[u][1] = movmatrix_trans(d1);
-          p[0] *= back[u][0], p[1] *= back[u][0], p[2] *= back[u][1], p[3] *= back[u][1];
-          l0 += p[0] + p[2];
-          l1 += p[1] + p[3];
+          mul2(p[0], p[1], back[u][0], back[u][0]);
+          mul2(p[2], p[3], back[u][1], back[u][1]);
+          add2(l0, l1, p[0], p[1]);
+          add2(l0, l1, p[2], p[3]);
 #pragma unroll
           for (int set = 0; set < SETS; ++set) {
             const float b0[4] = {bf16_lo_f32(vb0[u][set].x), bf16_hi_f32(vb0[u][set].x), bf16_lo_f32(vb0[u][set].y), bf16_hi_f32(vb0[u][set].y)};
             const float b1[4] = {bf16_lo_f32(vb1[u][set].x), bf16_hi_f32(vb1[u][set].x), bf16_lo_f32(vb1[u][set].y), bf16_hi_f32(vb1[u][set].y)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              o_b[set * 4 + j][0] = fmaf(b0[j], p[0], fmaf(b1[j], p[2], o_b[set * 4 + j][0]));
-              o_b[set * 4 + j][1] = fmaf(b0[j], p[1], fmaf(b1[j], p[3], o_b[set * 4 + j][1]));
-            }
+            for (int j = 0; j < 4; j += 2)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                fma2(o_b[h][set * 4 + j], o_b[h][set * 4 + j + 1], b0[j], b0[j + 1], p[h], p[h]);
+                fma2(o_b[h][set * 4 + j], o_b[h][set * 4 + j + 1], b1[j], b1[j + 1], p[2 + h], p[2 + h]);
+              }
           }
         }
         // ---- outputs. The matrix instruction truncates its f32 sum: hundreds of them in one accumulator shrink it
@@ -555,53 +651,62 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
               const uint32_t s0 = (pair & 1) ? (j ? f0.w : f0.z) : (j ? f0.y : f0.x);
               const uint32_t s1 = (pair & 1) ? (j ? f1.w : f1.z) : (j ? f1.y : f1.x);
               wh[u][j][0] = hmul2_u32(ph[u][0], s0), wh[u][j][1] = hmul2_u32(ph[u][1], s1);
-              wl[u][j][0] = hfma2_u32(pl[u][0], s0, hfma2_u32(ph[u][0], s0, wh[u][j][0] ^ 0x80008000u));
-              wl[u][j][1] = hfma2_u32(pl[u][1], s1, hfma2_u32(ph[u][1], s1, wh[u][j][1] ^ 0x80008000u));
+              wl[u][j][0] = hfma2_u32(pl[u][0], s0, hfms2_u32(ph[u][0], s0, wh[u][j][0]));
+              wl[u][j][1] = hfma2_u32(pl[u][1], s1, hfms2_u32(ph[u][1], s1, wh[u][j][1]));
             }
           }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            cu[j][0] = cu[j][1] = cu[j][2] = cu[j][3] = 0.0f;
-            cr[j][0] = cr[j][1] = cr[j][2] = cr[j][3] = 0.0f;
+          for (int u = 0; u < PP; ++u) {
+            const U4Word<0x6400> c00(w[u].x), c01(w[u].y), c10(w[u].z), c11(w[u].w);
+            const auto add = [&](float(&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+              if (u == 0) mma_f16_zero(c, a0, a1, a2, a3, b0, b1);   // the small parts of the weights first
+              else mma_f16(c, a0, a1, a2, a3, b0, b1);
+            };
+            add(cu[0], c00.a_u, c01.a_u, c00.b_u, c01.b_u, wl[u][0][0], wl[u][0][1]);
+            add(cr[0], c00.a_n, c01.a_n, c00.b_n, c01.b_n, wl[u][0][0], wl[u][0][1]);
+            add(cu[1], c10.a_u, c11.a_u, c10.b_u, c11.b_u, wl[u][1][0], wl[u][1][1]);
+            add(cr[1], c10.a_n, c11.a_n, c10.b_n, c11.b_n, wl[u][1][0], wl[u][1][1]);
+            mma_f16(cu[0], c00.a_u, c01.a_u, c00.b_u, c01.b_u, wh[u][0][0], wh[u][0][1]);
+            mma_f16(cr[0], c00.a_n, c01.a_n, c00.b_n, c01.b_n, wh[u][0][0], wh[u][0][1]);
+            mma_f16(cu[1], c10.a_u, c11.a_u, c10.b_u, c11.b_u, wh[u][1][0], wh[u][1][1]);
+            mma_f16(cr[1], c10.a_n, c11.a_n, c10.b_n, c11.b_n, wh[u][1][0], wh[u][1][1]);
           }
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int u = 0; u < PP; ++u)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const U4Word c0(j ? w[u].z : w[u].x), c1(j ? w[u].w : w[u].y);
-                const uint32_t b0 = part ? wh[u][j][0] : wl[u][j][0], b1 = part ? wh[u][j][1] : wl[u][j][1];
-                mma_f16(cu[j], c0.a_hi, c1.a_hi, c0.b_hi, c1.b_hi, b0, b1);
-                mma_f16(cr[j], c0.a_lo, c1.a_lo, c0.b_lo, c1.b_lo, b0, b1);
-              }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              o_hi[pair * 2 + j][c] += cu[j][c];
-              o_lo[pair * 2 + j][c] += cr[j][c];
+            for (int c = 0; c < 4; c += 2) {
+              add2(o_hi[pair * 2 + j][c], o_hi[pair * 2 + j][c + 1], cu[j][c], cu[j][c + 1]);
+              add2(o_lo[pair * 2 + j][c], o_lo[pair * 2 + j][c + 1], cr[j][c], cr[j][c + 1]);
             }
         }
       }
+      // the warp is done with these stages: their next pages, a lane for each
+      const int next = n + SLOTS;
       __syncwarp();
-      if (lane == 0) {
-#pragma unroll
-        for (int u = 0; u < PP; ++u)
-          if (u == 0 || i + u * MMA_CONSUMERS < my_pages) mbar_arrive(smem_u32(bars + MMA_MAX_STAGES + stages[u]));
+      if (next < count) {   // (uniform)
+        if (next - batch >= 32) {
+          batch += 32;
+          entries = entries_next;
+          entries_next = entry_of(batch + 32 + lane);
+        }
+        // (32 is a multiple of PP: an iteration's entries lie in one batch)
+        const int32_t page = __shfl_sync(0xffffffffu, entries, next - batch + lane);
+        if (lane < PP && next + lane < count) fetch(at + lane, page);
       }
+      at += PP;
+      if (at == SLOTS) at = 0, phase ^= 1;
     }
 
     // ---- hand this warp's state to the merge buffer (it aliases the ring) ----
-    asm volatile("bar.sync 1, %0;" ::"r"(MMA_CONSUMERS * 32) : "memory");
+    __syncthreads();
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, off);
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
 #pragma unroll
       for (int grp = 0; grp < G; ++grp) {
-        o_b[grp][0] += __shfl_xor_sync(0xffffffffu, o_b[grp][0], off);
-        o_b[grp][1] += __shfl_xor_sync(0xffffffffu, o_b[grp][1], off);
+        o_b[0][grp] += __shfl_xor_sync(0xffffffffu, o_b[0][grp], off);
+        o_b[1][grp] += __shfl_xor_sync(0xffffffffu, o_b[1][grp], off);
       }
     }
     float* ow = o_s + warp * 8 * S::OPAD;
@@ -610,8 +715,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
 #pragma unroll
       for (int c = 0; c < 4; ++c) {   // (dim g + 8 * (c / 2); head 2t + c % 2)
         float* to = ow + (2 * t + (c & 1)) * S::OPAD + grp * QGROUP + g + 8 * (c >> 1);
-        to[0] = o_lo[grp][c] + o_b[grp][c & 1];
-        to[16] = fmaf(o_hi[grp][c], 0.0625f, o_b[grp][c & 1]);
+        to[0] = o_lo[grp][c] + o_b[c & 1][grp];
+        to[16] = fmaf(fmaf(o_hi[grp][c], 16777216.0f, -o_lo[grp][c]), 0.0625f, o_b[c & 1][grp]);
       }
     if (g == 0) {
       ml_s[(warp * 8 + 2 * t) * 2] = m0;
@@ -621,7 +726,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u4_kernel(AttnArgs a
     }
   }
   __syncthreads();
-  finish_block<HD, CLUSTER, PEERS>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
+  finish_block<HD, CLUSTER, PEERS, U4_THREADS, 1>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
                                    splits, recv_s);
   if (PEERS) peers_finish(a, tid, flags);
 }
@@ -630,14 +735,8 @@ bool attention_u4_supported(int dtype, int head_dim, int gqa) {
   return dtype == KV_U4G32 && (head_dim == 128 || head_dim == 256) && gqa >= 1 && gqa <= 8;
 }
 
-int attention_u4_max_stages(int head_dim) {
-  size_t budget = 113 * 1024;  // two blocks per SM
-  size_t fixed = head_dim == 128 ? U4Smem<128>::FIXED : U4Smem<256>::FIXED;
-  size_t stage = head_dim == 128 ? U4Smem<128>::STAGE : U4Smem<256>::STAGE;
-  int n = static_cast<int>((budget - fixed - 128) / stage);
-  if (n > MMA_MAX_STAGES) n = MMA_MAX_STAGES;
-  return n / MMA_CONSUMERS * MMA_CONSUMERS;  // a stage always belongs to the same warp
-}
+int attention_u4_blocks_per_sm(int head_dim) { return head_dim == 128 ? U4Shape<128>::BLOCKS : U4Shape<256>::BLOCKS; }
+int attention_u4_stages(int head_dim) { return U4_WARPS * (head_dim == 128 ? U4Smem<128>::SLOTS : U4Smem<256>::SLOTS); }
 
 static const void* u4_kernel(int head_dim, bool cluster, bool peers) {
   if (head_dim == 128)
@@ -648,23 +747,21 @@ static const void* u4_kernel(int head_dim, bool cluster, bool peers) {
          : cluster ? reinterpret_cast<const void*>(attention_u4_kernel<256, true, false>)
                    : reinterpret_cast<const void*>(attention_u4_kernel<256, false, false>);
 }
-static size_t u4_smem(int head_dim, int n_stages) {
-  return head_dim == 128 ? U4Smem<128>::total(n_stages) : U4Smem<256>::total(n_stages);
-}
+static size_t u4_smem_bytes(int head_dim) { return head_dim == 128 ? U4Smem<128>::TOTAL : U4Smem<256>::TOTAL; }
 
-int attention_u4_resident_blocks(int head_dim, int n_stages) {
+int attention_u4_resident_blocks(int head_dim) {
   int blocks = 0;
-  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, u4_kernel(head_dim, false, false), MMA_THREADS,
-                                                                u4_smem(head_dim, n_stages));
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, u4_kernel(head_dim, false, false), U4_THREADS,
+                                                                u4_smem_bytes(head_dim));
   return e == cudaSuccess ? blocks : 0;
 }
 
 // How many clusters of `splits` blocks the device can hold at once (0: such a launch would fail).
-int attention_u4_max_clusters(int head_dim, int n_stages, int splits) {
+int attention_u4_max_clusters(int head_dim, int splits) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, 1, 1);
-  cfg.blockDim = dim3(MMA_THREADS);
-  cfg.dynamicSmemBytes = u4_smem(head_dim, n_stages);
+  cfg.blockDim = dim3(U4_THREADS);
+  cfg.dynamicSmemBytes = u4_smem_bytes(head_dim);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = splits;
@@ -695,8 +792,8 @@ cudaError_t attention_u4_configure() {
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.splits, a.pool.kv_heads, n_seq);
-  cfg.blockDim = dim3(MMA_THREADS);
-  cfg.dynamicSmemBytes = u4_smem(a.pool.head_dim, a.n_stages);
+  cfg.blockDim = dim3(U4_THREADS);
+  cfg.dynamicSmemBytes = u4_smem_bytes(a.pool.head_dim);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n_attr = 0;

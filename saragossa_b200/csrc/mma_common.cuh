@@ -513,11 +513,11 @@ __device__ __forceinline__ void cluster_merge(const AttnArgs& a, const float* re
 // (the {max, sum} pairs of the cell's head and the partial values) before the first
 // use, so a pass costs one L2 round trip and no block barrier. final != 0: writes the
 // normalised output; else writes one un-normalised partial (row dst_row of dst).
-template <int HD, int NT = MMA_THREADS, bool PEERS = false>
+template <int HD, int NT = MMA_THREADS, bool PEERS = false, int CELLS = (NT >= 256 ? 1 : 2)>
 __device__ __forceinline__ void merge_block(const AttnArgs& a, const Partials& src, int stride, int first, int count, int gqa,
                                             int64_t qh0, bool final, const Partials& dst,
                                             int dst_stride, int dst_row, int tid) {
-  constexpr int CELLS = NT >= 256 ? 1 : 2;   // the register budget of a 256-thread block is smaller
+  // CELLS per pass: one where the register budget is smaller
   const int total = gqa * (HD / 4);
   for (int base = 0; base < total; base += CELLS * NT) {
     float2 ml[CELLS][MERGE_MAX];
@@ -576,7 +576,7 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const Partials& s
 // CLUSTER: the kernel instance that is launched as clusters (its splits merge through distributed
 // shared memory). A separate instance, so that the other one is compiled without a trace of that path:
 // with both in one kernel the page loop of the long-stream case lost 1.3 % (register allocation).
-template <int HD, bool CLUSTER, bool PEERS = false, int NT = MMA_THREADS>
+template <int HD, bool CLUSTER, bool PEERS = false, int NT = MMA_THREADS, int CELLS = (NT >= 256 ? 1 : 2)>
 __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s, const float* ml_s, int opad,
                                              int* flags, int seq, int kvh, int split, int gqa, bool do_append,
                                              int32_t* len_ptr, int64_t len, int tid, int splits, float* recv) {
@@ -678,7 +678,7 @@ __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s
     if (splits > 1 && flags[1]) {
       // this block completed its group: merge the group (or everything, if one group)
       const bool single = n_groups == 1;
-      merge_block<HD, NT, PEERS>(a, a.part, a.splits, group_first, group_count, gqa, qh0, single, a.part2,
+      merge_block<HD, NT, PEERS, CELLS>(a, a.part, a.splits, group_first, group_count, gqa, qh0, single, a.part2,
                       a.max_groups, group, tid);
       if (tid == 0) SGK_TP(6);
       if (!single) {
@@ -690,7 +690,7 @@ __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s
         }
         __syncthreads();
         if (flags[1]) {
-          merge_block<HD, NT, PEERS>(a, a.part2, a.max_groups, 0, n_groups, gqa, qh0, true, a.part2,
+          merge_block<HD, NT, PEERS, CELLS>(a, a.part2, a.max_groups, 0, n_groups, gqa, qh0, true, a.part2,
                           a.max_groups, 0, tid);
           if (tid == 0) SGK_TP(7);
         }
