@@ -38,17 +38,20 @@ __device__ __forceinline__ int u4_code(const uint8_t* tile, int hd, int is_v, in
   return (tile[is_v ? u4_v_byte(row, dim, hd) : u4_k_byte(row, dim, hd)] >> (4 * u4_nibble(dim))) & 15;
 }
 
+// One element (row, dim) of a u4 tile decoded to f32 (the product is exact). A V tile is decoded where it lies, behind
+// its K tile.
+__device__ __forceinline__ float load_u4_elem(const uint8_t* tile, int hd, int is_v, int row, int dim) {
+  return fmaf(static_cast<float>(u4_code(tile, hd, is_v, row, dim)), u4_step(tile, hd, is_v, row, dim / QGROUP),
+              bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u4_bias_offset(row, dim / QGROUP, hd))));
+}
+
 // One stored element (row, dim) of a tile decoded to f32: f32 as is, bf16 upcast,
-// u8 q*scale+bias with separate roundings (src/quantization.rs:173-179), u4 the same (there the
-// product is exact). A V tile is decoded where it lies, behind its K tile.
+// u8 q*scale+bias with separate roundings (src/quantization.rs:173-179).
 __device__ __forceinline__ float load_tile_elem(const uint8_t* tile, int dtype, int hd, int is_v,
                                                 int row, int dim) {
   if (dtype == KV_F32) return reinterpret_cast<const float*>(tile)[row * hd + dim];
   if (dtype == KV_BF16)
     return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(tile)[bf16_elem_index(row, dim, hd)]);
-  if (dtype == KV_U4G32)
-    return __fadd_rn(__fmul_rn(static_cast<float>(u4_code(tile, hd, is_v, row, dim)), u4_step(tile, hd, is_v, row, dim / QGROUP)),
-                     bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u4_bias_offset(row, dim / QGROUP, hd))));
   int idx = is_v ? u8_v_code_index(row, dim, hd) : u8_k_code_index(row, dim, hd);
   float scale = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u8_scale_offset(row, dim / QGROUP, hd)));
   float bias = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(tile + u8_bias_offset(is_v, row, dim / QGROUP, hd)));

@@ -503,7 +503,6 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   if (kernel < 0) return fail(SGK_ERR_BACKEND, "tensor-core attention kernel does not take this shape");
   int64_t max_rows = 0;
   const int64_t sink_rows = kvs[0]->sink_rows;
-  if (kernel != 4 && sink_rows > 0 && (sliding_window > 0 || window_start > 0)) kernel = 1;
   for (Kv* kv : kvs) {
     int64_t len_after = kv->len() + (fused ? 1 : 0);
     if (fused && kv->len() >= kv->seq->capacity)
@@ -537,7 +536,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   a.out = d_out;
   a.window_start = window_start;
   a.sliding_window = sliding_window;
-  a.sink_rows = sink_rows;
+  a.sink_rows = sliding_window > 0 || window_start > 0 ? sink_rows : 0;   // without a window every row is seen
   float scalar = attn_scalar > 0.0f ? attn_scalar : static_cast<float>(pool->head_dim);
   a.scale_log2e = 1.4426950408889634f / std::sqrt(scalar);
   const bool chained = st->chain_member(stream) && kernel >= 2;

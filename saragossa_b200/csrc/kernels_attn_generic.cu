@@ -13,6 +13,8 @@ constexpr int GEN_THREADS = 128;
 constexpr int GEN_WARPS = GEN_THREADS / 32;
 constexpr int GEN_MAXJ = 16;  // head_dim <= 32 * 16
 
+// U4, SINKS: instances for u4 pages and for sinks beside a window, so that neither costs the others anything.
+template <bool U4, bool SINKS>
 __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs a) {
   extern __shared__ float smem[];
   const int hd = a.pool.head_dim;
@@ -30,7 +32,7 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
   int64_t ws = a.sliding_window > 0 ? (len > a.sliding_window ? len - a.sliding_window : 0) : a.window_start;
   if (ws > len) ws = len;
   // visible rows: `sinks` at the head, then [ws, len); i counts them, row i + (i < sinks ? 0 : gap)
-  const int64_t sinks = a.sink_rows < ws ? a.sink_rows : ws;
+  const int64_t sinks = !SINKS ? 0 : a.sink_rows < ws ? a.sink_rows : ws;
   const int64_t gap = ws - sinks;
   const int64_t n = len - gap;
   const int64_t i0 = (n * split) / a.splits;
@@ -47,7 +49,7 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
   for (int j = 0; j < GEN_MAXJ; ++j) acc[j] = 0.0f;
 
   for (int64_t i = i0 + warp; i < i1; i += GEN_WARPS) {
-    const int64_t r = i < sinks ? i : i + gap;
+    const int64_t r = SINKS && i < sinks ? i : i + gap;
     int32_t page = table[r / PAGE_TOKENS];
     if (page < 0 || page >= a.num_pages) {
       if (lane == 0) atomicExch(a.status, DEV_ERR_BAD_PAGE);
@@ -60,7 +62,7 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
 #pragma unroll
     for (int j = 0; j < GEN_MAXJ; ++j) {
       int d = lane + 32 * j;
-      if (d < hd) dot += q_s[d] * load_tile_elem(ktile, a.pool.dtype, hd, 0, rin, d);
+      if (d < hd) dot += q_s[d] * (U4 ? load_u4_elem(ktile, hd, 0, rin, d) : load_tile_elem(ktile, a.pool.dtype, hd, 0, rin, d));
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
@@ -71,7 +73,7 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
 #pragma unroll
     for (int j = 0; j < GEN_MAXJ; ++j) {
       int d = lane + 32 * j;
-      if (d < hd) acc[j] = acc[j] * alpha + p * load_tile_elem(vtile, a.pool.dtype, hd, 1, rin, d);
+      if (d < hd) acc[j] = acc[j] * alpha + p * (U4 ? load_u4_elem(vtile, hd, 1, rin, d) : load_tile_elem(vtile, a.pool.dtype, hd, 1, rin, d));
     }
     m = m_new;
   }
@@ -138,7 +140,11 @@ __global__ void __launch_bounds__(GEN_THREADS) attention_generic_kernel(AttnArgs
 cudaError_t launch_attention_generic(const AttnArgs& a, int n_seq, cudaStream_t stream) {
   dim3 grid(a.q_heads, a.splits, n_seq);
   size_t smem = (size_t(a.pool.head_dim) * (1 + GEN_WARPS) + 2 * GEN_WARPS) * sizeof(float);
-  attention_generic_kernel<<<grid, GEN_THREADS, smem, stream>>>(a);
+  const bool u4 = a.pool.dtype == KV_U4G32, sinks = a.sink_rows > 0;
+  if (u4 && sinks) attention_generic_kernel<true, true><<<grid, GEN_THREADS, smem, stream>>>(a);
+  else if (u4) attention_generic_kernel<true, false><<<grid, GEN_THREADS, smem, stream>>>(a);
+  else if (sinks) attention_generic_kernel<false, true><<<grid, GEN_THREADS, smem, stream>>>(a);
+  else attention_generic_kernel<false, false><<<grid, GEN_THREADS, smem, stream>>>(a);
   return cudaGetLastError();
 }
 

@@ -59,7 +59,9 @@ struct MmaSmem {
   static size_t total(int stages) { return ring_bytes(stages) + FIXED + 1024; }
 };
 
-template <int HD, bool CLUSTER, bool PEERS>
+// SINKS: the instance for a window beside which the first rows stay visible. A separate one: the walk over
+// two ranges of pages and the masking of rows between them cost the others nothing.
+template <int HD, bool CLUSTER, bool PEERS, bool SINKS = false>
 __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs a) {
   using S = MmaSmem<HD>;
   constexpr int KSTEPS = HD / 16;
@@ -104,7 +106,13 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
   if (ws >= len) ws = len > 0 ? len - 1 : 0;
   const int64_t p_first = ws / PAGE_TOKENS;
   const int64_t p_last = (len - 1) / PAGE_TOKENS;
-  const int64_t n_pages = p_last - p_first + 1;
+  // With sinks the pages are counted from 0: first those that hold the sinks, then the window's.
+  const int64_t sinks = SINKS ? (a.sink_rows < ws ? a.sink_rows : ws) : 0;   // rows [0, sinks) and [ws, len) are seen
+  const int64_t sink_pages = (sinks + PAGE_TOKENS - 1) / PAGE_TOKENS < p_first ? (sinks + PAGE_TOKENS - 1) / PAGE_TOKENS : p_first;
+  const int64_t base_page = SINKS ? 0 : p_first;
+  std::conditional_t<SINKS, PageMap, PageIdentity> map;
+  if constexpr (SINKS) map = PageMap{sink_pages, p_first - sink_pages};
+  const int64_t n_pages = p_last - p_first + 1 + (SINKS ? sink_pages : 0);
   // Sequences of one launch may differ a lot in length: each is cut into its own number of
   // splits of about pages_per_split pages, and the blocks beyond that number have nothing to do.
   int splits = a.splits;
@@ -113,14 +121,15 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
     splits = static_cast<int>(want < 1 ? 1 : (want > a.splits ? a.splits : want));
   }
   if (split >= splits) return;
-  const int64_t pb = p_first + (n_pages * split) / splits;        // this block's pages [pb, pe)
-  const int64_t pe = p_first + (n_pages * (split + 1)) / splits;
+  const int64_t pb = base_page + (n_pages * split) / splits;        // this block's pages [pb, pe)
+  const int64_t pe = base_page + (n_pages * (split + 1)) / splits;
   const int my_pages = static_cast<int>(pe - pb);
   const int32_t* table = a.pool.tables + int64_t(slot) * a.pool.table_stride;
   const int64_t head_off = int64_t(a.layer) * a.pool.layer_bytes + int64_t(kvh) * 2 * a.pool.tile_bytes;
   // Page that receives the appended row, and whether this block owns it.
   const int64_t append_page_index = len_old / PAGE_TOKENS;
-  const bool owns_append = do_append && append_page_index >= pb && append_page_index < pe;
+  const bool owns_append = SINKS ? do_append && pe == n_pages && my_pages > 0   // (the last page)
+                                 : do_append && append_page_index >= pb && append_page_index < pe;
 
   int32_t first_entry = -1;
   if (warp == MMA_CONSUMERS) {
@@ -135,7 +144,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (lane < my_pages) first_entry = table[pb + lane];
+    if (lane < my_pages) first_entry = table[map.page(pb + lane)];
   } else {
     // Q of the group: scale, split into bf16 hi/lo; rows of absent heads are zero.
     // All loads are issued before the first conversion.
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
 
   if (warp == MMA_CONSUMERS) {
     // ---------------- producer warp ----------------
-    produce_pages<S::STAGE>(a, table, pb, my_pages, first_entry, ring, bars, nst, head_off, abort_flag, lane);
+    produce_pages<S::STAGE>(a, table, pb, my_pages, first_entry, ring, bars, nst, head_off, abort_flag, lane, map);
     if (a.pdl_wait) pdl_wait();   // the tail writes to memory the earlier launch may still be using
     SGK_TP(12);
   } else {
@@ -241,7 +250,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
       if (i == 0) SGK_TP(2);
       uint8_t* ktile = ring + size_t(stage) * S::STAGE;
       uint8_t* vtile = ktile + S::TILE;
-      const int64_t page_index = pb + i;
+      const int64_t page_index = map.page(pb + i);
       const int64_t row_base = page_index * PAGE_TOKENS;
 
       if (ok && owns_append && page_index == append_page_index) {
@@ -311,7 +320,21 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
         for (int e = 0; e < 4; ++e)
           s[e] = ((acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e])) + ((acc[4][e] + acc[5][e]) + (acc[6][e] + acc[7][e]));
         // rows g (s0,s1) and g+8 (s2,s3); heads 2t (s0,s2) and 2t+1 (s1,s3)
-        if (row_base < ws || row_base + PAGE_TOKENS > len) {
+        uint32_t keep_a = 0xffffffffu, keep_b = 0xffffffffu;   // V rows 2t, 2t+1 and 2t+8, 2t+9
+        bool cut = false;
+        if (SINKS) {
+          cut = row_base + PAGE_TOKENS > len || (row_base < ws && row_base + PAGE_TOKENS > sinks);
+          if (cut) {
+            // a row that is not seen weighs nothing, whatever its bytes say: V rows of it become zeros
+            const auto seen = [&](int r) { return row_base + r < len && (row_base + r < sinks || row_base + r >= ws); };
+            if (!seen(g)) s[0] = s[1] = -1.0e30f;
+            if (!seen(g + 8)) s[2] = s[3] = -1.0e30f;
+            keep_a = (seen(2 * t) ? 0x0000ffffu : 0u) | (seen(2 * t + 1) ? 0xffff0000u : 0u);
+            keep_b = (seen(2 * t + 8) ? 0x0000ffffu : 0u) | (seen(2 * t + 9) ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int u = 0; u < CH; ++u) va[u][0] &= keep_a, va[u][1] &= keep_a, va[u][2] &= keep_b, va[u][3] &= keep_b;
+          }
+        } else if (row_base < ws || row_base + PAGE_TOKENS > len) {
           int64_t ra = row_base + g, rb = row_base + g + 8;
           if (ra < ws || ra >= len) s[0] = s[1] = -1.0e30f;
           if (rb < ws || rb >= len) s[2] = s[3] = -1.0e30f;
@@ -360,6 +383,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
               int chunk = 2 * (c * CH + u) + v_csel;
               int phys = (chunk & ~7) | ((chunk ^ v_row) & 7);
               ldmatrix_x4_trans(vbase + phys * 16, va[u][0], va[u][1], va[u][2], va[u][3]);
+            }
+            if (SINKS && cut) {
+#pragma unroll
+              for (int u = 0; u < CH; ++u) va[u][0] &= keep_a, va[u][1] &= keep_a, va[u][2] &= keep_b, va[u][3] &= keep_b;
             }
             if (c == NCH - 1) {
               __syncwarp();
@@ -478,17 +505,28 @@ int attention_mma_max_clusters(int head_dim, int n_stages, int splits) {
   return n;
 }
 
+using Kernel = void (*)(AttnArgs);
+static Kernel kernel_for(int head_dim, bool cluster, bool peers, bool sinks) {
+  // [head_dim][sinks][plain, cluster, peers]
+  static const Kernel kernels[2][2][3] = {
+      {{attention_mma_kernel<128, false, false, false>, attention_mma_kernel<128, true, false, false>, attention_mma_kernel<128, false, true, false>},
+       {attention_mma_kernel<128, false, false, true>, attention_mma_kernel<128, true, false, true>, attention_mma_kernel<128, false, true, true>}},
+      {{attention_mma_kernel<256, false, false, false>, attention_mma_kernel<256, true, false, false>, attention_mma_kernel<256, false, true, false>},
+       {attention_mma_kernel<256, false, false, true>, attention_mma_kernel<256, true, false, true>, attention_mma_kernel<256, false, true, true>}}};
+  return kernels[head_dim == 256][sinks][peers ? 2 : cluster ? 1 : 0];
+}
+
 cudaError_t attention_mma_configure() {
-  const void* kernels[6] = {reinterpret_cast<const void*>(attention_mma_kernel<128, false, false>), reinterpret_cast<const void*>(attention_mma_kernel<256, false, false>),
-                            reinterpret_cast<const void*>(attention_mma_kernel<128, true, false>), reinterpret_cast<const void*>(attention_mma_kernel<256, true, false>),
-                            reinterpret_cast<const void*>(attention_mma_kernel<128, false, true>), reinterpret_cast<const void*>(attention_mma_kernel<256, false, true>)};
-  for (int i = 0; i < 6; ++i) {
-    cudaError_t e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    if (e != cudaSuccess) return e;
-    // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
-    if (i == 2 || i == 3) e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
+  for (int head_dim : {128, 256})
+    for (int sinks = 0; sinks < 2; ++sinks)
+      for (int kind = 0; kind < 3; ++kind) {
+        const void* kernel = reinterpret_cast<const void*>(kernel_for(head_dim, kind == 1, kind == 2, sinks != 0));
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e != cudaSuccess) return e;
+        // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
+        if (kind == 1) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+      }
   return cudaSuccess;
 }
 
@@ -529,17 +567,10 @@ static cudaError_t launch_one(void (*kernel)(AttnArgs), dim3 grid, size_t smem, 
 }
 
 cudaError_t launch_attention_mma(const AttnArgs& a, int n_seq, cudaStream_t stream) {
-  dim3 grid(a.splits, a.pool.kv_heads, n_seq);
-  if (a.pool.head_dim == 128) {
-    if (a.n_peers > 0) return launch_one(attention_mma_kernel<128, false, true>, grid, MmaSmem<128>::total(a.n_stages), a, stream);
-    return a.cluster_merge ? launch_one(attention_mma_kernel<128, true, false>, grid, MmaSmem<128>::total(a.n_stages), a, stream)
-                           : launch_one(attention_mma_kernel<128, false, false>, grid, MmaSmem<128>::total(a.n_stages), a, stream);
-  } else {
-    if (a.n_peers > 0) return launch_one(attention_mma_kernel<256, false, true>, grid, MmaSmem<256>::total(a.n_stages), a, stream);
-    return a.cluster_merge ? launch_one(attention_mma_kernel<256, true, false>, grid, MmaSmem<256>::total(a.n_stages), a, stream)
-                           : launch_one(attention_mma_kernel<256, false, false>, grid, MmaSmem<256>::total(a.n_stages), a, stream);
-  }
-  return cudaGetLastError();
+  const dim3 grid(a.splits, a.pool.kv_heads, n_seq);
+  const int hd = a.pool.head_dim;
+  const size_t smem = hd == 128 ? MmaSmem<128>::total(a.n_stages) : MmaSmem<256>::total(a.n_stages);
+  return launch_one(kernel_for(hd, a.cluster_merge != 0, a.n_peers > 0, a.sink_rows > 0), grid, smem, a, stream);
 }
 
 }  // namespace sgk

@@ -137,7 +137,9 @@ __device__ __forceinline__ void load_row_scales(const uint8_t* p, float (&sc)[G]
   }
 }
 
-template <int HD, bool CLUSTER, bool PEERS>
+// SINKS: the instance for a window beside which the first rows stay visible. A separate one: the walk over
+// two ranges of pages and the masking of rows between them cost the others nothing.
+template <int HD, bool CLUSTER, bool PEERS, bool SINKS = false>
 __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a) {
   using S = U8Smem<HD>;
   constexpr int G = S::G;
@@ -185,7 +187,13 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
   if (ws >= len) ws = len > 0 ? len - 1 : 0;
   const int64_t p_first = ws / PAGE_TOKENS;
   const int64_t p_last = (len - 1) / PAGE_TOKENS;
-  const int64_t n_pages = p_last - p_first + 1;
+  // With sinks the pages are counted from 0: first those that hold the sinks, then the window's.
+  const int64_t sinks = SINKS ? (a.sink_rows < ws ? a.sink_rows : ws) : 0;   // rows [0, sinks) and [ws, len) are seen
+  const int64_t sink_pages = (sinks + PAGE_TOKENS - 1) / PAGE_TOKENS < p_first ? (sinks + PAGE_TOKENS - 1) / PAGE_TOKENS : p_first;
+  const int64_t base_page = SINKS ? 0 : p_first;
+  std::conditional_t<SINKS, PageMap, PageIdentity> map;
+  if constexpr (SINKS) map = PageMap{sink_pages, p_first - sink_pages};
+  const int64_t n_pages = p_last - p_first + 1 + (SINKS ? sink_pages : 0);
   // Sequences of one launch may differ a lot in length: each is cut into its own number of
   // splits of about pages_per_split pages, and the blocks beyond that number have nothing to do.
   int splits = a.splits;
@@ -194,13 +202,14 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
     splits = static_cast<int>(want < 1 ? 1 : (want > a.splits ? a.splits : want));
   }
   if (split >= splits) return;
-  const int64_t pb = p_first + (n_pages * split) / splits;
-  const int64_t pe = p_first + (n_pages * (split + 1)) / splits;
+  const int64_t pb = base_page + (n_pages * split) / splits;
+  const int64_t pe = base_page + (n_pages * (split + 1)) / splits;
   const int my_pages = static_cast<int>(pe - pb);
   const int32_t* table = a.pool.tables + int64_t(slot) * a.pool.table_stride;
   const int64_t head_off = int64_t(a.layer) * a.pool.layer_bytes + int64_t(kvh) * 2 * a.pool.tile_bytes;
   const int64_t append_page_index = len_old / PAGE_TOKENS;
-  const bool owns_append = do_append && append_page_index >= pb && append_page_index < pe;
+  const bool owns_append = SINKS ? do_append && pe == n_pages && my_pages > 0   // (the last page)
+                                 : do_append && append_page_index >= pb && append_page_index < pe;
   const float* kn = new_s;
   const float* vn = new_s + HD;
 
@@ -219,7 +228,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (lane < my_pages) first_entry = table[pb + lane];
+    if (lane < my_pages) first_entry = table[map.page(pb + lane)];
   } else {
     // Q of the group: scaled, fp16 hi/lo, rows of absent heads zero. One fp16 alone (11 bits)
     // would put an error of |logit| * 2^-12 on every logit, too much for rows with a large range.
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
 
   if (warp == MMA_CONSUMERS) {
     // ---------------- producer warp ----------------
-    produce_pages<S::STAGE>(a, table, pb, my_pages, first_entry, ring, bars, nst, head_off, abort_flag, lane);
+    produce_pages<S::STAGE>(a, table, pb, my_pages, first_entry, ring, bars, nst, head_off, abort_flag, lane, map);
     if (a.pdl_wait) pdl_wait();   // the tail writes to memory the earlier launch may still be using
     SGK_TP(12);
   } else {
@@ -415,7 +424,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
       if (i == 0) SGK_TP(2);
       uint8_t* ktile = ring + size_t(stage) * S::STAGE;
       uint8_t* vtile = ktile + S::TILE;
-      const int64_t page_index = pb + i;
+      const int64_t page_index = map.page(pb + i);
       const int64_t row_base = page_index * PAGE_TOKENS;
 
       if (ok && owns_append && page_index == append_page_index) {
@@ -513,7 +522,19 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[r] = fmaf(s[r], CODE_UNIT_INV, sb[r]);  // the codes were in units of 2^-24
         U8_PHASE(tp_s);
-        if (row_base < ws || row_base + PAGE_TOKENS > len) {
+        uint32_t keep_a = 0xffffffffu, keep_b = 0xffffffffu;   // V rows 2t, 2t+1 and 2t+8, 2t+9
+        bool seen_g = true, seen_g8 = true;
+        if (SINKS) {
+          if (row_base + PAGE_TOKENS > len || (row_base < ws && row_base + PAGE_TOKENS > sinks)) {
+            // a row that is not seen weighs nothing, whatever its bytes say: its V scales and biases count as zeros
+            const auto seen = [&](int r) { return row_base + r < len && (row_base + r < sinks || row_base + r >= ws); };
+            seen_g = seen(g), seen_g8 = seen(g + 8);
+            if (!seen_g) s[0] = s[1] = -1.0e30f;
+            if (!seen_g8) s[2] = s[3] = -1.0e30f;
+            keep_a = (seen(2 * t) ? 0x0000ffffu : 0u) | (seen(2 * t + 1) ? 0xffff0000u : 0u);
+            keep_b = (seen(2 * t + 8) ? 0x0000ffffu : 0u) | (seen(2 * t + 9) ? 0xffff0000u : 0u);
+          }
+        } else if (row_base < ws || row_base + PAGE_TOKENS > len) {
           int64_t ra = row_base + g, rb = row_base + g + 8;
           if (ra < ws || ra >= len) s[0] = s[1] = -1.0e30f;
           if (rb < ws || rb >= len) s[2] = s[3] = -1.0e30f;
@@ -566,8 +587,9 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
           const uint32_t ph0 = pack_bf16(p[0], p[1]), ph1 = pack_bf16(p[2], p[3]);
           const uint32_t pl0 = pack_bf16(p[0] - bf16_lo_f32(ph0), p[1] - bf16_hi_f32(ph0));
           const uint32_t pl1 = pack_bf16(p[2] - bf16_lo_f32(ph1), p[3] - bf16_hi_f32(ph1));
-          const uint32_t a0 = vb_on ? *reinterpret_cast<const uint32_t*>(ktile + vb_off) : 0u;
-          const uint32_t a2 = vb_on ? *reinterpret_cast<const uint32_t*>(ktile + vb_off + 16) : 0u;
+          uint32_t a0 = vb_on ? *reinterpret_cast<const uint32_t*>(ktile + vb_off) : 0u;
+          uint32_t a2 = vb_on ? *reinterpret_cast<const uint32_t*>(ktile + vb_off + 16) : 0u;
+          if (SINKS) a0 &= keep_a, a2 &= keep_b;
           mma_bf16(cacc, a0, 0u, a2, 0u, movmatrix_trans(ph0), movmatrix_trans(ph1));
           mma_bf16(cacc, a0, 0u, a2, 0u, movmatrix_trans(pl0), movmatrix_trans(pl1));
         }
@@ -581,7 +603,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
           const uint32_t pw0 = pack_f16(p[0], p[1]), pw1 = pack_f16(p[2], p[3]);
 #pragma unroll
           for (int grp = 0; grp < G; ++grp) {
-            const float x0 = sv0[grp] * pscale, x1 = sv1[grp] * pscale;
+            float x0 = sv0[grp] * pscale, x1 = sv1[grp] * pscale;
+            if (SINKS) x0 = seen_g ? x0 : 0.0f, x1 = seen_g8 ? x1 : 0.0f;
             pb0[grp] = movmatrix_trans(hmul2_u32(pw0, pack_f16(x0, x0)));   // rows 0-7
             pb1[grp] = movmatrix_trans(hmul2_u32(pw1, pack_f16(x1, x1)));   // rows 8-15
           }
@@ -696,17 +719,28 @@ int attention_u8_max_clusters(int head_dim, int n_stages, int splits) {
   return n;
 }
 
+using Kernel = void (*)(AttnArgs);
+static Kernel kernel_for(int head_dim, bool cluster, bool peers, bool sinks) {
+  // [head_dim][sinks][plain, cluster, peers]
+  static const Kernel kernels[2][2][3] = {
+      {{attention_u8_kernel<128, false, false, false>, attention_u8_kernel<128, true, false, false>, attention_u8_kernel<128, false, true, false>},
+       {attention_u8_kernel<128, false, false, true>, attention_u8_kernel<128, true, false, true>, attention_u8_kernel<128, false, true, true>}},
+      {{attention_u8_kernel<256, false, false, false>, attention_u8_kernel<256, true, false, false>, attention_u8_kernel<256, false, true, false>},
+       {attention_u8_kernel<256, false, false, true>, attention_u8_kernel<256, true, false, true>, attention_u8_kernel<256, false, true, true>}}};
+  return kernels[head_dim == 256][sinks][peers ? 2 : cluster ? 1 : 0];
+}
+
 cudaError_t attention_u8_configure() {
-  const void* kernels[6] = {reinterpret_cast<const void*>(attention_u8_kernel<128, false, false>), reinterpret_cast<const void*>(attention_u8_kernel<256, false, false>),
-                            reinterpret_cast<const void*>(attention_u8_kernel<128, true, false>), reinterpret_cast<const void*>(attention_u8_kernel<256, true, false>),
-                            reinterpret_cast<const void*>(attention_u8_kernel<128, false, true>), reinterpret_cast<const void*>(attention_u8_kernel<256, false, true>)};
-  for (int i = 0; i < 6; ++i) {
-    cudaError_t e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    if (e != cudaSuccess) return e;
-    // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
-    if (i == 2 || i == 3) e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
+  for (int head_dim : {128, 256})
+    for (int sinks = 0; sinks < 2; ++sinks)
+      for (int kind = 0; kind < 3; ++kind) {
+        const void* kernel = reinterpret_cast<const void*>(kernel_for(head_dim, kind == 1, kind == 2, sinks != 0));
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        if (e != cudaSuccess) return e;
+        // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
+        if (kind == 1) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+      }
   return cudaSuccess;
 }
 
@@ -747,17 +781,10 @@ static cudaError_t launch_one(void (*kernel)(AttnArgs), dim3 grid, size_t smem, 
 }
 
 cudaError_t launch_attention_u8(const AttnArgs& a, int n_seq, cudaStream_t stream) {
-  dim3 grid(a.splits, a.pool.kv_heads, n_seq);
-  if (a.pool.head_dim == 128) {
-    if (a.n_peers > 0) return launch_one(attention_u8_kernel<128, false, true>, grid, U8Smem<128>::total(a.n_stages), a, stream);
-    return a.cluster_merge ? launch_one(attention_u8_kernel<128, true, false>, grid, U8Smem<128>::total(a.n_stages), a, stream)
-                           : launch_one(attention_u8_kernel<128, false, false>, grid, U8Smem<128>::total(a.n_stages), a, stream);
-  } else {
-    if (a.n_peers > 0) return launch_one(attention_u8_kernel<256, false, true>, grid, U8Smem<256>::total(a.n_stages), a, stream);
-    return a.cluster_merge ? launch_one(attention_u8_kernel<256, true, false>, grid, U8Smem<256>::total(a.n_stages), a, stream)
-                           : launch_one(attention_u8_kernel<256, false, false>, grid, U8Smem<256>::total(a.n_stages), a, stream);
-  }
-  return cudaGetLastError();
+  const dim3 grid(a.splits, a.pool.kv_heads, n_seq);
+  const int hd = a.pool.head_dim;
+  const size_t smem = hd == 128 ? U8Smem<128>::total(a.n_stages) : U8Smem<256>::total(a.n_stages);
+  return launch_one(kernel_for(hd, a.cluster_merge != 0, a.n_peers > 0, a.sink_rows > 0), grid, smem, a, stream);
 }
 
 }  // namespace sgk

@@ -132,8 +132,8 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   // the same kernel selection as the allocating entry point: tensor-core kernels over bf16, u8 and
   // u4 group-32 pages, the generic kernel for everything else
   const bool u4 = attention_u4_supported(pool->dtype, hd, qh / kvh);
-  const bool u8 = sinks.rows == 0 && attention_u8_supported(pool->dtype, hd, qh / kvh);
-  const bool mma = u4 || u8 || (sinks.rows == 0 && attention_mma_supported(pool->dtype, hd, qh / kvh));
+  const bool u8 = attention_u8_supported(pool->dtype, hd, qh / kvh);
+  const bool mma = u4 || u8 || attention_mma_supported(pool->dtype, hd, qh / kvh);
   // split count: fill the SMs (two blocks each for the tensor-core kernel, eight for the
   // generic one), keep a few pages per split, and stay inside the static workspace
   const int64_t pages = (len - window_start + PAGE_TOKENS - 1) / PAGE_TOKENS + sinks.pages;
@@ -168,7 +168,7 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   a.out = d_out;
   a.window_start = window_start;
   a.sliding_window = 0;
-  a.sink_rows = kv->sink_rows;
+  a.sink_rows = window_start > 0 ? kv->sink_rows : 0;   // without a window every row is seen
   const float scalar = attn_scalar > 0.0f ? attn_scalar : static_cast<float>(hd);
   a.scale_log2e = 1.4426950408889634f / std::sqrt(scalar);
   a.splits = static_cast<int>(splits);
