@@ -263,7 +263,7 @@ int32_t sgk_kv_gather_rows_u4(sgk_kv* kv, int64_t row0, int64_t n, uint8_t* k_co
                               uint16_t* k_bias, uint8_t* v_codes, uint16_t* v_scale, uint16_t* v_bias);
 /* Same rows decoded to f32 (bf16 upcast, u8 and u4 q*scale+bias, src/quantization.rs:173-179). */
 int32_t sgk_kv_gather_rows_f32(sgk_kv* kv, int64_t row0, int64_t n, float* k_out, float* v_out);
-/* The decoded rows into device memory, [n][kv_dim] each, 16-byte aligned: enqueue only. */
+/* The decoded rows into device memory, [n][kv_dim] f32 each: enqueue only. */
 int32_t sgk_kv_enqueue_gather_rows_f32(sgk_kv* kv, void* stream, int64_t row0, int64_t n, float* d_k, float* d_v);
 int32_t sgk_kv_block_table(const sgk_kv* kv, int32_t* pages_out, int64_t cap, int64_t* n_out);
 /* Forces one attention kernel: 0 = automatic, 1 = generic CUDA-core kernel,

@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(128, DIRECT ? 16 : 8) append_tiles_kernel(Appe
     // walk one row each for the sequential sums hit one bank sixteen times per step, which made
     // a launch of 2056 tiles shared-memory bound (47.9 us against 15.3 us without rope).
     const int rin0 = static_cast<int>(row_lo % PAGE_TOKENS);
-    const bool stage_v = a.pool.dtype == KV_U8G32;
+    const bool stage_v = a.pool.dtype >= KV_U8G32;   // V is quantised too
     // head_dim is 64, 128 or 256 here: the chunk arithmetic is shifts and masks, not divisions
     const int chunk_shift = hd == 64 ? 3 : hd == 128 ? 4 : 5;
     const int chunks = 1 << chunk_shift, total = rows << chunk_shift;
@@ -442,6 +442,27 @@ __global__ void __launch_bounds__(128, DIRECT ? 16 : 8) append_tiles_kernel(Appe
                                      uint32_t(f32_to_bf16_bits(x1.z)) | (uint32_t(f32_to_bf16_bits(x1.w)) << 16));
           *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(ktile) + bf16_elem_index(rin0 + r, chunk * 8, hd)) = w;
         }
+      } else if (a.pool.dtype == KV_U4G32) {
+        const int tile_b = static_cast<int>(a.pool.tile_bytes);
+        const bool full = rows == PAGE_TOKENS;
+        uint8_t* kt = full ? stage : ktile;
+        const int row_lanes = hd / 8;
+        for (int base = 0; base < 2 * rows * row_lanes; base += blockDim.x) {
+          const int i = base + tid, task = i / row_lanes, sub = i % row_lanes, grp = sub >> 2, q = sub & 3;
+          const int r = min(task >> 1, rows - 1), is_v = task & 1;   // (lanes past the end repeat the last row, and store nothing)
+          const float* xs = (is_v ? vs + r * hd : ks + r * kstride) + grp * QGROUP + 4 * q;
+          const float4 x = *reinterpret_cast<const float4*>(xs), y = *reinterpret_cast<const float4*>(xs + 16);
+          float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          const uint32_t odd = (rin0 + r) & 1;
+          const U4Lane out = hd == 256   ? u4_quantize_lanes<32>(v, odd, lane)
+                             : hd == 128 ? u4_quantize_lanes<16>(v, odd, lane)
+                                         : u4_quantize_lanes<8>(v, odd, lane);
+          if ((task >> 1) < rows) u4_store_lane(kt, kt + tile_b, hd, is_v, rin0 + r, grp, q, out);
+        }
+        if (full) {
+          __syncthreads();
+          for (int i = tid; i < 2 * tile_b / 16; i += blockDim.x) reinterpret_cast<uint4*>(ktile)[i] = reinterpret_cast<const uint4*>(stage)[i];
+        }
       } else {
         uint32_t biggest = 0;
         // a full tile is put together in shared memory and leaves with 16-byte stores; a
@@ -491,6 +512,81 @@ __global__ void __launch_bounds__(128, DIRECT ? 16 : 8) append_tiles_kernel(Appe
   }
 }
 
+// ---- bulk append into u4 pages without rope: one block per (kv head, page, sequence) ----------------------
+// A thread takes eight values of a group (two 16-byte loads), so a group's range costs two shuffle steps and its bias,
+// step and exponent are worked out by four lanes instead of thirty-two (a warp per row, a lane per dim: 478 us for 32768
+// rows of 4 heads of 128; this: FILL). All rows of the page tile are in registers before the first is quantised. A full tile
+// is put together in shared memory and leaves with 16-byte stores, a partial one is written in place.
+template <int HD>
+__global__ void __launch_bounds__(128) append_u4_tiles_kernel(AppendArgs a) {
+  constexpr int ROW_LANES = HD / 8;
+  constexpr int TASKS = 2 * PAGE_TOKENS * ROW_LANES / 128;   // (row, K or V) pieces per thread
+  constexpr int TILE = 10 * HD + 16;
+  __shared__ __align__(16) uint8_t stage[2 * TILE];
+  const int head = blockIdx.x, tile_i = blockIdx.y, seq = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int kv_dim = a.pool.kv_heads * HD;
+  const int slot = a.slots ? a.slots[seq] : a.slot0;
+  int32_t* len_ptr = a.pool.lens + int64_t(slot) * a.pool.layers + a.layer;
+  const int64_t len0 = a.use_device_len ? static_cast<int64_t>(*len_ptr) : a.row0;
+  const int64_t page_index = len0 / PAGE_TOKENS + tile_i;
+  const int64_t row_lo = max(len0, page_index * PAGE_TOKENS);
+  const int64_t row_hi = min(len0 + a.n_rows, (page_index + 1) * PAGE_TOKENS);
+  const int rows = static_cast<int>(row_hi - row_lo);
+  if (rows > 0) {
+    int32_t page = -1;
+    if (page_index < a.pool.table_stride) page = a.pool.tables[int64_t(slot) * a.pool.table_stride + page_index];
+    const int rin0 = static_cast<int>(row_lo % PAGE_TOKENS);
+    const int64_t first = (int64_t(seq) * a.n_rows + (row_lo - len0)) * kv_dim + head * HD;
+    const int sub = tid % ROW_LANES, grp = sub >> 2, q = sub & 3;   // the same in every task
+    float4 x[TASKS], y[TASKS];
+#pragma unroll
+    for (int i = 0; i < TASKS; ++i) {
+      const int task = i * (128 / ROW_LANES) + tid / ROW_LANES;   // row r: 2 r is K, 2 r + 1 is V
+      const int r = task >> 1;
+      x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows) {
+        const float4* src = reinterpret_cast<const float4*>((task & 1 ? a.v : a.k) + first + int64_t(r) * kv_dim + grp * QGROUP + 4 * q);
+        x[i] = __ldg(src);
+        y[i] = __ldg(src + 4);
+      }
+    }
+    if (page >= 0 && page < a.num_pages) {
+      uint8_t* global = a.pool.base + tile_offset(a.pool, page, a.layer, head, 0);
+      const bool full = rows == PAGE_TOKENS;
+      uint8_t* ktile = full ? stage : global;
+#pragma unroll
+      for (int i = 0; i < TASKS; ++i) {
+        const int task = i * (128 / ROW_LANES) + tid / ROW_LANES;
+        const int r = task >> 1, rin = rin0 + r;
+        float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
+        const U4Lane out = u4_quantize_lanes<ROW_LANES>(v, rin & 1, lane);
+        if (r < rows) u4_store_lane(ktile, ktile + TILE, HD, task & 1, rin, grp, q, out);
+      }
+      if (full) {
+        __syncthreads();
+        for (int i = tid; i < 2 * TILE / 16; i += 128) reinterpret_cast<uint4*>(global)[i] = reinterpret_cast<const uint4*>(stage)[i];
+      }
+    } else if (tid == 0) {
+      atomicExch(a.status, DEV_ERR_BAD_PAGE);
+    }
+  }
+  if (a.bump_len) {
+    // The block that arrives last moves the cursor: every block has read it by then.
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      const int total = gridDim.x * gridDim.y;
+      const int old = atomicAdd(a.done_counters + seq, 1);
+      if (old == total - 1) {
+        *len_ptr = static_cast<int32_t>(len0 + a.n_rows);
+        a.done_counters[seq] = 0;
+        __threadfence();
+      }
+    }
+  }
+}
+
 __global__ void set_len_kernel(int32_t* ptr, int n, int32_t value) {
   int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i < n) ptr[i] = value;
@@ -521,14 +617,20 @@ cudaError_t launch_rope_table(float2* table, int64_t row0, int n_rows, const Rop
 
 cudaError_t launch_append_rows(const AppendArgs& a, int n_seq, cudaStream_t stream) {
   const int hd = a.pool.head_dim;
-  if (a.n_rows >= 4 && a.out_k == nullptr && (hd == 64 || hd == 128 || hd == 256) && a.pool.dtype != KV_U4G32) {
+  if (a.n_rows >= 4 && a.out_k == nullptr && (hd == 64 || hd == 128 || hd == 256)) {
     // bulk: one block per page tile; the first row may sit anywhere in its page, so one tile more
     dim3 grid(a.pool.kv_heads, (a.n_rows + PAGE_TOKENS - 1) / PAGE_TOKENS + 1, n_seq);
     // the kernel's carve-up: K rows, 1/rms per row, rope denominators (<= 128 pairs); V rows and a
     // tile pair being put together only where V is quantised
+    if (a.pool.dtype == KV_U4G32 && !a.has_rope) {
+      if (hd == 64) append_u4_tiles_kernel<64><<<grid, 128, 0, stream>>>(a);
+      else if (hd == 128) append_u4_tiles_kernel<128><<<grid, 128, 0, stream>>>(a);
+      else append_u4_tiles_kernel<256><<<grid, 128, 0, stream>>>(a);
+      return cudaGetLastError();
+    }
     size_t smem = (size_t(PAGE_TOKENS) * (hd + 4) + PAGE_TOKENS + 128) * sizeof(float);
-    if (a.pool.dtype == KV_U8G32) smem += size_t(PAGE_TOKENS) * hd * sizeof(float) + 2 * size_t(a.pool.tile_bytes);
-    if (!a.has_rope && a.pool.dtype != KV_U8G32) append_tiles_kernel<true><<<grid, 128, 0, stream>>>(a);
+    if (a.pool.dtype >= KV_U8G32) smem += size_t(PAGE_TOKENS) * hd * sizeof(float) + 2 * size_t(a.pool.tile_bytes);
+    if (!a.has_rope && a.pool.dtype < KV_U8G32) append_tiles_kernel<true><<<grid, 128, 0, stream>>>(a);
     else append_tiles_kernel<false><<<grid, 128, smem, stream>>>(a);
     return cudaGetLastError();
   }

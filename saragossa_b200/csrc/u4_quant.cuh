@@ -81,6 +81,28 @@ __device__ __forceinline__ uint32_t u4_code_of(float y, float bias, float step, 
   }
   return static_cast<uint32_t>(code);
 }
+// The same for eight values of a group at once: codes of v[0..3] and v[4..7] as the bytes v[j] + 16 v[j + 4]. The
+// borders are looked at only when one of the eight lies on one.
+__device__ __forceinline__ uint32_t u4_codes8(const float (&v)[8], float bias, float step, float inv) {
+  const float half = 0.5f * step;
+  uint32_t low = 0, high = 0;
+  bool border = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float t0 = __fsub_rn(v[j], bias), t1 = __fsub_rn(v[j + 4], bias);
+    const float g0 = fminf(fmaxf(t0 * inv, 0.0f), 15.0f) + 12582912.0f, g1 = fminf(fmaxf(t1 * inv, 0.0f), 15.0f) + 12582912.0f;
+    border = border || fabsf(fmaf(-(g0 - 12582912.0f), step, t0)) >= half || fabsf(fmaf(-(g1 - 12582912.0f), step, t1)) >= half;
+    low |= (__float_as_uint(g0) & 15u) << (8 * j);
+    high |= (__float_as_uint(g1) & 15u) << (8 * j);
+  }
+  uint32_t word = low | (high << 4);
+  if (border) {
+    word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) word |= u4_code_of(v[j], bias, step, inv) << (8 * (j & 3) + (j >> 2) * 4);
+  }
+  return word;
+}
 // fp16 bits of step / 2^row_exponent, with the row's sign: exact (8 significant bits, >= 2^-16).
 __device__ __forceinline__ uint16_t u4_v_factor_bits(uint16_t step_bits, int row_exponent, uint32_t odd) {
   if (step_bits == 0x7fc0) return 0x7e00;
@@ -153,6 +175,62 @@ __device__ __forceinline__ void u4_store_row(uint8_t* ktile, uint8_t* vtile, int
   if (is_v && lane == 0)
     *reinterpret_cast<uint16_t*>((row < 8 ? ktile : vtile) + u4_pow_offset(row, hd)) =
         static_cast<uint16_t>(__float_as_uint(pow2f(row_exponent)) >> 16);
+}
+
+// A head row spread over ROW_LANES = hd / 8 neighbouring lanes: four lanes per group, lane q = lane % 4 with dims 4q .. 4q+3
+// (v[0..3]) and 16 + 4q .. (v[4..7]) of the group, whose codes are four whole bytes. All lanes of the warp call.
+struct U4Lane {
+  uint32_t word;            // the four bytes
+  uint16_t step, bias;      // step positive, bias signed (bf16 bits)
+  int exponent;             // of the row
+};
+template <int ROW_LANES>
+__device__ __forceinline__ U4Lane u4_quantize_lanes(float (&v)[8], uint32_t odd, int lane) {
+  const float sign = odd ? -1.0f : 1.0f;
+  float lo = INFINITY, hi = -INFINITY, poison = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] *= sign;
+    lo = fminf(lo, v[j]);
+    hi = fmaxf(hi, v[j]);
+    poison = fmaf(v[j], 0.0f, poison);   // NaN once a value is not finite
+  }
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+  }
+  const uint32_t bad = __ballot_sync(0xffffffffu, poison != 0.0f) >> (lane & ~3) & 15u;
+  U4Range r = u4_range(lo, hi);
+  if (bad) r.finite = false, r.exponent = U4_EXP_MIN;
+  U4Lane out;
+  out.exponent = r.exponent;
+#pragma unroll
+  for (int off = 4; off < ROW_LANES; off <<= 1) out.exponent = max(out.exponent, __shfl_xor_sync(0xffffffffu, out.exponent, off));
+  out.step = u4_step_bits(r, out.exponent);
+  const float s = bf16_bits_to_f32(out.step);
+  out.word = r.finite ? u4_codes8(v, r.bias, s, __frcp_rn(s)) : 0u;
+  out.bias = static_cast<uint16_t>(r.finite ? (__float_as_uint(sign * r.bias) >> 16) : 0u);
+  return out;
+}
+// Stores what u4_quantize_lanes made of row `row`: group grp, lane q of four.
+__device__ __forceinline__ void u4_store_lane(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, int grp, int q, const U4Lane& x) {
+  uint8_t* tile = is_v ? vtile : ktile;
+  const uint32_t odd = row & 1;
+  const int dim = grp * QGROUP + 4 * q;
+  if (is_v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tile[u4_v_byte(row, dim + j, hd)] = static_cast<uint8_t>(x.word >> (8 * j));
+  } else {
+    *reinterpret_cast<uint32_t*>(tile + u4_k_byte(row, dim, hd)) = x.word;
+  }
+  if (q == 0) {
+    *reinterpret_cast<uint16_t*>(tile + u4_step_offset(is_v, row, grp, hd)) =
+        is_v ? u4_v_factor_bits(x.step, x.exponent, odd) : static_cast<uint16_t>(x.step ^ (odd << 15));
+    *reinterpret_cast<uint16_t*>(tile + u4_bias_offset(row, grp, hd)) = x.bias;
+    if (is_v && grp == 0)
+      *reinterpret_cast<uint16_t*>((row < 8 ? ktile : vtile) + u4_pow_offset(row, hd)) = static_cast<uint16_t>(__float_as_uint(pow2f(x.exponent)) >> 16);
+  }
 }
 
 }  // namespace sgk
