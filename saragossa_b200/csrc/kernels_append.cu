@@ -452,12 +452,15 @@ __global__ void __launch_bounds__(128, DIRECT ? 16 : 8) append_tiles_kernel(Appe
           const int r = min(task >> 1, rows - 1), is_v = task & 1;   // (lanes past the end repeat the last row, and store nothing)
           const float* xs = (is_v ? vs + r * hd : ks + r * kstride) + grp * QGROUP + 4 * q;
           const float4 x = *reinterpret_cast<const float4*>(xs), y = *reinterpret_cast<const float4*>(xs + 16);
-          float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
           const uint32_t odd = (rin0 + r) & 1;
           const U4Lane out = hd == 256   ? u4_quantize_lanes<32>(v, odd, lane)
                              : hd == 128 ? u4_quantize_lanes<16>(v, odd, lane)
                                          : u4_quantize_lanes<8>(v, odd, lane);
-          if ((task >> 1) < rows) u4_store_lane(kt, kt + tile_b, hd, is_v, rin0 + r, grp, q, out);
+          if ((task >> 1) < rows) {
+            u4_store_codes(is_v ? kt + tile_b : kt, hd, is_v, rin0 + r, grp, q, out.word);
+            u4_store_meta(kt, kt + tile_b, hd, is_v, rin0 + r, grp, q, out);
+          }
         }
         if (full) {
           __syncthreads();
@@ -539,33 +542,58 @@ __global__ void __launch_bounds__(128) append_u4_tiles_kernel(AppendArgs a) {
     const int rin0 = static_cast<int>(row_lo % PAGE_TOKENS);
     const int64_t first = (int64_t(seq) * a.n_rows + (row_lo - len0)) * kv_dim + head * HD;
     const int sub = tid % ROW_LANES, grp = sub >> 2, q = sub & 3;   // the same in every task
+    // piece 2 i is K, 2 i + 1 is V of row i * PASS + tid / ROW_LANES
+    constexpr int PASS = 128 / ROW_LANES;
     float4 x[TASKS], y[TASKS];
 #pragma unroll
     for (int i = 0; i < TASKS; ++i) {
-      const int task = i * (128 / ROW_LANES) + tid / ROW_LANES;   // row r: 2 r is K, 2 r + 1 is V
-      const int r = task >> 1;
+      const int r = (i >> 1) * PASS + tid / ROW_LANES;
       x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < rows) {
-        const float4* src = reinterpret_cast<const float4*>((task & 1 ? a.v : a.k) + first + int64_t(r) * kv_dim + grp * QGROUP + 4 * q);
+        const float4* src = reinterpret_cast<const float4*>((i & 1 ? a.v : a.k) + first + int64_t(r) * kv_dim + grp * QGROUP + 4 * q);
         x[i] = __ldg(src);
         y[i] = __ldg(src + 4);
       }
     }
     if (page >= 0 && page < a.num_pages) {
       uint8_t* global = a.pool.base + tile_offset(a.pool, page, a.layer, head, 0);
-      const bool full = rows == PAGE_TOKENS;
-      uint8_t* ktile = full ? stage : global;
+      if (rows == PAGE_TOKENS) {
+        uint32_t v_words[TASKS / 2];
 #pragma unroll
-      for (int i = 0; i < TASKS; ++i) {
-        const int task = i * (128 / ROW_LANES) + tid / ROW_LANES;
-        const int r = task >> 1, rin = rin0 + r;
-        float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
-        const U4Lane out = u4_quantize_lanes<ROW_LANES>(v, rin & 1, lane);
-        if (r < rows) u4_store_lane(ktile, ktile + TILE, HD, task & 1, rin, grp, q, out);
-      }
-      if (full) {
+        for (int i = 0; i < TASKS; ++i) {
+          const int r = (i >> 1) * PASS + tid / ROW_LANES;
+          const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
+          const U4Lane out = u4_quantize_lanes<ROW_LANES>(v, r & 1, lane);
+          u4_store_meta(stage, stage + TILE, HD, i & 1, r, grp, q, out);
+          if (i & 1) v_words[i >> 1] = out.word;
+          else u4_store_codes(stage, HD, 0, r, grp, q, out.word);
+        }
+        // V bytes of rows r and r + 8 are neighbours: where one thread has both, they leave together
+#pragma unroll
+        for (int i = 0; i < TASKS / 2; ++i) {
+          const int r = i * PASS + tid / ROW_LANES;
+          if (PASS > 8) {
+            u4_store_codes(stage + TILE, HD, 1, r, grp, q, v_words[i]);
+          } else if (i < TASKS / 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint16_t*>(stage + TILE + u4_v_byte(r, grp * QGROUP + 4 * q + j, HD)) =
+                  static_cast<uint16_t>(__byte_perm(v_words[i], v_words[i + TASKS / 4], 0x40 + 0x11 * j));
+          }
+        }
         __syncthreads();
         for (int i = tid; i < 2 * TILE / 16; i += 128) reinterpret_cast<uint4*>(global)[i] = reinterpret_cast<const uint4*>(stage)[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < TASKS; ++i) {
+          const int r = (i >> 1) * PASS + tid / ROW_LANES, rin = rin0 + r;
+          const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
+          const U4Lane out = u4_quantize_lanes<ROW_LANES>(v, rin & 1, lane);
+          if (r < rows) {
+            u4_store_codes(global + (i & 1) * TILE, HD, i & 1, rin, grp, q, out.word);
+            u4_store_meta(global, global + TILE, HD, i & 1, rin, grp, q, out);
+          }
+        }
       }
     } else if (tid == 0) {
       atomicExch(a.status, DEV_ERR_BAD_PAGE);

@@ -99,32 +99,41 @@ __global__ void __launch_bounds__(128) gather_u4_f32_kernel(GatherArgs a) {
   const uint4* src = reinterpret_cast<const uint4*>(a.pool.base + tile_offset(a.pool, page, a.layer, head, 0));
   for (int i = tid; i < 2 * TILE / 16; i += 128) reinterpret_cast<uint4*>(tile)[i] = __ldg(src + i);
   __syncthreads();
-  const int sub = tid % ROW_LANES, grp = sub >> 2, q = sub & 3;
-#pragma unroll 4
-  for (int task = tid / ROW_LANES; task < 2 * PAGE_TOKENS; task += 128 / ROW_LANES) {
-    const int rin = task >> 1, is_v = task & 1;
-    const int64_t row = page_index * PAGE_TOKENS + rin;
-    if (row < a.row0 || row >= a.row0 + a.n) continue;
+  const int sub = tid % ROW_LANES, grp = sub >> 2, q = sub & 3, dim = grp * QGROUP + 4 * q;
+  const int64_t row_first = page_index * PAGE_TOKENS - a.row0;   // rows of the output, negative before its first
+  const auto put = [&](int is_v, int rin, uint32_t w) {
+    const int64_t row = row_first + rin;
+    if (row < 0 || row >= a.n) return;
     const uint8_t* t = tile + is_v * TILE;
-    const int dim = grp * QGROUP + 4 * q;
-    uint32_t w = 0;
-    if (is_v) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w |= uint32_t(t[u4_v_byte(rin, dim + j, HD)]) << (8 * j);
-    } else {
-      w = *reinterpret_cast<const uint32_t*>(t + u4_k_byte(rin, dim, HD));
-    }
     const float step = u4_step(t, HD, is_v, rin, grp);
     const float bias = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(t + u4_bias_offset(rin, grp, HD)));
+    const uint32_t low = w & 0x0f0f0f0fu, high = (w >> 4) & 0x0f0f0f0fu;
     float v[8];   // code * step is exact: one rounding
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = fmaf(static_cast<float>((w >> (8 * j)) & 15u), step, bias);
-      v[j + 4] = fmaf(static_cast<float>((w >> (8 * j + 4)) & 15u), step, bias);
+      // the byte in the mantissa of 2^23 is 2^23 + code
+      v[j] = fmaf(__uint_as_float(__byte_perm(low, 0x4b000000u, 0x7650 + j)) - 8388608.0f, step, bias);
+      v[j + 4] = fmaf(__uint_as_float(__byte_perm(high, 0x4b000000u, 0x7650 + j)) - 8388608.0f, step, bias);
     }
-    float4* out = reinterpret_cast<float4*>(reinterpret_cast<float*>(is_v ? a.v_out : a.k_out) + (row - a.row0) * kv_dim + head * HD + dim);
+    float4* out = reinterpret_cast<float4*>(reinterpret_cast<float*>(is_v ? a.v_out : a.k_out) + row * kv_dim + head * HD + dim);
     out[0] = make_float4(v[0], v[1], v[2], v[3]);
     out[4] = make_float4(v[4], v[5], v[6], v[7]);
+  };
+  // V bytes of rows r and r + 8 are neighbours: a thread takes both rows
+  constexpr int PASS = 128 / ROW_LANES < 8 ? 128 / ROW_LANES : 8;   // rows per pass, of eight
+  if (tid / ROW_LANES < PASS) {
+#pragma unroll
+    for (int i = 0; i < 8 / PASS; ++i) {
+      const int r = i * PASS + tid / ROW_LANES;
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = *reinterpret_cast<const uint16_t*>(tile + TILE + u4_v_byte(r, dim + j, HD));
+      put(0, r, *reinterpret_cast<const uint32_t*>(tile + u4_k_byte(r, dim, HD)));
+      put(0, r + 8, *reinterpret_cast<const uint32_t*>(tile + u4_k_byte(r + 8, dim, HD)));
+      const uint32_t a0 = __byte_perm(h[0], h[1], 0x5140), a1 = __byte_perm(h[2], h[3], 0x5140);   // rows r, r, r + 8, r + 8
+      put(1, r, __byte_perm(a0, a1, 0x5410));
+      put(1, r + 8, __byte_perm(a0, a1, 0x7632));
+    }
   }
 }
 

@@ -43,26 +43,25 @@ __device__ __forceinline__ U4Range u4_range(float lo, float hi) {
   r.bias = bf16_bits_to_f32(f32_to_bf16_bits(lo));
   r.width = two_diff(hi, r.bias, r.err);
   r.finite = fabsf(r.bias) < INFINITY && r.width < INFINITY;
-  r.exponent = U4_EXP_MIN;
-  if (r.finite && r.width > 0x1p-37f) {   // 15 * 2^-40 < 2^-36: below that the floor of the exponent stands
-    int e = static_cast<int>(__float_as_uint(r.width * (1.0f / 15.0f)) >> 23) - 127;
-    const float at = 15.0f * pow2f(e);
-    if (r.width < at || (r.width == at && r.err < 0.0f)) e -= 1;
-    else if (r.width > 2.0f * at || (r.width == 2.0f * at && r.err >= 0.0f)) e += 1;
-    r.exponent = max(e, U4_EXP_MIN);
-  }
+  // floor(log2(width / 15)), from a quotient that may be a unit off; anything below the least exponent counts as that
+  const int guess = static_cast<int>(__float_as_uint(fmaxf(r.width, 0x1p-40f) * (1.0f / 15.0f)) >> 23);
+  const float at = 15.0f * __uint_as_float(static_cast<uint32_t>(guess) << 23);
+  int e = guess - 127;
+  if (r.width < at || (r.width == at && r.err < 0.0f)) e -= 1;
+  if (r.width > 2.0f * at || (r.width == 2.0f * at && r.err >= 0.0f)) e += 1;
+  r.exponent = r.finite ? max(e, U4_EXP_MIN) : U4_EXP_MIN;
   return r;
 }
 // bf16 bits of the (positive) step of a group; row_exponent = the largest exponent of the head row.
 __device__ __forceinline__ uint16_t u4_step_bits(const U4Range& r, int row_exponent) {
-  if (!r.finite) return 0x7fc0;
   const float floor_step = pow2f(max(row_exponent - 16, U4_EXP_MIN));
   const float at = 15.0f * floor_step;
-  if (r.width < at || (r.width == at && r.err <= 0.0f)) return static_cast<uint16_t>(__float_as_uint(floor_step) >> 16);
   const uint32_t low = __float_as_uint(r.width * (1.0f / 15.0f)) & 0xffff0000u;
   const float mid = 15.0f * __uint_as_float(low | 0x8000u);   // the border to the next bf16 value, times 15
   const bool up = r.width > mid || (r.width == mid && (r.err > 0.0f || (r.err == 0.0f && (low & 0x10000u))));
-  return static_cast<uint16_t>((low >> 16) + (up ? 1u : 0u));
+  uint32_t bits = (low >> 16) + (up ? 1u : 0u);
+  if (r.width < at || (r.width == at && r.err <= 0.0f)) bits = __float_as_uint(floor_step) >> 16;
+  return static_cast<uint16_t>(r.finite ? bits : 0x7fc0u);
 }
 // Code of y; inv ~ 1 / step (an error of a few units in the last place is mended below).
 __device__ __forceinline__ uint32_t u4_code_of(float y, float bias, float step, float inv) {
@@ -81,25 +80,28 @@ __device__ __forceinline__ uint32_t u4_code_of(float y, float bias, float step, 
   }
   return static_cast<uint32_t>(code);
 }
-// The same for eight values of a group at once: codes of v[0..3] and v[4..7] as the bytes v[j] + 16 v[j + 4]. The
+// The same for eight values sign * v of a group at once: codes of v[0..3] and v[4..7] as the bytes c[j] + 16 c[j + 4]. The
 // borders are looked at only when one of the eight lies on one.
-__device__ __forceinline__ uint32_t u4_codes8(const float (&v)[8], float bias, float step, float inv) {
-  const float half = 0.5f * step;
-  uint32_t low = 0, high = 0;
-  bool border = false;
+__device__ __forceinline__ uint32_t u4_codes8(const float (&v)[8], float sign, float bias, float step, float inv) {
+  // the rounded number sits in the low bits of guess: the eight are added up as integers, each at its place, and the
+  // upper bits (0x4b400000 each) are taken off as one constant
+  uint32_t word = 0;
+  float far = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float t0 = __fsub_rn(v[j], bias), t1 = __fsub_rn(v[j + 4], bias);
-    const float g0 = fminf(fmaxf(t0 * inv, 0.0f), 15.0f) + 12582912.0f, g1 = fminf(fmaxf(t1 * inv, 0.0f), 15.0f) + 12582912.0f;
-    border = border || fabsf(fmaf(-(g0 - 12582912.0f), step, t0)) >= half || fabsf(fmaf(-(g1 - 12582912.0f), step, t1)) >= half;
-    low |= (__float_as_uint(g0) & 15u) << (8 * j);
-    high |= (__float_as_uint(g1) & 15u) << (8 * j);
+  for (int j = 0; j < 8; ++j) {
+    const float t = fmaf(v[j], sign, -bias);
+    const float guess = fminf(fmaxf(t * inv, 0.0f), 15.0f) + 12582912.0f;
+    far = fmaxf(far, fabsf(fmaf(-(guess - 12582912.0f), step, t)));
+    word += __float_as_uint(guess) << (8 * (j & 3) + (j >> 2) * 4);
   }
-  uint32_t word = low | (high << 4);
-  if (border) {
+  uint32_t upper = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) upper += 0x4b400000u << (8 * (j & 3) + (j >> 2) * 4);
+  word -= upper;
+  if (far >= 0.5f * step) {
     word = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) word |= u4_code_of(v[j], bias, step, inv) << (8 * (j & 3) + (j >> 2) * 4);
+    for (int j = 0; j < 8; ++j) word |= u4_code_of(sign * v[j], bias, step, inv) << (8 * (j & 3) + (j >> 2) * 4);
   }
   return word;
 }
@@ -185,12 +187,11 @@ struct U4Lane {
   int exponent;             // of the row
 };
 template <int ROW_LANES>
-__device__ __forceinline__ U4Lane u4_quantize_lanes(float (&v)[8], uint32_t odd, int lane) {
+__device__ __forceinline__ U4Lane u4_quantize_lanes(const float (&v)[8], uint32_t odd, int lane) {
   const float sign = odd ? -1.0f : 1.0f;
-  float lo = INFINITY, hi = -INFINITY, poison = 0.0f;
+  float lo = v[0], hi = v[0], poison = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    v[j] *= sign;
     lo = fminf(lo, v[j]);
     hi = fmaxf(hi, v[j]);
     poison = fmaf(v[j], 0.0f, poison);   // NaN once a value is not finite
@@ -201,7 +202,7 @@ __device__ __forceinline__ U4Lane u4_quantize_lanes(float (&v)[8], uint32_t odd,
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
   }
   const uint32_t bad = __ballot_sync(0xffffffffu, poison != 0.0f) >> (lane & ~3) & 15u;
-  U4Range r = u4_range(lo, hi);
+  U4Range r = u4_range(odd ? -hi : lo, odd ? -lo : hi);
   if (bad) r.finite = false, r.exponent = U4_EXP_MIN;
   U4Lane out;
   out.exponent = r.exponent;
@@ -209,28 +210,30 @@ __device__ __forceinline__ U4Lane u4_quantize_lanes(float (&v)[8], uint32_t odd,
   for (int off = 4; off < ROW_LANES; off <<= 1) out.exponent = max(out.exponent, __shfl_xor_sync(0xffffffffu, out.exponent, off));
   out.step = u4_step_bits(r, out.exponent);
   const float s = bf16_bits_to_f32(out.step);
-  out.word = r.finite ? u4_codes8(v, r.bias, s, __frcp_rn(s)) : 0u;
+  const uint32_t word = u4_codes8(v, sign, r.bias, s, __frcp_rn(s));
+  out.word = r.finite ? word : 0u;
   out.bias = static_cast<uint16_t>(r.finite ? (__float_as_uint(sign * r.bias) >> 16) : 0u);
   return out;
 }
-// Stores what u4_quantize_lanes made of row `row`: group grp, lane q of four.
-__device__ __forceinline__ void u4_store_lane(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, int grp, int q, const U4Lane& x) {
-  uint8_t* tile = is_v ? vtile : ktile;
-  const uint32_t odd = row & 1;
+// Stores what u4_quantize_lanes made of row `row`, group grp, lane q of four: the codes, then the rest.
+__device__ __forceinline__ void u4_store_codes(uint8_t* tile, int hd, int is_v, int row, int grp, int q, uint32_t word) {
   const int dim = grp * QGROUP + 4 * q;
   if (is_v) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) tile[u4_v_byte(row, dim + j, hd)] = static_cast<uint8_t>(x.word >> (8 * j));
+    for (int j = 0; j < 4; ++j) tile[u4_v_byte(row, dim + j, hd)] = static_cast<uint8_t>(word >> (8 * j));
   } else {
-    *reinterpret_cast<uint32_t*>(tile + u4_k_byte(row, dim, hd)) = x.word;
+    *reinterpret_cast<uint32_t*>(tile + u4_k_byte(row, dim, hd)) = word;
   }
-  if (q == 0) {
-    *reinterpret_cast<uint16_t*>(tile + u4_step_offset(is_v, row, grp, hd)) =
-        is_v ? u4_v_factor_bits(x.step, x.exponent, odd) : static_cast<uint16_t>(x.step ^ (odd << 15));
-    *reinterpret_cast<uint16_t*>(tile + u4_bias_offset(row, grp, hd)) = x.bias;
-    if (is_v && grp == 0)
-      *reinterpret_cast<uint16_t*>((row < 8 ? ktile : vtile) + u4_pow_offset(row, hd)) = static_cast<uint16_t>(__float_as_uint(pow2f(x.exponent)) >> 16);
-  }
+}
+__device__ __forceinline__ void u4_store_meta(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, int grp, int q, const U4Lane& x) {
+  if (q != 0) return;
+  uint8_t* tile = is_v ? vtile : ktile;
+  const uint32_t odd = row & 1;
+  *reinterpret_cast<uint16_t*>(tile + u4_step_offset(is_v, row, grp, hd)) =
+      is_v ? u4_v_factor_bits(x.step, x.exponent, odd) : static_cast<uint16_t>(x.step ^ (odd << 15));
+  *reinterpret_cast<uint16_t*>(tile + u4_bias_offset(row, grp, hd)) = x.bias;
+  if (is_v && grp == 0)
+    *reinterpret_cast<uint16_t*>((row < 8 ? ktile : vtile) + u4_pow_offset(row, hd)) = static_cast<uint16_t>(__float_as_uint(pow2f(x.exponent)) >> 16);
 }
 
 }  // namespace sgk
