@@ -137,7 +137,6 @@ bool attention_u4_supported(int dtype, int head_dim, int gqa);
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream);
 cudaError_t attention_u4_configure();
 int attention_u4_blocks_per_sm(int head_dim);
-int attention_u4_stages(int head_dim);
 int attention_u4_resident_blocks(int head_dim);
 int attention_u4_max_clusters(int head_dim, int splits);
 

@@ -128,25 +128,32 @@ struct U4Word {
   }
 };
 
-constexpr int U4_WARPS = MMA_CONSUMERS;
-constexpr int U4_THREADS = U4_WARPS * 32;
 // Launch shape by head size; registers and shared memory are split evenly among the resident blocks.
 template <int HD>
 struct U4Shape;
-template <>
-struct U4Shape<128> {
-  static constexpr int BLOCKS = 3;   // resident per SM
-  static constexpr int PAGES = 2;    // a warp works on at once
-  static constexpr int SLOTS = 4;    // stages of a warp, a multiple of PAGES
+#ifndef U4_S128
+#define U4_S128 4, 3, 2, 6, 4
+#endif
+#ifndef U4_S256
+#define U4_S256 4, 2, 1, 4, 4
+#endif
+template <int W, int B, int P, int N, int C>
+struct U4ShapeOf {
+  static constexpr int WARPS = W;    // of a block
+  static constexpr int BLOCKS = B;   // resident per SM
+  static constexpr int PAGES = P;    // a warp works on at once
+  static constexpr int SLOTS = N, CLUSTER_SLOTS = C;    // stages of a warp, a multiple of PAGES
 };
 template <>
-struct U4Shape<256> {
-  static constexpr int BLOCKS = 2, PAGES = 1, SLOTS = 4;
-};
+struct U4Shape<128> : U4ShapeOf<U4_S128> {};
+template <>
+struct U4Shape<256> : U4ShapeOf<U4_S256> {};
 constexpr float U4_LIMIT = 14.0f;   // p'' <= 2^14
 constexpr float U4_LEVEL = 6.0f;    // p'' of the largest z when the reference moves
 
-template <int HD>
+// CLUSTER: the instance whose splits merge through distributed shared memory needs room to receive; the other gives that
+// room to the ring.
+template <int HD, bool CLUSTER>
 struct U4Smem {
   static constexpr int G = HD / QGROUP;
   static constexpr int STEPS = PAGE_TOKENS * HD / 2;          // 2 bytes per (row, group)
@@ -154,19 +161,19 @@ struct U4Smem {
   static constexpr int POWERS = BIASES + PAGE_TOKENS * G * 2; // 8 x bf16
   static constexpr int TILE = POWERS + 16;
   static constexpr int STAGE = 2 * TILE;
-  static constexpr int SLOTS = U4Shape<HD>::SLOTS;
+  static constexpr int SLOTS = CLUSTER ? U4Shape<HD>::CLUSTER_SLOTS : U4Shape<HD>::SLOTS, WARPS = U4Shape<HD>::WARPS, THREADS = WARPS * 32;
   static constexpr int OPAD = HD + 4;
   static constexpr int Q_BYTES = G * 2 * 32 * 16;             // B fragments: [group][high | low dims][lane]{hi, lo}
   static constexpr int QROWS_BYTES = 8 * HD * 4;              // q in f32 while the fragments are made
   static constexpr int QSUM_BYTES = 8 * 8 * 4 + 8 * 4;        // [head][8 groups], absent groups zero; power of two per head
-  static constexpr int O_BYTES = U4_WARPS * 8 * OPAD * 4;
-  static constexpr int ML_BYTES = 512;
-  static constexpr int BAR_BYTES = U4_WARPS * SLOTS * 8;
+  static constexpr int O_BYTES = WARPS * 8 * OPAD * 4;
+  static constexpr int ML_BYTES = (WARPS * 24 + 16) * 4;   // what finish_block asks for
+  static constexpr int BAR_BYTES = (WARPS * SLOTS * 8 + 15) / 16 * 16;
   // the row of a fused append: f32 K and V, afterwards its bytes (codes K | V, then 4 G + 1 half words)
   static constexpr int NEW_BYTES = 2 * HD * 4;
-  static constexpr int RECV_BYTES = ClusterRecv<HD>::BYTES;
+  static constexpr int RECV_BYTES = CLUSTER ? ClusterRecv<HD>::BYTES : 0;
   static constexpr int FIXED = Q_BYTES + QROWS_BYTES + QSUM_BYTES + ML_BYTES + BAR_BYTES + 64 + NEW_BYTES + RECV_BYTES;
-  static constexpr int RING_BYTES = U4_WARPS * SLOTS * STAGE > O_BYTES ? U4_WARPS * SLOTS * STAGE : O_BYTES;
+  static constexpr int RING_BYTES = WARPS * SLOTS * STAGE > O_BYTES ? WARPS * SLOTS * STAGE : O_BYTES;
   static constexpr int TOTAL = RING_BYTES + FIXED;
   static_assert(STAGE % 16 == 0 && TILE % 16 == 0 && QSUM_BYTES % 16 == 0, "16-byte pieces");
   static_assert(RING_BYTES % 16 == 0 && BAR_BYTES % 16 == 0, "16-byte pieces");
@@ -175,7 +182,7 @@ struct U4Smem {
 // Writes the row that a fused append has quantised (`park`) into a tile pair in global or shared memory; one warp.
 template <int HD>
 __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park, int rin, int lane) {
-  using S = U4Smem<HD>;
+  using S = U4Smem<HD, false>;
   uint8_t* vtile = ktile + S::TILE;
   const uint16_t* meta = reinterpret_cast<const uint16_t*>(park + HD);   // K step, K bias, V factor, V bias [G] each, power
   const int p = lane & 15;
@@ -197,10 +204,10 @@ __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park
 // PP: pages a warp works on at once. Two (head_dim 128) give the chains of matrix instructions twice the
 // independent work and share the query's fragments and the bookkeeping; with head_dim 256 one page fills the registers.
 template <int HD, bool CLUSTER, bool PEERS>
-__global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_kernel(AttnArgs a) {
-  using S = U4Smem<HD>;
+__global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) attention_u4_kernel(AttnArgs a) {
+  using S = U4Smem<HD, CLUSTER>;
   constexpr int G = S::G;
-    constexpr int PP = U4Shape<HD>::PAGES;
+    constexpr int PP = U4Shape<HD>::PAGES, WARPS = S::WARPS, THREADS = S::THREADS;
   constexpr int SETS = G / 4;
   // (not rounded up by hand: an address that went through an integer is a generic one to the compiler, and its loads too)
   extern __shared__ __align__(128) uint8_t u4_smem[];
@@ -212,7 +219,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
   float* o_s = reinterpret_cast<float*>(ring);    // aliases the ring once it has drained
   float* ml_s = qpow_s + 8;                                               // [warps][8][2]
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(ml_s) + S::ML_BYTES);
-  int* flags = reinterpret_cast<int*>(bars + U4_WARPS * S::SLOTS);
+  int* flags = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + S::BAR_BYTES);
   float* new_s = reinterpret_cast<float*>(flags + 16);
   float* recv_s = new_s + 2 * HD;
   volatile int* abort_flag = flags;
@@ -255,8 +262,8 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
   // needed about 640 cycles per page, waiting for the consumers' releases one by one).
   // Lane l holds the block-table entries of the warp's pages 32 k + l: batch k and the one after it.
   constexpr int SLOTS = S::SLOTS;
-  const int count = (my_pages - warp + U4_WARPS - 1) / U4_WARPS;   // this warp's pages
-  const auto entry_of = [&](int n) { return n < count ? table[map.page(pb + warp + U4_WARPS * n)] : -1; };
+  const int count = (my_pages - warp + WARPS - 1) / WARPS;   // this warp's pages
+  const auto entry_of = [&](int n) { return n < count ? table[map.page(pb + warp + WARPS * n)] : -1; };
   int32_t entries = entry_of(lane), entries_next = entry_of(32 + lane);
   uint64_t* my_bars = bars + warp * SLOTS;
   uint8_t* my_ring = ring + warp * SLOTS * S::STAGE;
@@ -283,7 +290,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
   if (lane < SLOTS && lane < count) fetch(lane, entries);
   {
     // ---------------- the query ----------------
-    constexpr int NV = HD / 64;
+    constexpr int NV = (8 * HD / 4 + THREADS - 1) / THREADS;   // 16-byte pieces of q per thread
     const float* q = a.q + (int64_t(seq) * a.q_heads + int64_t(kvh) * gqa) * HD;
     // q and the row to append come from the launch before this one; the cursor, the block table and
     // the pages the producer starts to copy do not
@@ -291,7 +298,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
     float4 v[NV];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int f = (tid + k * U4_THREADS) * 4;
+      const int f = (tid + k * THREADS) * 4;
       v[k] = (f / HD < gqa) ? __ldg(reinterpret_cast<const float4*>(q + f)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     if (owns_append && tid * 4 < 2 * HD) {
@@ -302,14 +309,14 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
     if (owns_append && tid == 0) flags[2] = table[len_old / PAGE_TOKENS];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int f = (tid + k * U4_THREADS) * 4;
+      const int f = (tid + k * THREADS) * 4;
       v[k].x *= a.scale_log2e, v[k].y *= a.scale_log2e, v[k].z *= a.scale_log2e, v[k].w *= a.scale_log2e;
-      *reinterpret_cast<float4*>(q_rows + f) = v[k];
+      if (f < 8 * HD) *reinterpret_cast<float4*>(q_rows + f) = v[k];
     }
     __syncthreads();
-    // Two heads per warp: sums of the groups, and the power of two that brings the largest |q| to 2^15..2^16.
+    // Sums of the groups, and the power of two that brings the largest |q| to 2^15..2^16.
 #pragma unroll
-    for (int h = 2 * warp; h < 2 * warp + 2; ++h) {
+    for (int h = warp; h < 8; h += WARPS) {
       float big = 0.0f;
 #pragma unroll
       for (int grp = 0; grp < G; ++grp) {
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
       }
     }
     __syncthreads();
-    for (int i = tid; i < G * 32; i += U4_THREADS) {
+    for (int i = tid; i < G * 32; i += THREADS) {
       const int grp = i >> 5, h = (i & 31) >> 2, t = i & 3;
       const float inv = 1.0f / qpow_s[h];
       const float* row = q_rows + h * HD + grp * QGROUP + 4 * t;
@@ -369,7 +376,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
     // on their way; its bytes go to the page in global memory and stay parked in shared memory for the warp
     // that will meet the page in the ring.
     uint8_t* park = reinterpret_cast<uint8_t*>(new_s);
-    if (owns_append && warp == U4_WARPS - 1) {
+    if (owns_append && warp == WARPS - 1) {
       const int rin = len_old % PAGE_TOKENS;
       const uint32_t odd = rin & 1;
       const int32_t page = flags[2];
@@ -429,8 +436,8 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
       int best = INT32_MAX;
       const auto consider = [&](int v) {   // ordinal of a page
         const int k = v - pb - warp;
-        if (k >= 0 && k % U4_WARPS == 0 && k / U4_WARPS < count) {
-          const int at = k / U4_WARPS / PP * PP;
+        if (k >= 0 && k % WARPS == 0 && k / WARPS < count) {
+          const int at = k / WARPS / PP * PP;
           if (at >= from) best = min(best, at);
         }
       };
@@ -465,8 +472,8 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
       const bool special = n == special_at;
       if (special) {
         special_at = next_special(n + PP);
-        const int k = n_pages - 1 - pb - warp - n * U4_WARPS;   // the last page is the iteration's page k / 4
-        if (owns_append && k >= 0 && k < PP * U4_WARPS && k % U4_WARPS == 0) {
+        const int k = n_pages - 1 - pb - warp - n * WARPS;   // the last page is the iteration's page k / 4
+        if (owns_append && k >= 0 && k < PP * WARPS && k % WARPS == 0) {
           // the new row joins the staged copy
           uint32_t spins = 0;
           while (*reinterpret_cast<volatile int*>(flags + 5) == 0) {
@@ -477,7 +484,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
             }
           }
           __syncwarp();
-          u4_place_row<HD>(my_ring + (at + k / U4_WARPS) * S::STAGE, park, len_old % PAGE_TOKENS, lane);
+          u4_place_row<HD>(my_ring + (at + k / WARPS) * S::STAGE, park, len_old % PAGE_TOKENS, lane);
           __syncwarp();
         }
       }
@@ -560,7 +567,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
           // A row that is not seen weighs nothing, whatever its bytes say.
 #pragma unroll
           for (int u = 0; u < PP; ++u) {
-            const int v = pb + warp + U4_WARPS * (n + u);
+            const int v = pb + warp + WARPS * (n + u);
             const int base = u == 0 || n + u < count ? (v + (v >= sink_pages ? p_first - sink_pages : 0)) * PAGE_TOKENS : len;
             const auto seen = [&](int r) {
               const int row = base + r;
@@ -690,8 +697,11 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
           entries_next = entry_of(batch + 32 + lane);
         }
         // (32 is a multiple of PP: an iteration's entries lie in one batch)
-        const int32_t page = __shfl_sync(0xffffffffu, entries, next - batch + lane);
-        if (lane < PP && next + lane < count) fetch(at + lane, page);
+#pragma unroll
+        for (int u = 0; u < PP; ++u) {
+          const int32_t page = __shfl_sync(0xffffffffu, entries, next - batch + u);
+          if (next + u < count && lane == 0) fetch(at + u, page);
+        }
       }
       at += PP;
       if (at == SLOTS) at = 0, phase ^= 1;
@@ -726,7 +736,7 @@ __global__ void __launch_bounds__(U4_THREADS, U4Shape<HD>::BLOCKS) attention_u4_
     }
   }
   __syncthreads();
-  finish_block<HD, CLUSTER, PEERS, U4_THREADS, 1>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
+  finish_block<HD, CLUSTER, PEERS, THREADS, 1, WARPS>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
                                    splits, recv_s);
   if (PEERS) peers_finish(a, tid, flags);
 }
@@ -736,8 +746,6 @@ bool attention_u4_supported(int dtype, int head_dim, int gqa) {
 }
 
 int attention_u4_blocks_per_sm(int head_dim) { return head_dim == 128 ? U4Shape<128>::BLOCKS : U4Shape<256>::BLOCKS; }
-int attention_u4_stages(int head_dim) { return U4_WARPS * (head_dim == 128 ? U4Smem<128>::SLOTS : U4Smem<256>::SLOTS); }
-
 static const void* u4_kernel(int head_dim, bool cluster, bool peers) {
   if (head_dim == 128)
     return peers     ? reinterpret_cast<const void*>(attention_u4_kernel<128, false, true>)
@@ -747,12 +755,17 @@ static const void* u4_kernel(int head_dim, bool cluster, bool peers) {
          : cluster ? reinterpret_cast<const void*>(attention_u4_kernel<256, true, false>)
                    : reinterpret_cast<const void*>(attention_u4_kernel<256, false, false>);
 }
-static size_t u4_smem_bytes(int head_dim) { return head_dim == 128 ? U4Smem<128>::TOTAL : U4Smem<256>::TOTAL; }
+static size_t u4_smem_bytes(int head_dim, bool cluster) {
+  if (head_dim == 128) return cluster ? U4Smem<128, true>::TOTAL : U4Smem<128, false>::TOTAL;
+  return cluster ? U4Smem<256, true>::TOTAL : U4Smem<256, false>::TOTAL;
+}
+
+static int u4_threads(int head_dim) { return 32 * (head_dim == 128 ? U4Shape<128>::WARPS : U4Shape<256>::WARPS); }
 
 int attention_u4_resident_blocks(int head_dim) {
   int blocks = 0;
-  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, u4_kernel(head_dim, false, false), U4_THREADS,
-                                                                u4_smem_bytes(head_dim));
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, u4_kernel(head_dim, false, false), u4_threads(head_dim),
+                                                                u4_smem_bytes(head_dim, false));
   return e == cudaSuccess ? blocks : 0;
 }
 
@@ -760,8 +773,8 @@ int attention_u4_resident_blocks(int head_dim) {
 int attention_u4_max_clusters(int head_dim, int splits) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, 1, 1);
-  cfg.blockDim = dim3(U4_THREADS);
-  cfg.dynamicSmemBytes = u4_smem_bytes(head_dim);
+  cfg.blockDim = dim3(u4_threads(head_dim));
+  cfg.dynamicSmemBytes = u4_smem_bytes(head_dim, true);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = splits;
@@ -792,8 +805,8 @@ cudaError_t attention_u4_configure() {
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.splits, a.pool.kv_heads, n_seq);
-  cfg.blockDim = dim3(U4_THREADS);
-  cfg.dynamicSmemBytes = u4_smem_bytes(a.pool.head_dim);
+  cfg.blockDim = dim3(u4_threads(a.pool.head_dim));
+  cfg.dynamicSmemBytes = u4_smem_bytes(a.pool.head_dim, a.cluster_merge && a.n_peers == 0);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n_attr = 0;
@@ -818,7 +831,7 @@ cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t strea
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
   void* args[1] = {const_cast<AttnArgs*>(&a)};
-  return cudaLaunchKernelExC(&cfg, u4_kernel(a.pool.head_dim, a.cluster_merge != 0, a.n_peers > 0), args);
+  return cudaLaunchKernelExC(&cfg, u4_kernel(a.pool.head_dim, a.cluster_merge && a.n_peers == 0, a.n_peers > 0), args);
 }
 
 }  // namespace sgk

@@ -578,7 +578,8 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const Partials& s
 // CLUSTER: the kernel instance that is launched as clusters (its splits merge through distributed
 // shared memory). A separate instance, so that the other one is compiled without a trace of that path:
 // with both in one kernel the page loop of the long-stream case lost 1.3 % (register allocation).
-template <int HD, bool CLUSTER, bool PEERS = false, int NT = MMA_THREADS, int CELLS = (NT >= 256 ? 1 : 2)>
+// WARPS: warps whose states are in o_s and ml_s; the area behind ml_s holds WARPS * 24 + 16 floats in all.
+template <int HD, bool CLUSTER, bool PEERS = false, int NT = MMA_THREADS, int CELLS = (NT >= 256 ? 1 : 2), int WARPS = MMA_CONSUMERS>
 __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s, const float* ml_s, int opad,
                                              int* flags, int seq, int kvh, int split, int gqa, bool do_append,
                                              int32_t* len_ptr, int64_t len, int tid, int splits, float* recv) {
@@ -590,18 +591,18 @@ __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s
   // ---- merge the consumer warps; write the partial or the final output ----
   // ml_s holds [warps][8]{max, sum}; behind it: the per-(head, warp) weights and the block's
   // {max, sum} per head (the shared-memory layouts reserve 512 bytes for this area).
-  float* wgt_s = const_cast<float*>(ml_s) + MMA_CONSUMERS * 8 * 2;   // [8][warps]
-  float* hml_s = wgt_s + 8 * MMA_CONSUMERS;                           // [8]{max, sum}
+  float* wgt_s = const_cast<float*>(ml_s) + WARPS * 8 * 2;   // [8][warps]
+  float* hml_s = wgt_s + 8 * WARPS;                           // [8]{max, sum}
   const int64_t qh0 = int64_t(seq) * a.q_heads + int64_t(kvh) * gqa;
   if (tid < 8) {
     float mb = -1.0e30f;
 #pragma unroll
-    for (int w = 0; w < MMA_CONSUMERS; ++w) mb = fmaxf(mb, ml_s[(w * 8 + tid) * 2]);
+    for (int w = 0; w < WARPS; ++w) mb = fmaxf(mb, ml_s[(w * 8 + tid) * 2]);
     float lb = 0.0f;
 #pragma unroll
-    for (int w = 0; w < MMA_CONSUMERS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const float wg = exp2f(ml_s[(w * 8 + tid) * 2] - mb);
-      wgt_s[tid * MMA_CONSUMERS + w] = wg;
+      wgt_s[tid * WARPS + w] = wg;
       lb += ml_s[(w * 8 + tid) * 2 + 1] * wg;
     }
     hml_s[2 * tid] = mb;
@@ -612,9 +613,9 @@ __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s
     const int h = idx / (HD / 4), d = (idx % (HD / 4)) * 4;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < MMA_CONSUMERS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const float4 v = *reinterpret_cast<const float4*>(o_s + (w * 8 + h) * opad + d);
-      const float wg = wgt_s[h * MMA_CONSUMERS + w];
+      const float wg = wgt_s[h * WARPS + w];
       o.x += v.x * wg;
       o.y += v.y * wg;
       o.z += v.z * wg;

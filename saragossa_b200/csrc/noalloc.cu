@@ -188,7 +188,6 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   a.k_new = nullptr;
   a.v_new = nullptr;
   if (u4) {
-    a.n_stages = attention_u4_stages(hd);
     SGK_CUDA(launch_attention_u4(a, 1, cs));
   } else if (u8) {
     a.n_stages = attention_u8_max_stages(hd);
