@@ -263,27 +263,34 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
   // Lane l holds the block-table entries of the warp's pages 32 k + l: batch k and the one after it.
   constexpr int SLOTS = S::SLOTS;
   const int count = (my_pages - warp + WARPS - 1) / WARPS;   // this warp's pages
-  const auto entry_of = [&](int n) { return n < count ? table[map.page(pb + warp + WARPS * n)] : -1; };
-  int32_t entries = entry_of(lane), entries_next = entry_of(32 + lane);
-  uint64_t* my_bars = bars + warp * SLOTS;
-  uint8_t* my_ring = ring + warp * SLOTS * S::STAGE;
-  const uint64_t policy = l2_policy_evict_first();
-  const auto fetch = [&](int slot_at, int32_t page) {   // one lane
-    if (page < 0 || page >= a.num_pages) {
-      atomicExch(a.status, DEV_ERR_BAD_PAGE);
-      *abort_flag = 1;
-      return;
+  const auto entry_of = [&](int n) {
+    int32_t page = 0;
+    if (n < count) {
+      page = table[map.page(pb + warp + WARPS * n)];
+      if (page < 0 || page >= a.num_pages) {   // reported; the page read in its place is one of the pool's
+        atomicExch(a.status, DEV_ERR_BAD_PAGE);
+        page = 0;
+      }
     }
-    const uint32_t bar = smem_u32(my_bars + slot_at);
+    return page;
+  };
+  int32_t entries = entry_of(lane), entries_next = entry_of(32 + lane);
+  const uint8_t* my_ring = ring + warp * SLOTS * S::STAGE;
+  const uint32_t my_ring_at = smem_u32(my_ring), my_bars = smem_u32(bars + warp * SLOTS);
+  const uint64_t policy = l2_policy_evict_first();
+  const uint8_t* const source = a.pool.base + head_off;
+  const int64_t page_bytes = a.pool.page_bytes;
+  const auto fetch = [&](int slot_at, int32_t page) {   // one lane
+    const uint32_t bar = my_bars + 8 * slot_at;
     mbar_expect_tx(bar, S::STAGE);
-    bulk_copy_g2s(smem_u32(my_ring + slot_at * S::STAGE), a.pool.base + int64_t(page) * a.pool.page_bytes + head_off, S::STAGE, bar, policy);
+    bulk_copy_g2s(my_ring_at + slot_at * S::STAGE, source + page * page_bytes, S::STAGE, bar, policy);
   };
   if (tid == 0) {
-    flags[0] = 0;   // a wait ran out, or a bad table entry
+    flags[0] = 0;   // a wait ran out
     flags[1] = 0;
     flags[5] = 0;   // set once the quantised row of a fused append is parked in shared memory
   }
-  if (lane < SLOTS) mbar_init(smem_u32(my_bars + lane), 1);
+  if (lane < SLOTS) mbar_init(my_bars + 8 * lane, 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
             static_cast<uint8_t>(lane < 16 ? code[grp] | (other << 4) : other | (code[G + grp] << 4));
       }
       __syncwarp();
-      // a bad table entry is reported by the producer, which meets it too
+      // a bad table entry is reported where the page is fetched
       if (page >= 0 && page < a.num_pages) u4_place_row<HD>(a.pool.base + int64_t(page) * a.pool.page_bytes + head_off, park, rin, lane);
       __syncwarp();
       if (lane == 0) {
@@ -453,19 +460,22 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
     for (int n = 0; n < count; n += PP) {
       const uint8_t* tile[PP];
       bool ok = true;
+      // (a missing second page stands in for itself by the first one)
 #pragma unroll
-      for (int u = 0; u < PP; ++u) {
-        const int slot_at = at + (u > 0 && n + u >= count ? 0 : u);   // a missing page stands in for itself by the first one
-        tile[u] = my_ring + slot_at * S::STAGE;
-        const uint32_t bar = smem_u32(my_bars + slot_at);
-        if (!mbar_try_wait(bar, phase)) ok = mbar_wait(bar, phase, abort_flag, a.status) && ok;
+      for (int u = 0; u < PP; ++u) tile[u] = my_ring + (at + (u > 0 && n + u >= count ? 0 : u)) * S::STAGE;
+      {
+        const uint32_t bar = my_bars + 8 * at;
+        const bool pair = PP > 1 && n + 1 < count;
+        bool ready = mbar_try_wait(bar, phase);
+        if (PP > 1) ready = (mbar_try_wait(bar + (pair ? 8 : 0), phase)) && ready;
+        if (!ready) ok = mbar_wait(bar, phase, abort_flag, a.status) && mbar_wait(bar + (pair ? 8 : 0), phase, abort_flag, a.status);
       }
       if (!ok) {
         // gave up (reported): the copies still on their way are waited for, with the short bound, before the block leaves
         for (int k = n; k < count && k < n + SLOTS; ++k) {
           int slot_at = at + (k - n), ph = phase;
           if (slot_at >= SLOTS) slot_at -= SLOTS, ph ^= 1;
-          mbar_wait(smem_u32(my_bars + slot_at), ph, abort_flag, a.status);
+          mbar_wait(my_bars + 8 * slot_at, ph, abort_flag, a.status);
         }
         break;
       }
@@ -484,7 +494,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
             }
           }
           __syncwarp();
-          u4_place_row<HD>(my_ring + (at + k / WARPS) * S::STAGE, park, len_old % PAGE_TOKENS, lane);
+          u4_place_row<HD>(ring + (warp * SLOTS + at + k / WARPS) * S::STAGE, park, len_old % PAGE_TOKENS, lane);
           __syncwarp();
         }
       }
