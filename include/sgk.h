@@ -60,7 +60,7 @@ enum { SGK_KV_F32 = 0, SGK_KV_BF16 = 1, SGK_KV_U8G32 = 2, SGK_KV_U4G32 = 3 };
  * of odd rows negative (sums of weighted values then lose no digits to a common offset). A group that
  * holds an infinity or a NaN, or whose range overflows, reads back as NaN. head_dim: a multiple of 32. A row of a head
  * takes head_dim * 10 / 16 + 1 bytes for K and as many for V. The tensor-core attention kernel takes
- * head_dim 128 and 256 with up to 8 query heads per KV head; other shapes go to the generic kernel. */
+ * head_dim 64, 128 and 256 with up to 8 query heads per KV head; other shapes go to the generic kernel. */
 
 /* Tokens per page. The page is the unit of allocation, sharing and copy. */
 #define SGK_PAGE_TOKENS 16

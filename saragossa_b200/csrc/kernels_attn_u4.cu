@@ -1,4 +1,4 @@
-// Paged split-K flash-decoding over u4 group-32 pages (head_dim 128 / 256, GQA group <= 8), with the
+// Paged split-K flash-decoding over u4 group-32 pages (head_dim 64 / 128 / 256, GQA group <= 8), with the
 // per-token append (quantisation included) fused in and with attention sinks beside the window.
 //
 // Same pipeline as the other paged kernels (producer warp, one bulk async copy per page into a
@@ -131,12 +131,6 @@ struct U4Word {
 // Launch shape by head size; registers and shared memory are split evenly among the resident blocks.
 template <int HD>
 struct U4Shape;
-#ifndef U4_S128
-#define U4_S128 4, 3, 2, 6, 4
-#endif
-#ifndef U4_S256
-#define U4_S256 4, 2, 1, 4, 4
-#endif
 template <int W, int B, int P, int N, int C>
 struct U4ShapeOf {
   static constexpr int WARPS = W;    // of a block
@@ -145,9 +139,11 @@ struct U4ShapeOf {
   static constexpr int SLOTS = N, CLUSTER_SLOTS = C;    // stages of a warp, a multiple of PAGES
 };
 template <>
-struct U4Shape<128> : U4ShapeOf<U4_S128> {};
+struct U4Shape<64> : U4ShapeOf<4, 4, 2, 8, 4> {};
 template <>
-struct U4Shape<256> : U4ShapeOf<U4_S256> {};
+struct U4Shape<128> : U4ShapeOf<4, 3, 2, 6, 4> {};
+template <>
+struct U4Shape<256> : U4ShapeOf<4, 2, 1, 4, 4> {};
 constexpr float U4_LIMIT = 14.0f;   // p'' <= 2^14
 constexpr float U4_LEVEL = 6.0f;    // p'' of the largest z when the reference moves
 
@@ -179,6 +175,23 @@ struct U4Smem {
   static_assert(RING_BYTES % 16 == 0 && BAR_BYTES % 16 == 0, "16-byte pieces");
 };
 
+// N words from shared memory with loads as wide as N words.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+    }
+  }
+}
+
 // Writes the row that a fused append has quantised (`park`) into a tile pair in global or shared memory; one warp.
 template <int HD>
 __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park, int rin, int lane) {
@@ -208,7 +221,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
   using S = U4Smem<HD, CLUSTER>;
   constexpr int G = S::G;
     constexpr int PP = U4Shape<HD>::PAGES, WARPS = S::WARPS, THREADS = S::THREADS;
-  constexpr int SETS = G / 4;
+  constexpr int GS = G < 4 ? G : 4, SETS = G / GS;   // groups whose products are formed side by side
   // (not rounded up by hand: an address that went through an integer is a generic one to the compiler, and its loads too)
   extern __shared__ __align__(128) uint8_t u4_smem[];
   uint8_t* ring = u4_smem;
@@ -361,18 +374,19 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       *reinterpret_cast<uint4*>(q_frag + ((grp * 2) * 32 + (i & 31)) * 16) = fu;
       *reinterpret_cast<uint4*>(q_frag + ((grp * 2 + 1) * 32 + (i & 31)) * 16) = fr;
     }
-    // The bias product's B fragment: group sums as three bf16 parts. With four groups the sixteen k-slots
-    // take {hi, mid, lo, nothing}; with eight, {hi, mid}, and lo goes through a k = 8 product.
+    // The bias product's B fragment: group sums as three bf16 parts. With two groups the sixteen k-slots take
+    // {hi, mid, lo, nothing x 5}, with four {hi, mid, lo, nothing}; with eight, {hi, mid}, and lo goes through a k = 8 product.
     uint32_t qs0, qs1, qs2 = 0;
     {
       const int g = lane >> 2, t = lane & 3;
-      const int pair = G == 4 ? (t & 1) : t;
+      const int pair = G == 2 ? 0 : G == 4 ? (t & 1) : t;
       const float2 x = *reinterpret_cast<const float2*>(qsum_s + g * 8 + 2 * pair);
       const uint32_t hi = pack_bf16(x.x, x.y);
       const float2 r = make_float2(x.x - bf16_lo_f32(hi), x.y - bf16_hi_f32(hi));
       const uint32_t mid = pack_bf16(r.x, r.y);
       const uint32_t lo = pack_bf16(r.x - bf16_lo_f32(mid), r.y - bf16_hi_f32(mid));
-      if (G == 4) qs0 = t < 2 ? hi : mid, qs1 = t < 2 ? lo : 0u;
+      if (G == 2) qs0 = t == 0 ? hi : t == 1 ? mid : t == 2 ? lo : 0u, qs1 = 0u;
+      else if (G == 4) qs0 = t < 2 ? hi : mid, qs1 = t < 2 ? lo : 0u;
       else qs0 = hi, qs1 = mid, qs2 = lo;
     }
     const int g = lane >> 2, t = lane & 3;
@@ -433,8 +447,8 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       o_b[0][grp] = o_b[1][grp] = 0.0f;
     }
     float m0 = -1.0e30f, m1 = -1.0e30f, l0 = 0.0f, l1 = 0.0f;
-    const int k_off = g * (HD / 2) + t * 16;                                  // + (set ^ odd row) * 64; row g + 8: + 4 * HD
-    const int kb_off = S::BIASES + g * G * 2 + (G == 4 ? (t & 1) : t) * 4;    // K biases of row g
+    const int k_off = g * (HD / 2) + t * (HD == 64 ? 4 : 16);                 // + (set ^ odd row) * 64; row g + 8: + 4 * HD
+    const int kb_off = S::BIASES + g * G * 2 + (G == 2 ? 0 : G == 4 ? (t & 1) : t) * 4;    // K biases of row g
     const int vs_off = S::TILE + S::STEPS + t * G * 4;                        // V factors of rows 2t, 2t+1; rows + 8: + 16 * G
     const int vb_off = S::TILE + S::BIASES + g * G * 2;                       // V biases of row g; row g + 8: + 16 * G
     // Iterations that are not like the others: a page is not seen whole (the last of the sinks, the window's first, the
@@ -501,27 +515,30 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       {
         // ---- scores ----
         float z[PP][4];   // (row g; heads 2t, 2t+1), (row g + 8; ...)
-        float acc[PP][4][4];
+        float acc[PP][GS][4];
 #pragma unroll
         for (int u = 0; u < PP; ++u) z[u][0] = z[u][1] = z[u][2] = z[u][3] = 0.0f;
 #pragma unroll
         for (int set = 0; set < SETS; ++set) {
-          uint4 w0[PP], w1[PP];
+          uint32_t w0[PP][GS], w1[PP][GS];   // codes of rows g and g + 8
 #pragma unroll
           for (int u = 0; u < PP; ++u) {
-            const int at = k_off + (SETS > 1 ? (set ^ (g & 1)) : 0) * 64;
-            w0[u] = *reinterpret_cast<const uint4*>(tile[u] + at);
-            w1[u] = *reinterpret_cast<const uint4*>(tile[u] + at + 4 * HD);
+            const uint8_t* at = tile[u] + k_off + (SETS > 1 ? (set ^ (g & 1)) : 0) * 64;
+            if constexpr (HD == 64) {
+              w0[u][0] = *reinterpret_cast<const uint32_t*>(at), w0[u][1] = *reinterpret_cast<const uint32_t*>(at + 16);
+              w1[u][0] = *reinterpret_cast<const uint32_t*>(at + 4 * HD), w1[u][1] = *reinterpret_cast<const uint32_t*>(at + 4 * HD + 16);
+            } else {
+              load_words<GS>(at, w0[u]);
+              load_words<GS>(at + 4 * HD, w1[u]);
+            }
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < GS; ++j) {
             const uint4 fu = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2) * 32 + lane) * 16);
             const uint4 fr = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2 + 1) * 32 + lane) * 16);
 #pragma unroll
             for (int u = 0; u < PP; ++u) {
-              const uint32_t x0 = j == 0 ? w0[u].x : j == 1 ? w0[u].y : j == 2 ? w0[u].z : w0[u].w;
-              const uint32_t x1 = j == 0 ? w1[u].x : j == 1 ? w1[u].y : j == 2 ? w1[u].z : w1[u].w;
-              const U4Word<0x2c00> c0(x0), c1(x1);
+              const U4Word<0x2c00> c0(w0[u][j]), c1(w1[u][j]);
               mma_f16_zero(acc[u][j], c0.a_u, c1.a_u, c0.b_u, c1.b_u, fu.z, fu.w);   // the small parts first: the
               mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.z, fr.w);   // accumulator is truncated after
               mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.x, fr.y);   // every product
@@ -530,16 +547,17 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
           }
 #pragma unroll
           for (int u = 0; u < PP; ++u) {
-            const uint2 s0 = *reinterpret_cast<const uint2*>(tile[u] + S::STEPS + g * G * 2 + set * 8);
-            const uint2 s1 = *reinterpret_cast<const uint2*>(tile[u] + S::STEPS + (g + 8) * G * 2 + set * 8);
-            const float a0[4] = {bf16_lo_f32(s0.x), bf16_hi_f32(s0.x), bf16_lo_f32(s0.y), bf16_hi_f32(s0.y)};
-            const float a1[4] = {bf16_lo_f32(s1.x), bf16_hi_f32(s1.x), bf16_lo_f32(s1.y), bf16_hi_f32(s1.y)};
+            uint32_t s0[GS / 2], s1[GS / 2];
+            load_words<GS / 2>(tile[u] + S::STEPS + g * G * 2 + set * 8, s0);
+            load_words<GS / 2>(tile[u] + S::STEPS + (g + 8) * G * 2 + set * 8, s1);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              z[u][0] = fmaf(a0[j], acc[u][j][0], z[u][0]);
-              z[u][1] = fmaf(a0[j], acc[u][j][1], z[u][1]);
-              z[u][2] = fmaf(a1[j], acc[u][j][2], z[u][2]);
-              z[u][3] = fmaf(a1[j], acc[u][j][3], z[u][3]);
+            for (int j = 0; j < GS; ++j) {
+              const float a0 = j & 1 ? bf16_hi_f32(s0[j >> 1]) : bf16_lo_f32(s0[j >> 1]);
+              const float a1 = j & 1 ? bf16_hi_f32(s1[j >> 1]) : bf16_lo_f32(s1[j >> 1]);
+              z[u][0] = fmaf(a0, acc[u][j][0], z[u][0]);
+              z[u][1] = fmaf(a0, acc[u][j][1], z[u][1]);
+              z[u][2] = fmaf(a1, acc[u][j][2], z[u][2]);
+              z[u][3] = fmaf(a1, acc[u][j][3], z[u][3]);
             }
           }
         }
@@ -562,17 +580,15 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
           fma2(sb[2], sb[3], z[u][2], z[u][3], ch0, ch1);
           z[u][0] = sb[0], z[u][1] = sb[1], z[u][2] = sb[2], z[u][3] = sb[3];
         }
-        uint4 vs0[PP][SETS], vs1[PP][SETS];   // V factors: rows (2t, 2t+1) and (2t+8, 2t+9)
-        uint2 vb0[PP][SETS], vb1[PP][SETS];   // V biases: rows g and g + 8
+        uint32_t vs0[PP][G], vs1[PP][G];           // V factors of the groups: rows (2t, 2t+1) and (2t+8, 2t+9)
+        uint32_t vb0[PP][G / 2], vb1[PP][G / 2];   // V biases, two groups a word: rows g and g + 8
 #pragma unroll
-        for (int u = 0; u < PP; ++u)
-#pragma unroll
-          for (int set = 0; set < SETS; ++set) {
-            vs0[u][set] = *reinterpret_cast<const uint4*>(tile[u] + vs_off + set * 16);
-            vs1[u][set] = *reinterpret_cast<const uint4*>(tile[u] + vs_off + 16 * G + set * 16);
-            vb0[u][set] = *reinterpret_cast<const uint2*>(tile[u] + vb_off + set * 8);
-            vb1[u][set] = *reinterpret_cast<const uint2*>(tile[u] + vb_off + 16 * G + set * 8);
-          }
+        for (int u = 0; u < PP; ++u) {
+          load_words<G>(tile[u] + vs_off, vs0[u]);
+          load_words<G>(tile[u] + vs_off + 16 * G, vs1[u]);
+          load_words<G / 2>(tile[u] + vb_off, vb0[u]);
+          load_words<G / 2>(tile[u] + vb_off + 16 * G, vb1[u]);
+        }
         if (special) {
           // A row that is not seen weighs nothing, whatever its bytes say.
 #pragma unroll
@@ -589,12 +605,9 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
             const uint32_t k0 = (seen(2 * t) ? 0x0000ffffu : 0u) | (seen(2 * t + 1) ? 0xffff0000u : 0u);
             const uint32_t k1 = (seen(2 * t + 8) ? 0x0000ffffu : 0u) | (seen(2 * t + 9) ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int set = 0; set < SETS; ++set) {
-              vs0[u][set] = make_uint4(vs0[u][set].x & k0, vs0[u][set].y & k0, vs0[u][set].z & k0, vs0[u][set].w & k0);
-              vs1[u][set] = make_uint4(vs1[u][set].x & k1, vs1[u][set].y & k1, vs1[u][set].z & k1, vs1[u][set].w & k1);
-              if (!s0) vb0[u][set] = make_uint2(0u, 0u);
-              if (!s1) vb1[u][set] = make_uint2(0u, 0u);
-            }
+            for (int grp = 0; grp < G; ++grp) vs0[u][grp] &= k0, vs1[u][grp] &= k1;
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) vb0[u][i] = s0 ? vb0[u][i] : 0u, vb1[u][i] = s1 ? vb1[u][i] : 0u;
           }
         }
         float mx0 = fmaxf(z[0][0], z[0][2]), mx1 = fmaxf(z[0][1], z[0][3]);
@@ -639,16 +652,13 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
           add2(l0, l1, p[0], p[1]);
           add2(l0, l1, p[2], p[3]);
 #pragma unroll
-          for (int set = 0; set < SETS; ++set) {
-            const float b0[4] = {bf16_lo_f32(vb0[u][set].x), bf16_hi_f32(vb0[u][set].x), bf16_lo_f32(vb0[u][set].y), bf16_hi_f32(vb0[u][set].y)};
-            const float b1[4] = {bf16_lo_f32(vb1[u][set].x), bf16_hi_f32(vb1[u][set].x), bf16_lo_f32(vb1[u][set].y), bf16_hi_f32(vb1[u][set].y)};
+          for (int i = 0; i < G / 2; ++i) {
+            const float b0[2] = {bf16_lo_f32(vb0[u][i]), bf16_hi_f32(vb0[u][i])}, b1[2] = {bf16_lo_f32(vb1[u][i]), bf16_hi_f32(vb1[u][i])};
 #pragma unroll
-            for (int j = 0; j < 4; j += 2)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                fma2(o_b[h][set * 4 + j], o_b[h][set * 4 + j + 1], b0[j], b0[j + 1], p[h], p[h]);
-                fma2(o_b[h][set * 4 + j], o_b[h][set * 4 + j + 1], b1[j], b1[j + 1], p[2 + h], p[2 + h]);
-              }
+            for (int h = 0; h < 2; ++h) {
+              fma2(o_b[h][2 * i], o_b[h][2 * i + 1], b0[0], b0[1], p[h], p[h]);
+              fma2(o_b[h][2 * i], o_b[h][2 * i + 1], b1[0], b1[1], p[2 + h], p[2 + h]);
+            }
           }
         }
         // ---- outputs. The matrix instruction truncates its f32 sum: hundreds of them in one accumulator shrink it
@@ -664,9 +674,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
             w[u] = *reinterpret_cast<const uint4*>(tile[u] + S::TILE + (pair * 32 + lane) * 16);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const uint4 f0 = vs0[u][pair >> 1], f1 = vs1[u][pair >> 1];
-              const uint32_t s0 = (pair & 1) ? (j ? f0.w : f0.z) : (j ? f0.y : f0.x);
-              const uint32_t s1 = (pair & 1) ? (j ? f1.w : f1.z) : (j ? f1.y : f1.x);
+              const uint32_t s0 = vs0[u][pair * 2 + j], s1 = vs1[u][pair * 2 + j];
               wh[u][j][0] = hmul2_u32(ph[u][0], s0), wh[u][j][1] = hmul2_u32(ph[u][1], s1);
               wl[u][j][0] = hfma2_u32(pl[u][0], s0, hfms2_u32(ph[u][0], s0, wh[u][j][0]));
               wl[u][j][1] = hfma2_u32(pl[u][1], s1, hfms2_u32(ph[u][1], s1, wh[u][j][1]));
@@ -752,39 +760,39 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
 }
 
 bool attention_u4_supported(int dtype, int head_dim, int gqa) {
-  return dtype == KV_U4G32 && (head_dim == 128 || head_dim == 256) && gqa >= 1 && gqa <= 8;
+  return dtype == KV_U4G32 && (head_dim == 64 || head_dim == 128 || head_dim == 256) && gqa >= 1 && gqa <= 8;
 }
 
-int attention_u4_blocks_per_sm(int head_dim) { return head_dim == 128 ? U4Shape<128>::BLOCKS : U4Shape<256>::BLOCKS; }
-static const void* u4_kernel(int head_dim, bool cluster, bool peers) {
-  if (head_dim == 128)
-    return peers     ? reinterpret_cast<const void*>(attention_u4_kernel<128, false, true>)
-           : cluster ? reinterpret_cast<const void*>(attention_u4_kernel<128, true, false>)
-                     : reinterpret_cast<const void*>(attention_u4_kernel<128, false, false>);
-  return peers     ? reinterpret_cast<const void*>(attention_u4_kernel<256, false, true>)
-         : cluster ? reinterpret_cast<const void*>(attention_u4_kernel<256, true, false>)
-                   : reinterpret_cast<const void*>(attention_u4_kernel<256, false, false>);
+// The instances of one head size, and what they need.
+struct U4Instance {
+  const void* kernels[3];   // plain, cluster, peers
+  int blocks_per_sm, threads, smem, cluster_smem;
+};
+template <int HD>
+static U4Instance u4_instance() {
+  return {{reinterpret_cast<const void*>(attention_u4_kernel<HD, false, false>), reinterpret_cast<const void*>(attention_u4_kernel<HD, true, false>),
+           reinterpret_cast<const void*>(attention_u4_kernel<HD, false, true>)},
+          U4Shape<HD>::BLOCKS, U4Shape<HD>::WARPS * 32, U4Smem<HD, false>::TOTAL, U4Smem<HD, true>::TOTAL};
 }
-static size_t u4_smem_bytes(int head_dim, bool cluster) {
-  if (head_dim == 128) return cluster ? U4Smem<128, true>::TOTAL : U4Smem<128, false>::TOTAL;
-  return cluster ? U4Smem<256, true>::TOTAL : U4Smem<256, false>::TOTAL;
+static U4Instance u4_instance(int head_dim) {
+  return head_dim == 64 ? u4_instance<64>() : head_dim == 128 ? u4_instance<128>() : u4_instance<256>();
 }
 
-static int u4_threads(int head_dim) { return 32 * (head_dim == 128 ? U4Shape<128>::WARPS : U4Shape<256>::WARPS); }
+int attention_u4_blocks_per_sm(int head_dim) { return u4_instance(head_dim).blocks_per_sm; }
 
 int attention_u4_resident_blocks(int head_dim) {
+  const U4Instance x = u4_instance(head_dim);
   int blocks = 0;
-  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, u4_kernel(head_dim, false, false), u4_threads(head_dim),
-                                                                u4_smem_bytes(head_dim, false));
-  return e == cudaSuccess ? blocks : 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, x.kernels[0], x.threads, x.smem) == cudaSuccess ? blocks : 0;
 }
 
 // How many clusters of `splits` blocks the device can hold at once (0: such a launch would fail).
 int attention_u4_max_clusters(int head_dim, int splits) {
+  const U4Instance x = u4_instance(head_dim);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, 1, 1);
-  cfg.blockDim = dim3(u4_threads(head_dim));
-  cfg.dynamicSmemBytes = u4_smem_bytes(head_dim, true);
+  cfg.blockDim = dim3(x.threads);
+  cfg.dynamicSmemBytes = x.cluster_smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = splits;
@@ -793,7 +801,7 @@ int attention_u4_max_clusters(int head_dim, int splits) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, u4_kernel(head_dim, true, false), &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, x.kernels[1], &cfg) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
@@ -801,26 +809,29 @@ int attention_u4_max_clusters(int head_dim, int splits) {
 }
 
 cudaError_t attention_u4_configure() {
-  for (int hd : {128, 256})
+  for (int hd : {64, 128, 256}) {
+    const U4Instance x = u4_instance(hd);
     for (int kind = 0; kind < 3; ++kind) {
-      const void* kernel = u4_kernel(hd, kind == 1, kind == 2);
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+      cudaError_t e = cudaFuncSetAttribute(x.kernels[kind], cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
       // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
-      if (e == cudaSuccess && kind == 1) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e == cudaSuccess && kind == 1) e = cudaFuncSetAttribute(x.kernels[kind], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return e;
     }
+  }
   return cudaSuccess;
 }
 
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream) {
+  const U4Instance x = u4_instance(a.pool.head_dim);
+  const bool peers = a.n_peers > 0, cluster = a.cluster_merge && !peers;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.splits, a.pool.kv_heads, n_seq);
-  cfg.blockDim = dim3(u4_threads(a.pool.head_dim));
-  cfg.dynamicSmemBytes = u4_smem_bytes(a.pool.head_dim, a.cluster_merge && a.n_peers == 0);
+  cfg.blockDim = dim3(x.threads);
+  cfg.dynamicSmemBytes = cluster ? x.cluster_smem : x.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n_attr = 0;
-  if (a.cluster_merge && a.n_peers == 0) {
+  if (cluster) {
     // the splits of a (sequence, KV head) are the x extent of the grid and of the cluster
     attr[n_attr].id = cudaLaunchAttributeClusterDimension;
     attr[n_attr].val.clusterDim.x = a.splits;
@@ -841,7 +852,7 @@ cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t strea
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
   void* args[1] = {const_cast<AttnArgs*>(&a)};
-  return cudaLaunchKernelExC(&cfg, u4_kernel(a.pool.head_dim, a.cluster_merge && a.n_peers == 0, a.n_peers > 0), args);
+  return cudaLaunchKernelExC(&cfg, x.kernels[peers ? 2 : cluster ? 1 : 0], args);
 }
 
 }  // namespace sgk
