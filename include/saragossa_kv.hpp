@@ -48,7 +48,7 @@ struct Result {
 };
 struct Unit {};
 
-enum class GpuElement : int32_t { F32 = SGK_KV_F32, Bf16 = SGK_KV_BF16, U8G32 = SGK_KV_U8G32 };
+enum class GpuElement : int32_t { F32 = SGK_KV_F32, Bf16 = SGK_KV_BF16, U8G32 = SGK_KV_U8G32, U4G32 = SGK_KV_U4G32 };
 
 // KV dtype policy of the reference (src/decode_resident/utils.rs:202-228): an explicit
 // RETI_RUST_KV_BF16 (1/true/on, 0/false/off) wins; otherwise bf16 when sampling, f32 greedy.
@@ -93,6 +93,11 @@ class FullAttentionState {
   size_t byte_len() const { return static_cast<size_t>(sgk_kv_byte_len(h_)); }
 
   Result<Unit> truncate(size_t len) { return unit(sgk_kv_truncate(h_, static_cast<int64_t>(len))); }
+  // truncate in stream order, without waiting
+  Result<Unit> encode_truncate(void* stream, size_t len) { return unit(sgk_kv_enqueue_truncate(h_, stream, static_cast<int64_t>(len))); }
+  // the first `rows` rows stay visible to every windowed attention
+  Result<Unit> set_attention_sinks(size_t rows) { return unit(sgk_kv_set_attention_sinks(h_, static_cast<int64_t>(rows))); }
+  size_t attention_sinks() const { return static_cast<size_t>(sgk_kv_attention_sinks(h_)); }
   Result<Unit> seed(const std::vector<float>& keys_rows, const std::vector<float>& values_rows, size_t n_rows) {
     return unit(sgk_kv_seed_f32(h_, keys_rows.data(), keys_rows.size(), values_rows.data(), values_rows.size(),
                                 static_cast<int64_t>(n_rows)));
@@ -130,6 +135,10 @@ class FullAttentionState {
                                        const float* d_knorm_weight, size_t rope_dims, float theta, float eps) {
     sgk_rope rope{static_cast<int32_t>(rope_dims), static_cast<int32_t>(rope_dims), theta, 1.0f, eps, 0};
     return unit(sgk_kv_enqueue_rope_append_rows(h_, stream, d_k_raw, d_v, static_cast<int64_t>(n_rows), d_knorm_weight, &rope));
+  }
+  // Rows [row0, row0 + n) decoded to f32 into device memory, [n][kv_dim] each.
+  Result<Unit> encode_gather_rows_f32(void* stream, size_t row0, size_t n, float* d_k, float* d_v) {
+    return unit(sgk_kv_enqueue_gather_rows_f32(h_, stream, static_cast<int64_t>(row0), static_cast<int64_t>(n), d_k, d_v));
   }
   // kv.keys() / kv.values() read-back of the valid rows, decoded to f32.
   Result<std::vector<float>> keys() { return rows(true); }

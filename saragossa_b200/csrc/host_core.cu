@@ -502,7 +502,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   int kernel = choose_kernel();
   if (kernel < 0) return fail(SGK_ERR_BACKEND, "tensor-core attention kernel does not take this shape");
   int64_t max_rows = 0;
-  const int64_t sink_rows = kvs[0]->sink_rows;
+  const int64_t sink_rows = std::min<int64_t>(kvs[0]->sink_rows, INT32_MAX);   // (no sequence is longer)
   for (Kv* kv : kvs) {
     int64_t len_after = kv->len() + (fused ? 1 : 0);
     if (fused && kv->len() >= kv->seq->capacity)
@@ -512,7 +512,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     if (ws < 0 || ws >= len_after)
       return fail(SGK_ERR_DIMENSION, "attention_decode empty window: start=%lld, len=%lld", (long long)ws,
                   (long long)len_after);
-    if (kv->sink_rows != sink_rows) return fail(SGK_ERR_CONFIG, "batch members must share the number of attention sinks");
+    if (kv->sink_rows != kvs[0]->sink_rows) return fail(SGK_ERR_CONFIG, "batch members must share the number of attention sinks");
     const SinkSpan sinks(sink_rows, ws);
     if (kv->seq->released(ws / PAGE_TOKENS, (len_after + PAGE_TOKENS - 1) / PAGE_TOKENS) || kv->seq->released(0, sinks.pages))
       return fail(SGK_ERR_DIMENSION, "attention window reaches rows released by the sliding window");

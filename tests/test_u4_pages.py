@@ -475,3 +475,83 @@ def test_verify_rows_and_prefix_restore_over_u4_pages(state):
     _check_codes(kv, k[:n + 2], v[:n + 2], hd)
     for x in (cache, seq, other, pool):
         x.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("spread", [[1e18, 1.0], [1e-12, 1.0], [1e12, 1e-12, 1.0], [1e-30], [1e15]])
+def test_values_of_very_different_sizes(state, hd, spread):
+    """V rows of very different ranges in one sequence, whatever their attention weights: every row keeps its share, and the
+    sum of the weights loses none."""
+    n, q_heads, kv_heads = 600, 8, 2
+    rng = np.random.default_rng(17)
+    k, v = rng.standard_normal((2, n, kv_heads * hd)).astype(np.float32)
+    v *= np.asarray(spread, np.float32)[np.arange(n) % len(spread)][:, None]
+    k[::7] *= np.float32(3.0)
+    kv = state.full_attention(n, q_heads, kv_heads, hd, sg.KV_U4G32, shuffled_seed=9)
+    kv.seed(k, v, n)
+    q = rng.standard_normal((q_heads, hd)).astype(np.float32)
+    want = ref.attention(q, ref.stored(k, 0, hd, 3), ref.stored(v, 0, hd, 3), kv_heads)
+    assert ref.close(kv.attention_decode(q), want)[0]
+    kv.close()
+
+
+@pytest.mark.gpu
+def test_two_streams_and_a_pending_append(state):
+    """Two KV states of one pool used on two streams of the caller, each with its own batch; then the append and the attention
+    of one of them in stream order behind a long computation."""
+    import torch
+    q_heads, kv_heads, hd, n = 16, 2, 128, 1500
+    rng = np.random.default_rng(23)
+    state.set_concurrent_streams(True)
+    kvs = [filled(state, n, q_heads, kv_heads, hd, seed=s, cap=n + 40) for s in (1, 2)]
+    q = rng.standard_normal((2, q_heads, hd)).astype(np.float32)
+    new = rng.standard_normal((2, 2, 20, kv_heads * hd)).astype(np.float32)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    busy = torch.randn(4096, 4096, device="cuda")
+    bufs = [[state.upload(x) for x in (new[s, 0], new[s, 1], q[s])] + [state.alloc(q[s].nbytes)] for s in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for (kv, k, v), st, (d_k, d_v, d_q, d_out) in zip(kvs, streams, bufs):
+            with torch.cuda.stream(st):
+                busy @ busy
+            h = st.cuda_stream
+            kv.encode_truncate(n, stream=h)
+            kv.encode_append_rows(d_k, d_v, 20, stream=h)
+            kv.encode_attention_decode_windowed(d_q, d_out, stream=h)
+    torch.cuda.synchronize()
+    for s, (kv, k, v) in enumerate(kvs):
+        rows = [np.concatenate([old, ref.stored(x, n, hd, 3)]) for old, x in ((k, new[s, 0]), (v, new[s, 1]))]
+        assert kv.len() == n + 20
+        assert ref.close(bufs[s][3].download(), ref.attention(q[s], *rows, kv_heads))[0], s
+        kv.close()
+    state.set_concurrent_streams(False)
+
+
+@pytest.mark.gpu
+def test_batched_truncate_moves_every_cursor(state):
+    n_seq, cap = 600, 33                     # more members than one launch takes
+    pool = state.pool(2, 1, 32, sg.KV_U4G32, n_seq * 3, n_seq, cap)
+    seqs = [pool.sequence(cap) for _ in range(n_seq)]
+    kvs = [s.layer(1, 1) for s in seqs]
+    batch = sg.Batch(state, kvs)
+    d = state.upload(np.ones((n_seq, 32), np.float32))
+    for _ in range(20):
+        batch.enqueue_append(d, d)
+    lens = [(7 * i) % 21 for i in range(n_seq)]
+    batch.enqueue_truncate(lens)
+    batch.enqueue_append(d, d)               # the device's cursors are the ones that count here
+    state.sync()
+    assert [kv.len() for kv in kvs] == [n + 1 for n in lens]
+    assert all(s.layer(0, 1).len() == 0 for s in seqs[:5])
+    for i in (0, 1, 2, 511, 512, 599):
+        kvs[i].gather_rows_f32(0, lens[i] + 1)
+    bad = list(lens)
+    bad[599] = cap + 1
+    for wrong in (bad, lens[:-1]):
+        with pytest.raises(sg.InferError) as e:
+            batch.enqueue_truncate(wrong)
+        assert e.value.kind == "Dimension"
+    assert [kv.len() for kv in kvs] == [n + 1 for n in lens]
+    for x in (batch, *seqs, pool):
+        x.close()
