@@ -334,25 +334,18 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       if (f < 8 * HD) *reinterpret_cast<float4*>(q_rows + f) = v[k];
     }
     __syncthreads();
-    // Sums of the groups, and the power of two that brings the largest |q| to 2^15..2^16.
+    // The power of two that brings the largest |q| of a head to 2^15..2^16.
 #pragma unroll
     for (int h = warp; h < 8; h += WARPS) {
       float big = 0.0f;
 #pragma unroll
-      for (int grp = 0; grp < G; ++grp) {
-        const float x = q_rows[h * HD + grp * QGROUP + lane];
-        big = fmaxf(big, fabsf(x));
-        float sum = x;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == grp) qsum_s[h * 8 + grp] = sum;
-      }
-      if (G < 8 && lane >= G && lane < 8) qsum_s[h * 8 + lane] = 0.0f;
+      for (int grp = 0; grp < G; ++grp) big = fmaxf(big, fabsf(q_rows[h * HD + grp * QGROUP + lane]));
       asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(big) : "f"(big));
       if (lane == 0) {
         const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
         qpow_s[h] = pow2f(max(-90, min(90, e - 15)));   // q = qpow * (what the fragments hold)
       }
+      if (G < 8 && lane >= G && lane < 8) qsum_s[h * 8 + lane] = 0.0f;
     }
     __syncthreads();
     for (int i = tid; i < G * 32; i += THREADS) {
@@ -360,6 +353,11 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       const float inv = 1.0f / qpow_s[h];
       const float* row = q_rows + h * HD + grp * QGROUP + 4 * t;
       const float4 x = *reinterpret_cast<const float4*>(row), y = *reinterpret_cast<const float4*>(row + 16);
+      // the group's sum, over the four threads that hold it
+      float sum = (x.x + x.y) + (x.z + x.w) + ((y.x + y.y) + (y.z + y.w));
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (t == 0) qsum_s[h * 8 + grp] = sum;
       // n0 x + n1 y = n0 (x - y / 16) + u (y / 16), with u in units of 2^-24 and n0 in units of 2^-14
       const float s = inv * 0.0625f, d = 0x1p-10f;
       const float u[4] = {y.x * s, y.y * s, y.z * s, y.w * s};
@@ -374,6 +372,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       *reinterpret_cast<uint4*>(q_frag + ((grp * 2) * 32 + (i & 31)) * 16) = fu;
       *reinterpret_cast<uint4*>(q_frag + ((grp * 2 + 1) * 32 + (i & 31)) * 16) = fr;
     }
+    __syncthreads();   // fragments and sums written
     // The bias product's B fragment: group sums as three bf16 parts. With two groups the sixteen k-slots take
     // {hi, mid, lo, nothing x 5}, with four {hi, mid, lo, nothing}; with eight, {hi, mid}, and lo goes through a k = 8 product.
     uint32_t qs0, qs1, qs2 = 0;
@@ -391,7 +390,6 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
     }
     const int g = lane >> 2, t = lane & 3;
     const float ch0 = qpow_s[2 * t] * 16777216.0f, ch1 = qpow_s[2 * t + 1] * 16777216.0f;   // products are in units of 2^-24
-    __syncthreads();   // fragments written
 
     // The row of a fused append is quantised now, by the warp with the fewest pages, while the first pages are
     // on their way; its bytes go to the page in global memory and stay parked in shared memory for the warp
@@ -754,7 +752,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
     }
   }
   __syncthreads();
-  finish_block<HD, CLUSTER, PEERS, THREADS, 1, WARPS>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
+  finish_block<HD, CLUSTER, PEERS, THREADS, 1, WARPS, true>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
                                    splits, recv_s);
   if (PEERS) peers_finish(a, tid, flags);
 }
