@@ -231,7 +231,8 @@ int32_t sgk_rms_norm_rope_decode(sgk_state* state, const float* x, const float* 
  * src/decoder/attention_ops.rs:912). */
 int32_t sgk_kv_attention_decode(sgk_kv* kv, const float* q, size_t q_len, int64_t window_start,
                                 float attn_scalar, float* out);
-/* kv.encode_attention_decode_windowed(enc,q,scores,out,ws) (attention.rs:736-835) */
+/* kv.encode_attention_decode_windowed(enc,q,scores,out,ws) (attention.rs:736-835). Rows (q, out, k, v) at addresses
+ * that are not multiples of 16 bytes go to the generic kernels here and in the append and step calls. */
 int32_t sgk_kv_enqueue_attention(sgk_kv* kv, void* stream, const float* d_q, float* d_out,
                                  int64_t window_start, float attn_scalar);
 /* NO COUNTERPART IN THE REFERENCE. Same computation and same errors as
@@ -287,7 +288,8 @@ int32_t sgk_batch_enqueue_step(sgk_batch* batch, void* stream, const float* d_k,
                                const float* d_q, float* d_out, int64_t sliding_window,
                                float attn_scalar);
 /* Moves the cursor of every member, in stream order (lens: [n], host memory; one launch per 512 members):
- * drops the rejected tails of a batched verify, which differ from sequence to sequence. */
+ * drops the rejected tails of a batched verify, which differ from sequence to sequence. A sequence that is a member
+ * twice has one length (Dimension error otherwise). */
 int32_t sgk_batch_enqueue_truncate(sgk_batch* batch, void* stream, const int64_t* lens);
 /* Tuning hooks read by the benchmark: 0 = automatic. */
 /* Speculative-decoding verify (src/decode_resident/layers.rs:1295-1433; CPU twin

@@ -36,6 +36,9 @@ const char* last_error_cstr();
     if (rc_ != SGK_OK) return rc_; \
   } while (0)
 
+// The vector loads and stores of the fast kernels take 16-byte aligned addresses (null counts as aligned).
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 struct Exchange;
 // What an attention over rows [0, len) with a window from row `start` sees beside the window: the pages
 // [0, pages) that hold the sinks (fewer where they reach the window's first page) and `rows` rows of them.

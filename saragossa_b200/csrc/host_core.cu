@@ -186,7 +186,7 @@ void Seq::new_epoch() {
 
 int Seq::release_between(int64_t first_row, int64_t row) {
   const int64_t have = static_cast<int64_t>(pages.size());
-  int64_t first = std::min((first_row + PAGE_TOKENS - 1) / PAGE_TOKENS, have);
+  int64_t first = std::min(first_row / PAGE_TOKENS + (first_row % PAGE_TOKENS != 0), have);
   int64_t upto = std::min<int64_t>(row / PAGE_TOKENS, have);
   if (upto > first && released_pages > released_first) {
     // what has been returned stays one range: it grows at either end
@@ -477,6 +477,11 @@ int Batch::enqueue_truncate(cudaStream_t stream, const int64_t* lens) {
   for (int i = 0; i < n(); ++i)
     if (lens[i] < 0 || lens[i] > kvs[i]->seq->capacity)
       return fail(SGK_ERR_DIMENSION, "truncate KV %lld > capacity %lld", (long long)lens[i], (long long)kvs[i]->seq->capacity);
+  for (int i = 0; i < n(); ++i)
+    for (int j = 0; j < i; ++j)
+      if (kvs[i]->seq == kvs[j]->seq && lens[i] != lens[j])
+        return fail(SGK_ERR_DIMENSION, "truncate: members %d and %d are one sequence, with lengths %lld and %lld", j, i,
+                    (long long)lens[j], (long long)lens[i]);
   for (int i = 0; i < n(); ++i) SGK_TRY(kvs[i]->seq->reserve(lens[i]));
   SetLensArgs a{};
   a.lens = pool->d_lens;
@@ -501,6 +506,10 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
   const bool fused = d_k_new != nullptr;
   int kernel = choose_kernel();
   if (kernel < 0) return fail(SGK_ERR_BACKEND, "tensor-core attention kernel does not take this shape");
+  if (kernel >= 2 && !(aligned16(d_q) && aligned16(d_out) && aligned16(d_k_new) && aligned16(d_v_new))) {
+    if (kernel_override == 2) return fail(SGK_ERR_BACKEND, "tensor-core attention kernel needs 16-byte aligned rows");
+    kernel = 1;   // reads and writes single floats
+  }
   int64_t max_rows = 0;
   const int64_t sink_rows = std::min<int64_t>(kvs[0]->sink_rows, INT32_MAX);   // (no sequence is longer)
   for (Kv* kv : kvs) {
@@ -550,7 +559,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     std::vector<int64_t> pages_of;
     for (Kv* kv : kvs) {
       int64_t rows = kv->len() + (fused ? 1 : 0);
-      if (sliding_window > 0) rows = std::min<int64_t>(rows, sliding_window + PAGE_TOKENS + sink_rows);
+      if (sliding_window > 0) rows = std::min<int64_t>(rows, std::min(sliding_window, rows) + PAGE_TOKENS + sink_rows);
       else rows -= std::min<int64_t>(rows, window_start) - SinkSpan(sink_rows, std::min<int64_t>(rows, window_start)).rows;
       const int64_t pages = (rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
       lo = std::min(lo, pages), hi = std::max(hi, pages), total += pages;

@@ -517,8 +517,7 @@ __global__ void __launch_bounds__(128, DIRECT ? 16 : 8) append_tiles_kernel(Appe
 
 // ---- bulk append into u4 pages without rope: one block per (kv head, page, sequence) ----------------------
 // A thread takes eight values of a group (two 16-byte loads), so a group's range costs two shuffle steps and its bias,
-// step and exponent are worked out by four lanes instead of thirty-two (a warp per row, a lane per dim: 478 us for 32768
-// rows of 4 heads of 128; this: FILL). All rows of the page tile are in registers before the first is quantised. A full tile
+// step and exponent are worked out by four lanes instead of thirty-two. All rows of the page tile are in registers before the first is quantised. A full tile
 // is put together in shared memory and leaves with 16-byte stores, a partial one is written in place.
 template <int HD>
 __global__ void __launch_bounds__(128) append_u4_tiles_kernel(AppendArgs a) {
@@ -645,7 +644,8 @@ cudaError_t launch_rope_table(float2* table, int64_t row0, int n_rows, const Rop
 
 cudaError_t launch_append_rows(const AppendArgs& a, int n_seq, cudaStream_t stream) {
   const int hd = a.pool.head_dim;
-  if (a.n_rows >= 4 && a.out_k == nullptr && (hd == 64 || hd == 128 || hd == 256)) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) % 16 == 0;   // 16-byte loads
+  if (a.n_rows >= 4 && aligned && a.out_k == nullptr && (hd == 64 || hd == 128 || hd == 256)) {
     // bulk: one block per page tile; the first row may sit anywhere in its page, so one tile more
     dim3 grid(a.pool.kv_heads, (a.n_rows + PAGE_TOKENS - 1) / PAGE_TOKENS + 1, n_seq);
     // the kernel's carve-up: K rows, 1/rms per row, rope denominators (<= 128 pairs); V rows and a

@@ -131,9 +131,10 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
 
   // the same kernel selection as the allocating entry point: tensor-core kernels over bf16, u8 and
   // u4 group-32 pages, the generic kernel for everything else
-  const bool u4 = attention_u4_supported(pool->dtype, hd, qh / kvh);
-  const bool u8 = attention_u8_supported(pool->dtype, hd, qh / kvh);
-  const bool mma = u4 || u8 || attention_mma_supported(pool->dtype, hd, qh / kvh);
+  const bool aligned = aligned16(d_q) && aligned16(d_out);   // else the generic kernel, which reads and writes single floats
+  const bool u4 = aligned && attention_u4_supported(pool->dtype, hd, qh / kvh);
+  const bool u8 = aligned && attention_u8_supported(pool->dtype, hd, qh / kvh);
+  const bool mma = u4 || u8 || (aligned && attention_mma_supported(pool->dtype, hd, qh / kvh));
   // split count: fill the SMs (two blocks each for the tensor-core kernel, eight for the
   // generic one), keep a few pages per split, and stay inside the static workspace
   const int64_t pages = (len - window_start + PAGE_TOKENS - 1) / PAGE_TOKENS + sinks.pages;

@@ -33,6 +33,7 @@ def _held(seq):
     ([(100, 20)], list(range(8))),
     ([(4, 100), (0, 0), (90, 10)], [0, 6, 7]),
     ([(0, 1000)], []),
+    ([(2**63 - 1, 100), (0, 2**63 - 1)], []),      # the first names no page
 ])
 def test_release_between(calls, held):
     pool, seq = _host_seq(128)
@@ -287,4 +288,78 @@ def test_uneven_batch_with_sinks(state, dtype, splits):
     for i in range(len(lens)):
         assert _close(got[i], want[i], dtype), (splits, i)
     for x in (batch, *seqs, pool):
+        x.close()
+
+
+class _At:
+    """A device address that is not a multiple of 16."""
+
+    def __init__(self, state, array):
+        self.buf = state.alloc(array.nbytes + 16)
+        self.ptr, self.shape, self.state = self.buf.ptr + 4, array.shape, state
+        self.base = np.zeros(array.size + 4, np.float32)
+        self.base[1:1 + array.size] = array.ravel()
+        self.buf.upload(self.base)
+
+    def download(self):
+        return self.buf.download()[1:1 + int(np.prod(self.shape))].reshape(self.shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [sg.KV_U4G32, sg.KV_BF16, sg.KV_U8G32])
+def test_addresses_between_the_vector_boundaries(state, dtype):
+    n, q_heads, kv_heads, hd, window, sinks = 90, 8, 2, 128, 40, 6
+    rng = np.random.default_rng(3)
+    k, v = rng.standard_normal((2, n + 1, kv_heads * hd)).astype(np.float32)
+    q = rng.standard_normal((q_heads, hd)).astype(np.float32)
+    twin = state.full_attention(n + 8, q_heads, kv_heads, hd, dtype)     # the same rows from aligned addresses
+    twin.seed(k, v, n + 1)
+    held = [x.reshape(n + 1, -1).astype(np.float64) for x in twin.gather_rows_f32(0, n + 1)]
+    twin.close()
+    kv = state.full_attention(n + 8, q_heads, kv_heads, hd, dtype, shuffled_seed=4)
+    kv.set_attention_sinks(sinks)
+    d_out = _At(state, np.zeros_like(q))
+    kv.encode_append_rows(_At(state, k[:n]), _At(state, v[:n]), n)
+    state.sync()
+    assert np.array_equal(kv.gather_rows_f32(0, n)[0], held[0][:n].astype(np.float32))
+    for call in (kv.encode_attention_decode_windowed, kv.encode_attention_decode_noalloc):
+        call(_At(state, q), d_out, n - window)
+        state.sync()
+        assert ref.close(d_out.download(), ref.attention(q, held[0][:n], held[1][:n], kv_heads, n - window, sinks))[0]
+    kv.encode_append_attention(_At(state, k[n:]), _At(state, v[n:]), _At(state, q), d_out, window)
+    state.sync()
+    assert ref.close(d_out.download(), ref.attention(q, *held, kv_heads, n + 1 - window, sinks))[0]
+    assert np.array_equal(kv.gather_rows_f32(n, 1)[1], held[1][n:].astype(np.float32))
+    kv.close()
+
+
+@pytest.mark.gpu
+def test_uneven_batch_with_the_widest_window(state):
+    lens, hd = (600, 9), 64
+    pool = state.pool(1, 1, hd, sg.KV_U4G32, 64, 2, 640)
+    rng = np.random.default_rng(8)
+    seqs = [pool.sequence(640) for _ in lens]
+    kvs, want, q = [s.layer(0, 2) for s in seqs], [], rng.standard_normal((2, 2, hd)).astype(np.float32)
+    for i, n in enumerate(lens):
+        k, v = rng.standard_normal((2, n, hd)).astype(np.float32)
+        kvs[i].seed(k, v, n)
+        kvs[i].set_attention_sinks(2**63 - 1)
+        want.append(ref.attention(q[i], *(ref.stored(x, 0, hd, sg.KV_U4G32) for x in (k, v)), 1))
+    batch = sg.Batch(state, kvs)
+    d_q, d_out = state.upload(q), state.alloc(q.nbytes)
+    for window in (2**63 - 1, 1):                 # every row is in the window, or every row is a sink
+        batch.enqueue_attention(d_q, d_out, window)
+        state.sync()
+        got = d_out.download().reshape(q.shape)
+        assert all(ref.close(got[i], want[i])[0] for i in range(2))
+    twice = sg.Batch(state, [kvs[0], kvs[0]])     # one sequence, two queries
+    twice.enqueue_attention(d_q, d_out, 0)
+    state.sync()
+    assert ref.close(d_out.download().reshape(q.shape)[0], want[0])[0]
+    with pytest.raises(sg.InferError) as e:       # but not two lengths
+        twice.enqueue_truncate([20, 30])
+    assert e.value.kind == "Dimension" and kvs[0].len() == 600
+    twice.enqueue_truncate([20, 20])
+    assert kvs[0].len() == 20
+    for x in (twice, batch, *seqs, pool):
         x.close()
