@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(128, DIRECT ? 16 : 8) append_tiles_kernel(Appe
                                          : u4_quantize_lanes<8>(v, odd, lane);
           if ((task >> 1) < rows) {
             u4_store_codes(is_v ? kt + tile_b : kt, hd, is_v, rin0 + r, grp, q, out.word);
-            u4_store_meta(kt, kt + tile_b, hd, is_v, rin0 + r, grp, q, out);
+            if (q == 0) u4_store_meta(kt, kt + tile_b, hd, is_v, rin0 + r, grp, out);
           }
         }
         if (full) {
@@ -556,28 +556,41 @@ __global__ void __launch_bounds__(128) append_u4_tiles_kernel(AppendArgs a) {
     }
     if (page >= 0 && page < a.num_pages) {
       uint8_t* global = a.pool.base + tile_offset(a.pool, page, a.layer, head, 0);
-      if (rows == PAGE_TOKENS) {
-        uint32_t v_words[TASKS / 2];
+      const bool full = rows == PAGE_TOKENS;
+      constexpr int B = TASKS < 4 ? TASKS : 4;   // pieces whose ranges the four lanes of a group share
+      static_assert(PASS % 2 == 0, "rows of a thread have one parity");
+      const uint32_t odd = (rin0 + tid / ROW_LANES) & 1;
+      uint32_t word[TASKS];
 #pragma unroll
-        for (int i = 0; i < TASKS; ++i) {
-          const int r = (i >> 1) * PASS + tid / ROW_LANES;
-          const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
-          const U4Lane out = u4_quantize_lanes<ROW_LANES>(v, r & 1, lane);
-          u4_store_meta(stage, stage + TILE, HD, i & 1, r, grp, q, out);
-          if (i & 1) v_words[i >> 1] = out.word;
-          else u4_store_codes(stage, HD, 0, r, grp, q, out.word);
+      for (int base = 0; base < TASKS; base += B) {
+        float v[B][8];
+        uint32_t w[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const float4 lo = x[base + i], hi = y[base + i];
+          v[i][0] = lo.x, v[i][1] = lo.y, v[i][2] = lo.z, v[i][3] = lo.w;
+          v[i][4] = hi.x, v[i][5] = hi.y, v[i][6] = hi.z, v[i][7] = hi.w;
         }
-        // V bytes of rows r and r + 8 are neighbours: where one thread has both, they leave together
+        const U4Lane out = u4_quantize_pieces<ROW_LANES, B>(v, odd, lane, w);
+#pragma unroll
+        for (int i = 0; i < B; ++i) word[base + i] = w[i];
+        const int mine = base + q, r = (mine >> 1) * PASS + tid / ROW_LANES;   // the piece whose range this lane has
+        if (q < B && full) u4_store_meta(stage, stage + TILE, HD, mine & 1, r, grp, out);
+        else if (q < B && r < rows) u4_store_meta(global, global + TILE, HD, mine & 1, rin0 + r, grp, out);
+      }
+      if (full) {
 #pragma unroll
         for (int i = 0; i < TASKS / 2; ++i) {
           const int r = i * PASS + tid / ROW_LANES;
+          u4_store_codes(stage, HD, 0, r, grp, q, word[2 * i]);
+          // V bytes of rows r and r + 8 are neighbours: where one thread has both, they leave together
           if (PASS > 8) {
-            u4_store_codes(stage + TILE, HD, 1, r, grp, q, v_words[i]);
+            u4_store_codes(stage + TILE, HD, 1, r, grp, q, word[2 * i + 1]);
           } else if (i < TASKS / 4) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *reinterpret_cast<uint16_t*>(stage + TILE + u4_v_byte(r, grp * QGROUP + 4 * q + j, HD)) =
-                  static_cast<uint16_t>(__byte_perm(v_words[i], v_words[i + TASKS / 4], 0x40 + 0x11 * j));
+                  static_cast<uint16_t>(__byte_perm(word[2 * i + 1], word[(2 * i + TASKS / 2 + 1) % TASKS], 0x40 + 0x11 * j));
           }
         }
         __syncthreads();
@@ -585,13 +598,8 @@ __global__ void __launch_bounds__(128) append_u4_tiles_kernel(AppendArgs a) {
       } else {
 #pragma unroll
         for (int i = 0; i < TASKS; ++i) {
-          const int r = (i >> 1) * PASS + tid / ROW_LANES, rin = rin0 + r;
-          const float v[8] = {x[i].x, x[i].y, x[i].z, x[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
-          const U4Lane out = u4_quantize_lanes<ROW_LANES>(v, rin & 1, lane);
-          if (r < rows) {
-            u4_store_codes(global + (i & 1) * TILE, HD, i & 1, rin, grp, q, out.word);
-            u4_store_meta(global, global + TILE, HD, i & 1, rin, grp, q, out);
-          }
+          const int r = (i >> 1) * PASS + tid / ROW_LANES;
+          if (r < rows) u4_store_codes(global + (i & 1) * TILE, HD, i & 1, rin0 + r, grp, q, word[i]);
         }
       }
     } else if (tid == 0) {

@@ -44,28 +44,6 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
-// two f32 operations in one instruction
-__device__ __forceinline__ uint64_t pair_of(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // (x, y) += (a, b)
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(x, y)), "l"(pair_of(a, b)));
-  unpair(r, x, y);
-}
-__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float c, float d) {   // (x, y) += (a, b) * (c, d)
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a, b)), "l"(pair_of(c, d)), "l"(pair_of(x, y)));
-  unpair(r, x, y);
-}
-__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x, y) *= (a, b)
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(x, y)), "l"(pair_of(a, b)));
-  unpair(r, x, y);
-}
 // 2^x; results below 2^-126 are zero
 __device__ __forceinline__ float exp2_ftz(float x) {
   float y;

@@ -21,6 +21,29 @@
 
 namespace sgk {
 
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // (x, y) += (a, b)
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(x, y)), "l"(pair_of(a, b)));
+  unpair(r, x, y);
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float c, float d) {   // (x, y) += (a, b) * (c, d)
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a, b)), "l"(pair_of(c, d)), "l"(pair_of(x, y)));
+  unpair(r, x, y);
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // (x, y) *= (a, b)
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(x, y)), "l"(pair_of(a, b)));
+  unpair(r, x, y);
+}
+
 constexpr int U4_EXP_MIN = -40;   // smallest step 2^-40
 
 // a - b = d + err exactly
@@ -80,28 +103,38 @@ __device__ __forceinline__ uint32_t u4_code_of(float y, float bias, float step, 
   }
   return static_cast<uint32_t>(code);
 }
-// The same for eight values sign * v of a group at once: codes of v[0..3] and v[4..7] as the bytes c[j] + 16 c[j + 4]. The
+// The same for eight values sign * v of a group at once: codes of v[0..3] and v[4..7] as the bytes c[j] + 16 c[j + 4]; inv15 ~
+// 1 / (15 step). The code is guessed, and right when t is less than half a step from it: t and the distance are rounded
+// once each, and a border between two codes is a number that f32 holds, so neither rounding carries a value across it. The
 // borders are looked at only when one of the eight lies on one.
-__device__ __forceinline__ uint32_t u4_codes8(const float (&v)[8], float sign, float bias, float step, float inv) {
-  // the rounded number sits in the low bits of guess: the eight are added up as integers, each at its place, and the
-  // upper bits (0x4b400000 each) are taken off as one constant
-  uint32_t word = 0;
+__device__ __forceinline__ uint32_t u4_codes8(const float (&v)[8], float sign, float bias, float step, float inv15) {
+  float t[8], n[8], d[8], byte[4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = -bias, n[j] = 12582912.0f;   // 1.5 * 2^23: rounds to a whole number
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    fma2(t[j], t[j + 1], v[j], v[j + 1], sign, sign);
+    fma2(n[j], n[j + 1], __saturatef(t[j] * inv15), __saturatef(t[j + 1] * inv15), 15.0f, 15.0f);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) byte[j] = n[j];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    add2(n[j], n[j + 1], -12582912.0f, -12582912.0f);
+    d[j] = t[j], d[j + 1] = t[j + 1];
+    fma2(d[j], d[j + 1], n[j], n[j + 1], -step, -step);
+  }
+  fma2(byte[0], byte[1], n[4], n[5], 16.0f, 16.0f);
+  fma2(byte[2], byte[3], n[6], n[7], 16.0f, 16.0f);
+  uint32_t word = __byte_perm(__byte_perm(__float_as_uint(byte[0]), __float_as_uint(byte[1]), 0x0040),
+                              __byte_perm(__float_as_uint(byte[2]), __float_as_uint(byte[3]), 0x0040), 0x5410);
   float far = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float t = fmaf(v[j], sign, -bias);
-    const float guess = fminf(fmaxf(t * inv, 0.0f), 15.0f) + 12582912.0f;
-    far = fmaxf(far, fabsf(fmaf(-(guess - 12582912.0f), step, t)));
-    word += __float_as_uint(guess) << (8 * (j & 3) + (j >> 2) * 4);
-  }
-  uint32_t upper = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) upper += 0x4b400000u << (8 * (j & 3) + (j >> 2) * 4);
-  word -= upper;
+  for (int j = 0; j < 8; ++j) far = fmaxf(far, fabsf(d[j]));
   if (far >= 0.5f * step) {
     word = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) word |= u4_code_of(sign * v[j], bias, step, inv) << (8 * (j & 3) + (j >> 2) * 4);
+    for (int j = 0; j < 8; ++j) word |= u4_code_of(sign * v[j], bias, step, 15.0f * inv15) << (8 * (j & 3) + (j >> 2) * 4);
   }
   return word;
 }
@@ -186,36 +219,86 @@ struct U4Lane {
   uint16_t step, bias;      // step positive, bias signed (bf16 bits)
   int exponent;             // of the row
 };
+__device__ __forceinline__ float min_nan(float a, float b) {   // NaN when either is
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void min_max8(const float (&v)[8], float& lo, float& hi) {   // NaN when one of the eight is
+  lo = hi = v[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) lo = min_nan(lo, v[j]), hi = max_nan(hi, v[j]);
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Range, step and row exponent of one group from its least and largest value; step NaN when the group is not finite.
 template <int ROW_LANES>
-__device__ __forceinline__ U4Lane u4_quantize_lanes(const float (&v)[8], uint32_t odd, int lane) {
-  const float sign = odd ? -1.0f : 1.0f;
-  float lo = v[0], hi = v[0], poison = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    lo = fminf(lo, v[j]);
-    hi = fmaxf(hi, v[j]);
-    poison = fmaf(v[j], 0.0f, poison);   // NaN once a value is not finite
-  }
-#pragma unroll
-  for (int off = 1; off < 4; off <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-  }
-  const uint32_t bad = __ballot_sync(0xffffffffu, poison != 0.0f) >> (lane & ~3) & 15u;
-  U4Range r = u4_range(odd ? -hi : lo, odd ? -lo : hi);
-  if (bad) r.finite = false, r.exponent = U4_EXP_MIN;
-  U4Lane out;
+__device__ __forceinline__ U4Range u4_group(float lo, float hi, uint32_t odd, U4Lane& out) {
+  const U4Range r = u4_range(odd ? -hi : lo, odd ? -lo : hi);
   out.exponent = r.exponent;
 #pragma unroll
   for (int off = 4; off < ROW_LANES; off <<= 1) out.exponent = max(out.exponent, __shfl_xor_sync(0xffffffffu, out.exponent, off));
   out.step = u4_step_bits(r, out.exponent);
+  out.bias = static_cast<uint16_t>(r.finite ? (__float_as_uint(odd ? -r.bias : r.bias) >> 16) : 0u);
+  return r;
+}
+template <int ROW_LANES>
+__device__ __forceinline__ U4Lane u4_quantize_lanes(const float (&v)[8], uint32_t odd, int lane) {
+  float lo, hi;
+  min_max8(v, lo, hi);
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+  }
+  U4Lane out;
+  const U4Range r = u4_group<ROW_LANES>(lo, hi, odd, out);
   const float s = bf16_bits_to_f32(out.step);
-  const uint32_t word = u4_codes8(v, sign, r.bias, s, __frcp_rn(s));
+  const uint32_t word = u4_codes8(v, odd ? -1.0f : 1.0f, r.bias, s, rcp_approx(s) * (1.0f / 15.0f));
   out.word = r.finite ? word : 0u;
-  out.bias = static_cast<uint16_t>(r.finite ? (__float_as_uint(sign * r.bias) >> 16) : 0u);
   return out;
 }
-// Stores what u4_quantize_lanes made of row `row`, group grp, lane q of four: the codes, then the rest.
+// The same for B (two or four) pieces a lane at once, of rows of the same parity: lane q works out the range and the step of
+// piece q % B of its group for all four lanes. word[i]: the codes of piece i; the rest belongs to piece q % B.
+template <int ROW_LANES, int B>
+__device__ __forceinline__ U4Lane u4_quantize_pieces(const float (&v)[B][8], uint32_t odd, int lane, uint32_t (&word)[B]) {
+  static_assert(B == 2 || B == 4, "pieces are shared among four lanes");
+  float lo[B], hi[B];
+#pragma unroll
+  for (int i = 0; i < B; ++i) min_max8(v[i], lo[i], hi[i]);
+  const bool b0 = lane & 1, b1 = lane & 2;
+  // each exchange halves the pieces a lane has partial minima of
+#pragma unroll
+  for (int i = 0; i < B; i += 2) {
+    const float lo_got = __shfl_xor_sync(0xffffffffu, b0 ? lo[i] : lo[i + 1], 1), hi_got = __shfl_xor_sync(0xffffffffu, b0 ? hi[i] : hi[i + 1], 1);
+    lo[i / 2] = min_nan(b0 ? lo[i + 1] : lo[i], lo_got);
+    hi[i / 2] = max_nan(b0 ? hi[i + 1] : hi[i], hi_got);
+  }
+  constexpr int LAST = B / 2 - 1;
+  const float lo_got = __shfl_xor_sync(0xffffffffu, b1 ? lo[0] : lo[LAST], 2), hi_got = __shfl_xor_sync(0xffffffffu, b1 ? hi[0] : hi[LAST], 2);
+  U4Lane out;
+  const U4Range r = u4_group<ROW_LANES>(min_nan(b1 ? lo[LAST] : lo[0], lo_got), max_nan(b1 ? hi[LAST] : hi[0], hi_got), odd, out);
+  const float s = bf16_bits_to_f32(out.step), inv15 = rcp_approx(s) * (1.0f / 15.0f);
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    const int from = (lane & ~3) | i;
+    const float bias_i = __shfl_sync(0xffffffffu, r.bias, from), s_i = __shfl_sync(0xffffffffu, s, from),
+                inv_i = __shfl_sync(0xffffffffu, inv15, from);
+    const uint32_t w = u4_codes8(v[i], odd ? -1.0f : 1.0f, bias_i, s_i, inv_i);
+    word[i] = s_i == s_i ? w : 0u;
+  }
+  out.word = 0;
+  return out;
+}
+// Stores what became of row `row`, group grp: the codes of lane q of four, and the rest, which one lane stores.
 __device__ __forceinline__ void u4_store_codes(uint8_t* tile, int hd, int is_v, int row, int grp, int q, uint32_t word) {
   const int dim = grp * QGROUP + 4 * q;
   if (is_v) {
@@ -225,8 +308,7 @@ __device__ __forceinline__ void u4_store_codes(uint8_t* tile, int hd, int is_v, 
     *reinterpret_cast<uint32_t*>(tile + u4_k_byte(row, dim, hd)) = word;
   }
 }
-__device__ __forceinline__ void u4_store_meta(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, int grp, int q, const U4Lane& x) {
-  if (q != 0) return;
+__device__ __forceinline__ void u4_store_meta(uint8_t* ktile, uint8_t* vtile, int hd, int is_v, int row, int grp, const U4Lane& x) {
   uint8_t* tile = is_v ? vtile : ktile;
   const uint32_t odd = row & 1;
   *reinterpret_cast<uint16_t*>(tile + u4_step_offset(is_v, row, grp, hd)) =
