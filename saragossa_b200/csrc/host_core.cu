@@ -629,7 +629,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     static const bool shared_merge_off = std::getenv("SGK_NO_SHARED_MERGE") != nullptr;
     if (!shared_merge_off && a.pages_per_split == 0 && a.splits > 12 && a.splits <= 160) {
       if (resident_per_sm < 0 || resident_stages != a.n_stages)   // asked once per batch
-        resident_per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim)
+        resident_per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim, q_heads / pool->kv_heads)
                           : kernel == 3 ? attention_u8_resident_blocks(pool->head_dim, a.n_stages)
                                       : attention_mma_resident_blocks(pool->head_dim, a.n_stages),
         resident_stages = a.n_stages;
@@ -660,7 +660,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
         cluster_stages = a.n_stages;
       }
       if (max_clusters[a.splits] < 0)
-        max_clusters[a.splits] = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, a.splits)
+        max_clusters[a.splits] = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, q_heads / pool->kv_heads, a.splits)
                                  : kernel == 3 ? attention_u8_max_clusters(pool->head_dim, a.n_stages, a.splits)
                                              : attention_mma_max_clusters(pool->head_dim, a.n_stages, a.splits);
       a.cluster_merge = int64_t(pool->kv_heads) * n() <= max_clusters[a.splits];

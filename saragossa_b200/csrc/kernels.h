@@ -137,8 +137,8 @@ bool attention_u4_supported(int dtype, int head_dim, int gqa);
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream);
 cudaError_t attention_u4_configure();
 int attention_u4_blocks_per_sm(int head_dim);
-int attention_u4_resident_blocks(int head_dim);
-int attention_u4_max_clusters(int head_dim, int splits);
+int attention_u4_resident_blocks(int head_dim, int gqa);
+int attention_u4_max_clusters(int head_dim, int gqa, int splits);
 
 // Gather rows [row0, row0+n) of one layer into contiguous [n, kv_dim] arrays.
 // mode 0: storage type (f32 / bf16 bits), 1: decoded f32, 2: u8 or u4 codes (a byte each) + scale + bias.

@@ -194,11 +194,13 @@ __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park
 
 // PP: pages a warp works on at once. Two (head_dim 128) give the chains of matrix instructions twice the
 // independent work and share the query's fragments and the bookkeeping; with head_dim 256 one page fills the registers.
-template <int HD, bool CLUSTER, bool PEERS>
+// PAIRED (up to four query heads per KV head): the matrix instruction has eight columns, so column h + 4 takes the lo parts
+// of head h's query and weights beside the hi parts in column h: half the products and half their chains.
+template <int HD, bool CLUSTER, bool PEERS, bool PAIRED>
 __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) attention_u4_kernel(AttnArgs a) {
   using S = U4Smem<HD, CLUSTER>;
   constexpr int G = S::G;
-    constexpr int PP = U4Shape<HD>::PAGES, WARPS = S::WARPS, THREADS = S::THREADS;
+  constexpr int PP = U4Shape<HD>::PAGES, WARPS = S::WARPS, THREADS = S::THREADS;
   constexpr int GS = G < 4 ? G : 4, SETS = G / GS;   // groups whose products are formed side by side
   // (not rounded up by hand: an address that went through an integer is a generic one to the compiler, and its loads too)
   extern __shared__ __align__(128) uint8_t u4_smem[];
@@ -327,7 +329,8 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
     }
     __syncthreads();
     for (int i = tid; i < G * 32; i += THREADS) {
-      const int grp = i >> 5, h = (i & 31) >> 2, t = i & 3;
+      const int grp = i >> 5, column = (i & 31) >> 2, t = i & 3;
+      const int h = PAIRED ? column & 3 : column;
       const float inv = 1.0f / qpow_s[h];
       const float* row = q_rows + h * HD + grp * QGROUP + 4 * t;
       const float4 x = *reinterpret_cast<const float4*>(row), y = *reinterpret_cast<const float4*>(row + 16);
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       float sum = (x.x + x.y) + (x.z + x.w) + ((y.x + y.y) + (y.z + y.w));
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) qsum_s[h * 8 + grp] = sum;
+      if (t == 0) qsum_s[column * 8 + grp] = PAIRED && column > 3 ? 0.0f : sum;
       // n0 x + n1 y = n0 (x - y / 16) + u (y / 16), with u in units of 2^-24 and n0 in units of 2^-14
       const float s = inv * 0.0625f, d = 0x1p-10f;
       const float u[4] = {y.x * s, y.y * s, y.z * s, y.w * s};
@@ -347,8 +350,12 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       const float2 u0 = unpack_f16(fu.x), u1 = unpack_f16(fu.y), r0 = unpack_f16(fr.x), r1 = unpack_f16(fr.y);
       fu.z = pack_f16(u[0] - u0.x, u[2] - u0.y), fu.w = pack_f16(u[1] - u1.x, u[3] - u1.y);
       fr.z = pack_f16(r[0] - r0.x, r[2] - r0.y), fr.w = pack_f16(r[1] - r1.x, r[3] - r1.y);
-      *reinterpret_cast<uint4*>(q_frag + ((grp * 2) * 32 + (i & 31)) * 16) = fu;
-      *reinterpret_cast<uint4*>(q_frag + ((grp * 2 + 1) * 32 + (i & 31)) * 16) = fr;
+      if (PAIRED) {
+        *reinterpret_cast<uint4*>(q_frag + i * 16) = column < 4 ? make_uint4(fu.x, fu.y, fr.x, fr.y) : make_uint4(fu.z, fu.w, fr.z, fr.w);
+      } else {
+        *reinterpret_cast<uint4*>(q_frag + ((grp * 2) * 32 + (i & 31)) * 16) = fu;
+        *reinterpret_cast<uint4*>(q_frag + ((grp * 2 + 1) * 32 + (i & 31)) * 16) = fr;
+      }
     }
     __syncthreads();   // fragments and sums written
     // The bias product's B fragment: group sums as three bf16 parts. With two groups the sixteen k-slots take
@@ -367,7 +374,10 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       else qs0 = hi, qs1 = mid, qs2 = lo;
     }
     const int g = lane >> 2, t = lane & 3;
-    const float ch0 = qpow_s[2 * t] * 16777216.0f, ch1 = qpow_s[2 * t + 1] * 16777216.0f;   // products are in units of 2^-24
+    const int h0 = PAIRED ? 2 * (t & 1) : 2 * t;   // this thread's heads: h0 and h0 + 1
+    const float ch0 = qpow_s[h0] * 16777216.0f, ch1 = qpow_s[h0 + 1] * 16777216.0f;   // products are in units of 2^-24
+    const float once = PAIRED && t > 1 ? 0.0f : 1.0f;             // what is added to a score once: in the hi column
+    const uint32_t low = PAIRED && g < 4 ? 0u : 0xffffffffu;      // PAIRED: column g takes lo parts
 
     // The row of a fused append is quantised now, by the warp with the fewest pages, while the first pages are
     // on their way; its bytes go to the page in global memory and stay parked in shared memory for the warp
@@ -510,14 +520,24 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
           }
 #pragma unroll
           for (int j = 0; j < GS; ++j) {
-            const uint4 fu = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2) * 32 + lane) * 16);
-            const uint4 fr = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2 + 1) * 32 + lane) * 16);
+            uint4 fu, fr;
+            if (PAIRED) {
+              fu = *reinterpret_cast<const uint4*>(q_frag + ((set * 4 + j) * 32 + lane) * 16);
+              fr = make_uint4(fu.z, fu.w, 0u, 0u);
+            } else {
+              fu = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2) * 32 + lane) * 16);
+              fr = *reinterpret_cast<const uint4*>(q_frag + (((set * 4 + j) * 2 + 1) * 32 + lane) * 16);
+            }
 #pragma unroll
             for (int u = 0; u < PP; ++u) {
               const U4Word<0x2c00> c0(w0[u][j]), c1(w1[u][j]);
-              mma_f16_zero(acc[u][j], c0.a_u, c1.a_u, c0.b_u, c1.b_u, fu.z, fu.w);   // the small parts first: the
-              mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.z, fr.w);   // accumulator is truncated after
-              mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.x, fr.y);   // every product
+              if (PAIRED) {
+                mma_f16_zero(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.x, fr.y);
+              } else {
+                mma_f16_zero(acc[u][j], c0.a_u, c1.a_u, c0.b_u, c1.b_u, fu.z, fu.w);   // the small parts first: the
+                mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.z, fr.w);   // accumulator is truncated after
+                mma_f16(acc[u][j], c0.a_n, c1.a_n, c0.b_n, c1.b_n, fr.x, fr.y);   // every product
+              }
               mma_f16(acc[u][j], c0.a_u, c1.a_u, c0.b_u, c1.b_u, fu.x, fu.y);
             }
           }
@@ -545,8 +565,8 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
           const uint32_t e1 = *reinterpret_cast<const uint16_t*>(tile[u] + S::TILE + S::POWERS + 2 * g);
           back[u][0] = __uint_as_float(0x7f000000u - (e0 << 16));
           back[u][1] = __uint_as_float(0x7f000000u - (e1 << 16));
-          const float x0 = __uint_as_float(0x4b000000u | (e0 >> 7)) - 8388735.0f;   // e = exponent field - 127
-          const float x1 = __uint_as_float(0x4b000000u | (e1 >> 7)) - 8388735.0f;
+          const float x0 = fmaf(__uint_as_float(0x4b000000u | (e0 >> 7)), once, -8388735.0f * once);   // e = exponent field - 127
+          const float x1 = fmaf(__uint_as_float(0x4b000000u | (e1 >> 7)), once, -8388735.0f * once);
           float sb[4] = {x0, x0, x1, x1};
           const uint32_t b0 = *reinterpret_cast<const uint32_t*>(tile[u] + kb_off);
           const uint32_t b1 = *reinterpret_cast<const uint32_t*>(tile[u] + kb_off + 16 * G);
@@ -554,6 +574,12 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
           if (G == 8) mma_bf16_k8(sb, b0, b1, qs2);
           fma2(sb[0], sb[1], z[u][0], z[u][1], ch0, ch1);
           fma2(sb[2], sb[3], z[u][2], z[u][3], ch0, ch1);
+          if (PAIRED) {   // hi and lo columns
+            const float other[4] = {__shfl_xor_sync(0xffffffffu, sb[0], 2), __shfl_xor_sync(0xffffffffu, sb[1], 2),
+                                    __shfl_xor_sync(0xffffffffu, sb[2], 2), __shfl_xor_sync(0xffffffffu, sb[3], 2)};
+            add2(sb[0], sb[1], other[0], other[1]);
+            add2(sb[2], sb[3], other[2], other[3]);
+          }
           z[u][0] = sb[0], z[u][1] = sb[1], z[u][2] = sb[2], z[u][3] = sb[3];
         }
         uint32_t vs0[PP][G], vs1[PP][G];           // V factors of the groups: rows (2t, 2t+1) and (2t+8, 2t+9)
@@ -651,9 +677,10 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const uint32_t s0 = vs0[u][pair * 2 + j], s1 = vs1[u][pair * 2 + j];
-              wh[u][j][0] = hmul2_u32(ph[u][0], s0), wh[u][j][1] = hmul2_u32(ph[u][1], s1);
-              wl[u][j][0] = hfma2_u32(pl[u][0], s0, hfms2_u32(ph[u][0], s0, wh[u][j][0]));
-              wl[u][j][1] = hfma2_u32(pl[u][1], s1, hfms2_u32(ph[u][1], s1, wh[u][j][1]));
+              // PAIRED: a hi column has zeros for what is subtracted and for the lo part, so wl is its hi product
+              wh[u][j][0] = hmul2_u32(ph[u][0] & low, s0), wh[u][j][1] = hmul2_u32(ph[u][1] & low, s1);
+              wl[u][j][0] = hfma2_u32(pl[u][0] & low, s0, hfms2_u32(ph[u][0], s0, wh[u][j][0]));
+              wl[u][j][1] = hfma2_u32(pl[u][1] & low, s1, hfms2_u32(ph[u][1], s1, wh[u][j][1]));
             }
           }
 #pragma unroll
@@ -667,10 +694,12 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
             add(cr[0], c00.a_n, c01.a_n, c00.b_n, c01.b_n, wl[u][0][0], wl[u][0][1]);
             add(cu[1], c10.a_u, c11.a_u, c10.b_u, c11.b_u, wl[u][1][0], wl[u][1][1]);
             add(cr[1], c10.a_n, c11.a_n, c10.b_n, c11.b_n, wl[u][1][0], wl[u][1][1]);
-            mma_f16(cu[0], c00.a_u, c01.a_u, c00.b_u, c01.b_u, wh[u][0][0], wh[u][0][1]);
-            mma_f16(cr[0], c00.a_n, c01.a_n, c00.b_n, c01.b_n, wh[u][0][0], wh[u][0][1]);
-            mma_f16(cu[1], c10.a_u, c11.a_u, c10.b_u, c11.b_u, wh[u][1][0], wh[u][1][1]);
-            mma_f16(cr[1], c10.a_n, c11.a_n, c10.b_n, c11.b_n, wh[u][1][0], wh[u][1][1]);
+            if (!PAIRED) {
+              mma_f16(cu[0], c00.a_u, c01.a_u, c00.b_u, c01.b_u, wh[u][0][0], wh[u][0][1]);
+              mma_f16(cr[0], c00.a_n, c01.a_n, c00.b_n, c01.b_n, wh[u][0][0], wh[u][0][1]);
+              mma_f16(cu[1], c10.a_u, c11.a_u, c10.b_u, c11.b_u, wh[u][1][0], wh[u][1][1]);
+              mma_f16(cr[1], c10.a_n, c11.a_n, c10.b_n, c11.b_n, wh[u][1][0], wh[u][1][1]);
+            }
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
@@ -713,11 +742,20 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
         o_b[1][grp] += __shfl_xor_sync(0xffffffffu, o_b[1][grp], off);
       }
     }
+    if (PAIRED) {
+#pragma unroll
+      for (int grp = 0; grp < G; ++grp)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          o_hi[grp][c] += __shfl_xor_sync(0xffffffffu, o_hi[grp][c], 2);
+          o_lo[grp][c] += __shfl_xor_sync(0xffffffffu, o_lo[grp][c], 2);
+        }
+    }
     float* ow = o_s + warp * 8 * S::OPAD;
 #pragma unroll
     for (int grp = 0; grp < G; ++grp)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {   // (dim g + 8 * (c / 2); head 2t + c % 2)
+      for (int c = 0; c < 4; ++c) {   // (dim g + 8 * (c / 2); head 2t + c % 2; PAIRED: rows 4 to 7 repeat rows 0 to 3, unread)
         float* to = ow + (2 * t + (c & 1)) * S::OPAD + grp * QGROUP + g + 8 * (c >> 1);
         to[0] = o_lo[grp][c] + o_b[c & 1][grp];
         to[16] = fmaf(fmaf(o_hi[grp][c], 16777216.0f, -o_lo[grp][c]), 0.0625f, o_b[c & 1][grp]);
@@ -739,32 +777,34 @@ bool attention_u4_supported(int dtype, int head_dim, int gqa) {
   return dtype == KV_U4G32 && (head_dim == 64 || head_dim == 128 || head_dim == 256) && gqa >= 1 && gqa <= 8;
 }
 
-// The instances of one head size, and what they need.
+// The instances of one head size and group of query heads, and what they need.
 struct U4Instance {
   const void* kernels[3];   // plain, cluster, peers
   int blocks_per_sm, threads, smem, cluster_smem;
 };
-template <int HD>
+template <int HD, bool PAIRED>
 static U4Instance u4_instance() {
-  return {{reinterpret_cast<const void*>(attention_u4_kernel<HD, false, false>), reinterpret_cast<const void*>(attention_u4_kernel<HD, true, false>),
-           reinterpret_cast<const void*>(attention_u4_kernel<HD, false, true>)},
+  return {{reinterpret_cast<const void*>(attention_u4_kernel<HD, false, false, PAIRED>),
+           reinterpret_cast<const void*>(attention_u4_kernel<HD, true, false, PAIRED>),
+           reinterpret_cast<const void*>(attention_u4_kernel<HD, false, true, PAIRED>)},
           U4Shape<HD>::BLOCKS, U4Shape<HD>::WARPS * 32, U4Smem<HD, false>::TOTAL, U4Smem<HD, true>::TOTAL};
 }
-static U4Instance u4_instance(int head_dim) {
-  return head_dim == 64 ? u4_instance<64>() : head_dim == 128 ? u4_instance<128>() : u4_instance<256>();
+static U4Instance u4_instance(int head_dim, int gqa) {
+  if (gqa <= 4) return head_dim == 64 ? u4_instance<64, true>() : head_dim == 128 ? u4_instance<128, true>() : u4_instance<256, true>();
+  return head_dim == 64 ? u4_instance<64, false>() : head_dim == 128 ? u4_instance<128, false>() : u4_instance<256, false>();
 }
 
-int attention_u4_blocks_per_sm(int head_dim) { return u4_instance(head_dim).blocks_per_sm; }
+int attention_u4_blocks_per_sm(int head_dim) { return u4_instance(head_dim, 8).blocks_per_sm; }
 
-int attention_u4_resident_blocks(int head_dim) {
-  const U4Instance x = u4_instance(head_dim);
+int attention_u4_resident_blocks(int head_dim, int gqa) {
+  const U4Instance x = u4_instance(head_dim, gqa);
   int blocks = 0;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, x.kernels[0], x.threads, x.smem) == cudaSuccess ? blocks : 0;
 }
 
 // How many clusters of `splits` blocks the device can hold at once (0: such a launch would fail).
-int attention_u4_max_clusters(int head_dim, int splits) {
-  const U4Instance x = u4_instance(head_dim);
+int attention_u4_max_clusters(int head_dim, int gqa, int splits) {
+  const U4Instance x = u4_instance(head_dim, gqa);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, 1, 1);
   cfg.blockDim = dim3(x.threads);
@@ -785,8 +825,8 @@ int attention_u4_max_clusters(int head_dim, int splits) {
 }
 
 cudaError_t attention_u4_configure() {
-  for (int hd : {64, 128, 256}) {
-    const U4Instance x = u4_instance(hd);
+  for (int i = 0; i < 6; ++i) {
+    const U4Instance x = u4_instance(64 << i / 2, i % 2 ? 8 : 4);
     for (int kind = 0; kind < 3; ++kind) {
       cudaError_t e = cudaFuncSetAttribute(x.kernels[kind], cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
       // clusters of more than 8 blocks (up to 16 splits merge as one cluster) are an opt-in
@@ -798,7 +838,7 @@ cudaError_t attention_u4_configure() {
 }
 
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream) {
-  const U4Instance x = u4_instance(a.pool.head_dim);
+  const U4Instance x = u4_instance(a.pool.head_dim, a.q_heads / a.pool.kv_heads);
   const bool peers = a.n_peers > 0, cluster = a.cluster_merge && !peers;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.splits, a.pool.kv_heads, n_seq);
