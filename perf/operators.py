@@ -252,19 +252,22 @@ class _Cache:
 
 def _own_run(state):
     case, cache = state["case"], state["cache"]
+    # the stream that torch works on, where the results are read; its default stream has the handle 0, which the package
+    # takes for its own stream, so that one goes by its other name (cudaStreamLegacy)
+    stream = torch.cuda.current_stream().cuda_stream or 1
     if case["op"] == "write":
         kv = cache.kvs[0]
-        kv.encode_truncate(case["offset"])
-        kv.encode_append_rows(state["k"], state["v"], case["rows"])
-        kv.encode_gather_rows_f32(state["k_out"], state["v_out"], case["offset"], case["rows"])
+        kv.encode_truncate(case["offset"], stream=stream)
+        kv.encode_append_rows(state["k"], state["v"], case["rows"], stream=stream)
+        kv.encode_gather_rows_f32(state["k_out"], state["v_out"], case["offset"], case["rows"], stream=stream)
         return {"k": state["k_out"].tensor, "v": state["v_out"].tensor}
     if not case.get("append"):
-        cache.batch.enqueue_attention(state["q"], state["out"], case.get("window", 0))
+        cache.batch.enqueue_attention(state["q"], state["out"], case.get("window", 0), stream=stream)
         return {"out": state["out"].tensor}
-    cache.batch.enqueue_truncate([n - 1 for n in cache.lens])
-    cache.batch.enqueue_step(state["new_k"], state["new_v"], state["q"], state["out"])
+    cache.batch.enqueue_truncate([n - 1 for n in cache.lens], stream=stream)
+    cache.batch.enqueue_step(state["new_k"], state["new_v"], state["q"], state["out"], stream=stream)
     for kv, n, (k, v) in zip(cache.kvs, cache.lens, state["rows_out"]):
-        kv.encode_gather_rows_f32(k, v, n - 1, 1)
+        kv.encode_gather_rows_f32(k, v, n - 1, 1, stream=stream)
     return {"out": state["out"].tensor, "new_k": state["k_out"], "new_v": state["v_out"]}
 
 
