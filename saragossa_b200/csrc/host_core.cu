@@ -311,11 +311,8 @@ int create_batch(State* st, Kv** kvs, int n, Batch** out) {
     slots.push_back(kvs[i]->seq->slot);
   }
   const int heads = std::max(b->q_heads, b->pool->kv_heads);
-  // Splits never need to exceed the blocks that are resident at once.
-  const int blocks_per_sm = attention_u4_supported(b->pool->dtype, b->pool->head_dim, b->q_heads / b->pool->kv_heads)
-                                ? attention_u4_blocks_per_sm(b->pool->head_dim)
-                                : 2;
-  int by_sm = (blocks_per_sm * st->sm_count) / (n * b->pool->kv_heads);
+  // Splits never need to exceed about two blocks per SM for the whole launch.
+  int by_sm = (2 * st->sm_count) / (n * b->pool->kv_heads);
   b->uniform_splits = std::min(144, std::max(1, by_sm));  // two merge levels of at most 12 partials each
   // an uneven batch cuts its long sequences finer than that (the workspace is sized for it)
   b->max_splits = n > 1 ? std::max(b->uniform_splits, 16) : b->uniform_splits;
@@ -364,7 +361,9 @@ int Batch::choose_splits(int kernel, int64_t max_rows) const {
     // with the best whole-wave fill (first one above 98.5%), while every split
     // keeps a few pages of work.
     const int heads = kernel >= 2 ? pool->kv_heads : q_heads;
-    const int64_t slots = int64_t(st->sm_count) * (kernel == 4 ? attention_u4_blocks_per_sm(pool->head_dim) : kernel >= 2 ? 2 : 8);
+    // (Over u4 pages two blocks per SM are as fast as the three or four that fit, with fewer partials to merge: one
+    // sequence of 32768 rows, 4 heads of 128, 16.4 us against 18.4; eight of them 51.5 against 53.3.)
+    const int64_t slots = int64_t(st->sm_count) * (kernel >= 2 ? 2 : 8);
     const int64_t units = int64_t(heads) * n();
     const int64_t pages = (max_rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
     const int min_pages = kernel >= 2 ? 8 : 2;
@@ -382,6 +381,9 @@ int Batch::choose_splits(int kernel, int64_t max_rows) const {
       }
       if (eff >= 0.985) break;
     }
+    // Nine to twelve splits over u4 pages neither merge as a cluster (up to 8) nor all together (from 13 on), and are no
+    // faster than eight that do: 8 sequences, 4 heads of 128, 2048 rows 12.3 us against 10.3, 8192 rows 21.6 against 18.8.
+    if (kernel == 4 && best > 8 && best <= 12) best = 8;
     s = best;
   }
   return std::max(1, std::min(s, max_splits));
@@ -572,13 +574,15 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
         // Over u4 pages the multiplications are the bound, not the stream, and what a block spends on its start and its
         // merge counts for more: pieces just large enough for one wave (24 sequences of 200 to 20000 rows, 8 heads of 128:
         // 45.9 us with three waves, 43.4 with two, 38.4 with one).
+        // A sequence of at most half a piece counts half: two such blocks share a place one after the other (40.9 us against
+        // 44.6 where each counts as a block).
         pps = std::max<int64_t>(1, total * pool->kv_heads / slots);
-        const auto blocks = [&] {
+        const auto half_blocks = [&] {
           int64_t sum = 0;
-          for (int64_t p : pages_of) sum += (p + pps - 1) / pps;
+          for (int64_t p : pages_of) sum += 2 * p <= pps ? 1 : 2 * ((p + pps - 1) / pps);
           return sum * pool->kv_heads;
         };
-        while (blocks() > slots) pps += (pps + 15) / 16;
+        while (half_blocks() > 2 * slots) pps += (pps + 15) / 16;
       }
       pps = std::max<int64_t>(pps, 8);
       const int64_t need = (hi + pps - 1) / pps + 1;   // one spare: lengths grow while a graph is replayed
@@ -652,9 +656,10 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     // Up to 16 splits run as one thread-block cluster and merge through distributed shared memory:
     // no partial goes through L2 and no device-wide atomic sits between the last page and the output.
     // Only when every cluster of the launch is resident at once: a launch that would fit one wave of
-    // blocks must not get a second one from the placement of clusters.
+    // blocks must not get a second one from the placement of clusters. Over u4 pages up to 8: larger clusters fill some SMs
+    // with three blocks and leave others one (8 sequences of 32768 rows, 4 heads of 128, 9 splits: 64.6 us, without 51.2).
     static const bool cluster_merge_off = std::getenv("SGK_NO_CLUSTER_MERGE") != nullptr;
-    if (!cluster_merge_off && a.pages_per_split == 0 && a.splits >= 2 && a.splits <= 16) {
+    if (!cluster_merge_off && a.pages_per_split == 0 && a.splits >= 2 && a.splits <= (kernel == 4 ? 8 : 16)) {
       if (cluster_stages != a.n_stages) {
         for (int& c : max_clusters) c = -1;
         cluster_stages = a.n_stages;

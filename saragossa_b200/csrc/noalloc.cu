@@ -139,7 +139,7 @@ extern "C" int32_t sgk_kv_enqueue_attention_noalloc(sgk_kv* kv, void* stream, co
   // generic one), keep a few pages per split, and stay inside the static workspace
   const int64_t pages = (len - window_start + PAGE_TOKENS - 1) / PAGE_TOKENS + sinks.pages;
   const int64_t units = mma ? kvh : qh;
-  const int64_t slots = int64_t(st->sm_count) * (u4 ? attention_u4_blocks_per_sm(hd) : mma ? 2 : 8);
+  const int64_t slots = int64_t(st->sm_count) * (mma ? 2 : 8);
   int64_t splits = std::max<int64_t>(1, slots / units);
   splits = std::min<int64_t>(splits, std::max<int64_t>(1, pages / (mma ? 8 : 2)));
   splits = std::min<int64_t>(splits, 144);
