@@ -573,7 +573,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       if (kernel == 4 && int64_t(n()) * pool->kv_heads * 2 <= slots) {
         // Over u4 pages the multiplications are the bound, not the stream, and what a block spends on its start and its
         // merge counts for more: pieces just large enough for one wave (24 sequences of 200 to 20000 rows, 8 heads of 128:
-        // 45.9 us with three waves, 43.4 with two, 38.4 with one).
+        // pieces of 149 pages 41.0 us, of 100 to 130, which need a second wave, 48.7 to 50.5, of 185 47.1).
         // A sequence of at most half a piece counts half: two such blocks share a place one after the other (40.9 us against
         // 44.6 where each counts as a block).
         pps = std::max<int64_t>(1, total * pool->kv_heads / slots);

@@ -22,11 +22,11 @@
 // all count up from a minimum, hundreds of times larger than the result under flat attention, and f32
 // would lose those digits.
 //
-// B200, f32 queries, 32 query heads over 4 KV heads of 128: 8 sequences of 32768 rows 44.7 us = 3.76 TB/s of page bytes (57 %
-// of the copy rate; DRAM reads 1.013 of the page bytes), one sequence 12.0 us; 24 uneven sequences of 200 to 20000 rows, 32
-// over 8 heads, 34.4 us = 4.1 TB/s; 64 windows of 2000 rows, 16 over 2 heads of 256, 23.7 us = 3.6 TB/s. A copy of the kernel that
-// only fetches takes 24 to 29 us for the first, one that only computes 38: what bounds it is the warps' instruction stream
-// (355 instructions per page and KV head, 0.47 issued per scheduler and cycle, tensor pipe 33 %, ALU 31 %), not memory.
+// B200, one call after another on one stream, f32 queries, 32 query heads over 4 KV heads of 128: 8 sequences of 32768 rows
+// 51.5 us = 3.3 TB/s of page bytes (50 % of the copy rate; DRAM reads 1.013 of the page bytes), one sequence 16.4 us; 24 uneven
+// sequences of 200 to 20000 rows, 32 over 8 heads, 41.0 us = 3.4 TB/s; 64 windows of 2000 rows, 16 over 2 heads of 256, 30.8 us =
+// 2.8 TB/s. Not memory bounds it but the warps' instruction stream (364 instructions per page and KV head with start and
+// merge, 0.46 issued per scheduler and cycle, tensor pipe 34 %, ALU 29 %) and, below about 10 MB, start and merge.
 //
 // The reference's KV has no 4-bit form; this kernel computes cached_attention_one
 // (src/decoder/attention_ops.rs:889-974) over the rows' values code * scale + bias.

@@ -277,8 +277,8 @@ __device__ __forceinline__ void peers_finish(const AttnArgs& a, int tid, int* fl
 // two merge levels done by single blocks. Returns false when the wait ran out.
 constexpr int SHARED_MERGE_MAX_SPLITS = 160;   // five partials per lane
 // WIDE (up to 32 splits): a warp takes 32 neighbouring cells, a lane per cell, and walks the partials with coalesced loads
-// and no shuffles, in a different order of additions than the lane-per-partial form. With the query's sums taken where its
-// fragments are made, one step of 16/2 heads of 256 over 4-bit pages went from 18.3 to 17.0 us, 1 x 32768 rows from 12.6 to 12.0.
+// and no shuffles, in a different order of additions than the lane-per-partial form. Together with
+// taking the query's sums where its fragments are made it took 4 to 7 % off the calls of one or two sequences over 4-bit pages.
 template <int HD, int NT, bool PEERS = false, bool WIDE = false>
 __device__ __forceinline__ bool shared_merge(const AttnArgs& a, int splits, int split, int gqa, int64_t qh0,
                                              int32_t* arrive_counter, int32_t* depart_counter, int* flags, int tid) {
