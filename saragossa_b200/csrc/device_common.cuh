@@ -26,6 +26,12 @@ __device__ __forceinline__ float bf16_bits_to_f32(uint16_t b) {
   return __uint_as_float(static_cast<uint32_t>(b) << 16);
 }
 
+// f32 bits of a u8 group's scale for the pool's largest one: an infinite scale (a group whose values read back as no numbers)
+// counts as none, or every other row of the pool would lose its weights to it from then on.
+__device__ __forceinline__ uint32_t u8_scale_for_max(uint32_t scale_bits) {
+  return scale_bits < 0x7f80u ? scale_bits << 16 : 0u;
+}
+
 // Signed step of (row, group) of a u4 tile as f32. V steps are stored divided by their row's power of two.
 __device__ __forceinline__ float u4_step(const uint8_t* tile, int hd, int is_v, int row, int grp) {
   const uint16_t bits = *reinterpret_cast<const uint16_t*>(tile + u4_step_offset(is_v, row, grp, hd));

@@ -97,7 +97,7 @@ __device__ void store_head_row(uint8_t* tile, int dtype, int hd, int is_v, int r
         *reinterpret_cast<uint16_t*>(tile + u8_scale_offset(row, g, hd)) = static_cast<uint16_t>(meta & 0xffffu);
         *reinterpret_cast<uint16_t*>(tile + u8_bias_offset(is_v, row, g, hd)) = static_cast<uint16_t>(meta >> 16);
         // largest scale of the pool (positive floats order like their bit patterns)
-        const uint32_t scale_f32_bits = (meta & 0xffffu) << 16;
+        const uint32_t scale_f32_bits = u8_scale_for_max(meta & 0xffffu);
         if (scale_max != nullptr && scale_f32_bits > *reinterpret_cast<volatile uint32_t*>(scale_max))
           atomicMax(scale_max, scale_f32_bits);
       }
@@ -212,7 +212,7 @@ __device__ __forceinline__ uint32_t store_u8_row(uint8_t* tile, int hd, int is_v
   for (int g = 0; g < G; ++g) {
     const int dim = g * QGROUP + lane;
     tile[is_v ? u8_v_code_index(rin, dim, hd) : u8_k_code_index(rin, dim, hd)] = static_cast<uint8_t>(code[g]);
-    biggest = max(biggest, (meta[g] & 0xffffu) << 16);
+    biggest = max(biggest, u8_scale_for_max(meta[g] & 0xffffu));
     if (lane == g) {
       *reinterpret_cast<uint16_t*>(tile + u8_scale_offset(rin, g, hd)) = static_cast<uint16_t>(meta[g] & 0xffffu);
       *reinterpret_cast<uint16_t*>(tile + u8_bias_offset(is_v, rin, g, hd)) = static_cast<uint16_t>(meta[g] >> 16);

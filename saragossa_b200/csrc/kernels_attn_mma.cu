@@ -59,6 +59,19 @@ struct MmaSmem {
   static size_t total(int stages) { return ring_bytes(stages) + FIXED + 1024; }
 };
 
+// A row that is not seen weighs nothing, whatever its bytes say: the staged V rows before `first` and from `last` on become
+// zeros (a weight of zero times a NaN left there is a NaN). One warp, for the page in which a window starts and the last
+// page. Not inlined: the page loop keeps its registers.
+template <int HD>
+__device__ __noinline__ void blank_v_rows(uint8_t* vtile, int first, int last, int lane) {
+  for (int i = lane; i < PAGE_TOKENS * (HD / 8); i += 32) {
+    const int r = i / (HD / 8);
+    if (r < first || r >= last) *reinterpret_cast<uint4*>(vtile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the copy that refills the stage
+  __syncwarp();
+}
+
 // SINKS: the instance for a window beside which the first rows stay visible. A separate one: the walk over
 // two ranges of pages and the masking of rows between them cost the others nothing.
 template <int HD, bool CLUSTER, bool PEERS, bool SINKS = false>
@@ -252,6 +265,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
       uint8_t* vtile = ktile + S::TILE;
       const int64_t page_index = map.page(pb + i);
       const int64_t row_base = page_index * PAGE_TOKENS;
+      // rows [first_row, last_row) of the page lie in the window and before the cursor
+      const int first_row = static_cast<int>(ws - row_base), last_row = static_cast<int>(len - row_base);
 
       if (ok && owns_append && page_index == append_page_index) {
         // The new row (converted in the prologue, already on its way to the page) joins the staged copy.
@@ -263,6 +278,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
         }
         __syncwarp();
       }
+      if (!SINKS && ok && (first_row > 0 || last_row < PAGE_TOKENS)) blank_v_rows<HD>(vtile, first_row, last_row, lane);
 
       if (ok) {
         // The tensor-core instructions have a long latency, so the page is processed as
@@ -334,10 +350,9 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
 #pragma unroll
             for (int u = 0; u < CH; ++u) va[u][0] &= keep_a, va[u][1] &= keep_a, va[u][2] &= keep_b, va[u][3] &= keep_b;
           }
-        } else if (row_base < ws || row_base + PAGE_TOKENS > len) {
-          int64_t ra = row_base + g, rb = row_base + g + 8;
-          if (ra < ws || ra >= len) s[0] = s[1] = -1.0e30f;
-          if (rb < ws || rb >= len) s[2] = s[3] = -1.0e30f;
+        } else if (first_row > 0 || last_row < PAGE_TOKENS) {
+          if (g < first_row || g >= last_row) s[0] = s[1] = -1.0e30f;
+          if (g + 8 < first_row || g + 8 >= last_row) s[2] = s[3] = -1.0e30f;
         }
         float mx0 = fmaxf(s[0], s[2]), mx1 = fmaxf(s[1], s[3]);
 #pragma unroll

@@ -68,7 +68,7 @@ struct PoolView {
   int64_t tile_bytes;
   const int32_t* tables;  // [max_seqs][table_stride] page ids
   int32_t* lens;          // [max_seqs][layers] rows held, per layer
-  uint32_t* scale_max;    // u8 pools: f32 bits of the largest group scale ever stored (else NULL)
+  uint32_t* scale_max;    // u8 pools: f32 bits of the largest finite group scale ever stored (else NULL)
   int32_t table_stride;
   int32_t layers;
   int32_t kv_heads;
