@@ -59,7 +59,10 @@ enum { SGK_KV_F32 = 0, SGK_KV_BF16 = 1, SGK_KV_U8G32 = 2, SGK_KV_U4G32 = 3 };
  * value = code * scale + bias is what the row reads back as: the affine formula of the u8 format, the scales
  * of odd rows negative (sums of weighted values then lose no digits to a common offset). A group that
  * holds an infinity or a NaN, or whose range overflows, reads back as NaN. Attention takes V values up to 1e18 beside
- * ones of any smaller size (beyond that the weights of rows 2^100 apart no longer fit one f32 sum). head_dim: a multiple of 32. A row of a head
+ * ones of any smaller size, in other rows or in other groups of the same row (beyond that the weights of rows 2^100 apart no
+ * longer fit one f32 sum). Weights are off by about 1e-6, by up to 1e-5 for rows whose V values are some 2^32 away from 1 (the
+ * row's power of two joins its score), and by up to 2^(k-28) (k <= 16) for the codes of a group whose step is 2^-k of the widest of its row.
+ * head_dim: a multiple of 32. A row of a head
  * takes head_dim * 10 / 16 + 1 bytes for K and as many for V. The tensor-core attention kernel takes
  * head_dim 64, 128 and 256 with up to 8 query heads per KV head; other shapes go to the generic kernel. */
 

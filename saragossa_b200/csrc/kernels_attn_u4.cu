@@ -14,8 +14,14 @@
 //   softmax  a V row's steps are stored as f * 2^e with fp16 f (layout.h); 2^e joins the score, so the weight
 //            p'' = exp2(z - M) is bounded whatever the row's range, and w = p'' f needs no scaling. p = p'' 2^-e
 //            feeds the sum of the weights and the bias part of V. M is a reference, not the maximum: it moves only
-//            when a z exceeds it by more than 14 (then to 6 below the largest z), so a page costs one vote
+//            when a z exceeds it by more than 14.9 (then to 9 or 10 below the largest z), so a page costs one vote
 //            instead of the shuffles of a maximum, and p'' stays inside fp16.
+//   classes  That holds while the 2^e of the rows lie within a factor of 16. One row of a wide range would raise M for all: the
+//            others' weights would leave fp16 at its lower end, in the groups too where that row says nothing. So M belongs
+//            to a class of rows: the vote also asks for rows with a 2^e below the class, and an iteration that meets rows of
+//            another class goes through its pages once per class, M moving with the class by the exact power of two. A
+//            row's weights are then off by 2^-28 of 2^e and of the largest weight at most: the codes of a group whose
+//            step is 2^-k of the widest of its row by 2^(k-28) of their share (k <= 16), everything else by less than the scores.
 //   outputs  O[d][h] = sum_row code w with w as fp16 hi + lo (22 bits; one part of 11 bits would leave 1e-4 of the result).
 //
 // Rows of odd position are stored negated (u4_quant.cuh): without it O would be a sum of codes that
@@ -126,8 +132,10 @@ template <>
 struct U4Shape<128> : U4ShapeOf<4, 3, 2, 6, 4> {};
 template <>
 struct U4Shape<256> : U4ShapeOf<4, 2, 1, 4, 4> {};
-constexpr float U4_LIMIT = 14.0f;   // p'' <= 2^14
-constexpr float U4_LEVEL = 6.0f;    // p'' of the largest z when the reference moves
+constexpr float U4_LIMIT = 14.9f;   // p'' <= 2^14.9, and p'' f below the largest fp16 number
+constexpr float U4_LEVEL = 9.0f;    // p'' of the largest z when the reference moves
+constexpr float U4_SPREAD = 16.0f;  // a class of rows: powers of two down to 1 / 16 of its largest
+constexpr float U4_REACH = 0x1p90f; // how far below the widest class yet a reference follows: outputs scaled up by it still fit f32
 
 // CLUSTER: the instance whose splits merge through distributed shared memory needs room to receive; the other gives that
 // room to the ring.
@@ -200,8 +208,11 @@ __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park
 // independent work and share the query's fragments and the bookkeeping; with head_dim 256 one page fills the registers.
 // PAIRED (up to four query heads per KV head): the matrix instruction has eight columns, so column h + 4 takes the lo parts
 // of head h's query and weights beside the hi parts in column h: half the products and half their chains.
+// (Even batches place two blocks per SM: the cluster instance, which only they use, is compiled for no more than that. At three
+// it spilled, and 8 sequences of 32768 rows, 32/4 heads of 128, took 55.3 us instead of 53.2.)
 template <int HD, bool CLUSTER, bool PEERS, bool PAIRED>
-__global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) attention_u4_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD>::BLOCKS == 3 ? 2 : U4Shape<HD>::BLOCKS)
+    attention_u4_kernel(AttnArgs a) {
   using S = U4Smem<HD, CLUSTER>;
   constexpr int G = S::G;
   constexpr int PP = U4Shape<HD>::PAGES, WARPS = S::WARPS, THREADS = S::THREADS;
@@ -437,6 +448,9 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
       o_b[0][grp] = o_b[1][grp] = 0.0f;
     }
     float m0 = -1.0e30f, m1 = -1.0e30f, l0 = 0.0f, l1 = 0.0f;
+    // The references are for rows with 2^-e <= back_limit (0: for none yet). While an iteration's rows are worked on class by class
+    // back_limit is negative, and rows with 2^-e <= taken are done.
+    float back_limit = 0.0f, taken = 0.0f, widest = INFINITY;   // widest: the least back_limit so far
     const int k_off = g * (HD / 2) + t * (HD == 64 ? 4 : 16);                 // + (set ^ odd row) * 64; row g + 8: + 4 * HD
     const int kb_off = S::BIASES + g * G * 2 + (G == 2 ? 0 : G == 4 ? (t & 1) : t) * 4;    // K biases of row g
     const int vs_off = S::TILE + S::STEPS + t * G * 4;                        // V factors of rows 2t, 2t+1; rows + 8: + 16 * G
@@ -463,7 +477,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
     int batch = 0;           // first page of the entries held
     for (int n = 0; n < count; n += PP) {
       const uint8_t* tile[PP];
-      bool ok = true;
+      bool ok = true, again = false;
       // (a missing second page stands in for itself by the first one)
 #pragma unroll
       for (int u = 0; u < PP; ++u) tile[u] = my_ring + (at + (u > 0 && n + u >= count ? 0 : u)) * S::STAGE;
@@ -616,16 +630,48 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
             for (int i = 0; i < G / 2; ++i) vb0[u][i] = s0 ? vb0[u][i] : 0u, vb1[u][i] = s1 ? vb1[u][i] : 0u;
           }
         }
-        float mx0 = fmaxf(z[0][0], z[0][2]), mx1 = fmaxf(z[0][1], z[0][3]);
-        if (PP == 2) mx0 = fmaxf(mx0, fmaxf(z[PP - 1][0], z[PP - 1][2])), mx1 = fmaxf(mx1, fmaxf(z[PP - 1][1], z[PP - 1][3]));
-        over = mx0 > m0 + U4_LIMIT || mx1 > m1 + U4_LIMIT;
+        float mx0 = fmaxf(z[0][0], z[0][2]), mx1 = fmaxf(z[0][1], z[0][3]), most_back = fmaxf(back[0][0], back[0][1]);
+        if (PP == 2) {
+          mx0 = fmaxf(mx0, fmaxf(z[PP - 1][0], z[PP - 1][2])), mx1 = fmaxf(mx1, fmaxf(z[PP - 1][1], z[PP - 1][3]));
+          most_back = fmaxf(most_back, fmaxf(back[PP - 1][0], back[PP - 1][1]));
+        }
+        over = mx0 > m0 + U4_LIMIT || mx1 > m1 + U4_LIMIT || most_back > back_limit;
         if (__any_sync(0xffffffffu, over)) {
+          // The class of this pass: the rows left with the largest powers of two, down to 1 / U4_SPREAD of the largest.
+          float least = INFINITY;
+#pragma unroll
+          for (int u = 0; u < PP; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (back[u][r] > taken) least = fminf(least, back[u][r]);
+          asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(least) : "f"(least));
+          const float limit = least * U4_SPREAD;
+          bool left = false;
+#pragma unroll
+          for (int u = 0; u < PP; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              left = left || back[u][r] > limit;
+              if (back[u][r] > limit || back[u][r] <= taken) z[u][2 * r] = z[u][2 * r + 1] = -INFINITY, back[u][r] = 0.0f;
+            }
+          again = __any_sync(0xffffffffu, left);
+          // Its references: the ones there are, moved by the distance of the classes in powers of two, so that a row's p'' goes by
+          // its share in the sum of the weights, whatever class it is of; raised below where a score asks for it.
+          const float ref = fminf(limit, widest * U4_REACH);
+          widest = fminf(widest, limit);
+          const float shift = static_cast<float>((__float_as_int(fabsf(back_limit)) - __float_as_int(ref)) >> 23);
+          taken = again ? limit : 0.0f;
+          back_limit = again ? -ref : ref;
+          mx0 = fmaxf(z[0][0], z[0][2]), mx1 = fmaxf(z[0][1], z[0][3]);
+          if (PP == 2) mx0 = fmaxf(mx0, fmaxf(z[PP - 1][0], z[PP - 1][2])), mx1 = fmaxf(mx1, fmaxf(z[PP - 1][1], z[PP - 1][3]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) {
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
           }
-          const float mn0 = mx0 > m0 + U4_LIMIT ? mx0 - U4_LEVEL : m0, mn1 = mx1 > m1 + U4_LIMIT ? mx1 - U4_LEVEL : m1;
+          float mn0 = m0 + shift, mn1 = m1 + shift;
+          if (mx0 > mn0 + U4_LIMIT) mn0 = floorf(mx0 - U4_LEVEL);   // whole numbers: what is scaled below loses nothing
+          if (mx1 > mn1 + U4_LIMIT) mn1 = floorf(mx1 - U4_LEVEL);
           const float al0 = exp2f(m0 - mn0), al1 = exp2f(m1 - mn1);
           l0 *= al0;
           l1 *= al1;
@@ -713,6 +759,11 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, U4Shape<HD>::BLOCKS) 
               add2(o_lo[pair * 2 + j][c], o_lo[pair * 2 + j][c + 1], cr[j][c], cr[j][c + 1]);
             }
         }
+      }
+      if (again) {   // the same pages for the next class of their rows
+        if (special) special_at = n;
+        n -= PP;
+        continue;
       }
       // the warp is done with these stages: their next pages, a lane for each
       const int next = n + SLOTS;
