@@ -161,6 +161,7 @@ struct U4Smem {
   static constexpr int FIXED = Q_BYTES + QROWS_BYTES + QSUM_BYTES + ML_BYTES + BAR_BYTES + 64 + NEW_BYTES + RECV_BYTES;
   static constexpr int RING_BYTES = WARPS * SLOTS * STAGE > O_BYTES ? WARPS * SLOTS * STAGE : O_BYTES;
   static constexpr int TOTAL = RING_BYTES + FIXED;
+  static_assert(U4_EXP_MIN == -40, "the largest 2^-e of a row is 2^40");
   static_assert(STAGE % 16 == 0 && TILE % 16 == 0 && QSUM_BYTES % 16 == 0, "16-byte pieces");
   static_assert(RING_BYTES % 16 == 0 && BAR_BYTES % 16 == 0, "16-byte pieces");
 };
@@ -642,8 +643,13 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
 #pragma unroll
           for (int u = 0; u < PP; ++u)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 2; ++r) {
+              if (back[u][r] > 0x1p40f) {   // a row that nobody wrote: zeros, its e read as -127, which becomes the least there is
+                z[u][2 * r] += 127 + U4_EXP_MIN, z[u][2 * r + 1] += 127 + U4_EXP_MIN;
+                back[u][r] = 0x1p40f;
+              }
               if (back[u][r] > taken) least = fminf(least, back[u][r]);
+            }
           asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(least) : "f"(least));
           const float limit = least * U4_SPREAD;
           bool left = false;

@@ -88,3 +88,22 @@ def test_a_step_behind_a_rejected_tail(state, dtype, hd, n, window):
         held[n] = row
     assert _close(d_out.download(), ref.attention(q, k[:n + 1], v[:n + 1], kv_heads, first), dtype)
     kv.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_heads,kv_heads,hd", [(8, 2, 128), (16, 2, 256), (4, 2, 64), (2, 1, 96)])
+def test_rows_that_nobody_wrote_are_zeros(state, dtype, q_heads, kv_heads, hd):
+    """A cursor moved ahead of what was written: the rows between read back as zeros, and weigh as zeros do."""
+    rng = np.random.default_rng(hd)
+    kv = state.full_attention(90, q_heads, kv_heads, hd, dtype, shuffled_seed=3)
+    q = rng.standard_normal((q_heads, hd)).astype(np.float32)
+    kv.truncate(37)
+    assert not kv.gather_rows_f32()[1].any()
+    assert not kv.attention_decode(q).any()
+    k, v = rng.standard_normal((2, 40, kv_heads * hd)).astype(np.float32)
+    kv.append_batch(k, v)
+    held = [x.astype(np.float64) for x in kv.gather_rows_f32()]
+    for start in (0, 36, 37):
+        assert _close(kv.attention_decode_windowed(q, start), ref.attention(q, *held, kv_heads, start), dtype), start
+    kv.close()
