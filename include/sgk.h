@@ -117,8 +117,8 @@ int64_t sgk_state_launches(const sgk_state* state);
 int32_t sgk_state_chain_begin(sgk_state* state, void* stream);
 int32_t sgk_state_chain_end(sgk_state* state);
 
-/* Failure-detection self test: launches a kernel whose only wait (on an mbarrier nobody
- * completes) must expire. Returns SGK_ERR_TIMEOUT when the bounded wait reported through the
+/* Failure-detection self test: launches a kernel whose waits (on an mbarrier nobody
+ * completes; then a whole warp of which half the lanes wait on a completed one) must expire. Returns SGK_ERR_TIMEOUT when the bounded wait reported through the
  * status word as designed; the device and the state stay usable. */
 int32_t sgk_state_selftest_wait_timeout(sgk_state* state);
 

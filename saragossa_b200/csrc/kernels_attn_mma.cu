@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
         next_stage -= nst;
         next_parity ^= 1;
       }
-      const bool ok = mbar_wait(smem_u32(bars + stage), parity, abort_flag, a.status);
+      const bool ok = mbar_wait_warp(smem_u32(bars + stage), parity, abort_flag, a.status);
       if (i == 0) SGK_TP(2);
       uint8_t* ktile = ring + size_t(stage) * S::STAGE;
       uint8_t* vtile = ktile + S::TILE;
@@ -455,15 +455,23 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_mma_kernel(AttnArgs 
 // The wait gives up after its spin limit, sets the device status word and the kernel returns;
 // the context stays usable. Used by the failure-detection test.
 __global__ void wait_timeout_selftest_kernel(int32_t* status) {
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bar, done;
   __shared__ int abort_flag;
   if (threadIdx.x == 0) {
     abort_flag = 1;  // start with the short spin limit
     mbar_init(smem_u32(&bar), 1);
+    mbar_init(smem_u32(&done), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    mbar_arrive(smem_u32(&done));
   }
   __syncthreads();
   if (threadIdx.x == 0) mbar_wait(smem_u32(&bar), 0, &abort_flag, status);
+  __syncthreads();
+  // Lanes whose waits end differently get one answer: half of them wait on a barrier that is complete. A lane that is told
+  // that all is well says so with the other error.
+  const bool ok = mbar_wait_warp(smem_u32(threadIdx.x & 1 ? &done : &bar), 0, &abort_flag, status);
+  __syncthreads();
+  if (ok) atomicExch(status, DEV_ERR_BAD_PAGE);
 }
 
 cudaError_t launch_wait_timeout_selftest(int32_t* status, cudaStream_t stream) {

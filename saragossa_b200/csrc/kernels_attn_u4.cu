@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
         const bool pair = PP > 1 && n + 1 < count;
         bool ready = mbar_try_wait(bar, phase);
         if (PP > 1) ready = (mbar_try_wait(bar + (pair ? 8 : 0), phase)) && ready;
-        if (!ready) ok = mbar_wait(bar, phase, abort_flag, a.status) && mbar_wait(bar + (pair ? 8 : 0), phase, abort_flag, a.status);
+        if (__any_sync(0xffffffffu, !ready))
+          ok = mbar_wait_warp(bar, phase, abort_flag, a.status) && mbar_wait_warp(bar + (pair ? 8 : 0), phase, abort_flag, a.status);
       }
       if (!ok) {
         // gave up (reported): the copies still on their way are waited for, with the short bound, before the block leaves

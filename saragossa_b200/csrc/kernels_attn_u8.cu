@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(MMA_THREADS, 2) attention_u8_kernel(AttnArgs a
     uint32_t parity = 0;
     bool ready = false;  // the page's barrier was already seen complete during the previous page
     for (int i = warp; i < my_pages; i += MMA_CONSUMERS) {
-      const bool ok = ready || mbar_wait(smem_u32(bars + stage), parity, abort_flag, a.status);
+      bool ok = true;
+      if (__any_sync(0xffffffffu, !ready)) ok = mbar_wait_warp(smem_u32(bars + stage), parity, abort_flag, a.status);
       U8_PHASE(tp_wait);
       if (i == 0) SGK_TP(2);
       uint8_t* ktile = ring + size_t(stage) * S::STAGE;

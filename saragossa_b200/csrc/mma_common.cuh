@@ -67,6 +67,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   atomicExch(status, DEV_ERR_WAIT_TIMEOUT);
   return false;
 }
+// The same for a whole warp, with one answer for all its lanes: what follows has votes, shuffles and matrix instructions of the
+// whole warp, and lanes whose own waits ended differently would wait there for one another.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+  const bool ok = mbar_wait(bar, parity, abort_flag, status);
+  return __all_sync(0xffffffffu, ok);
+}
 // Pages are read once per launch: their copies carry the L2 evict-first policy, so that they do
 // not push the small data every block needs at once (cursors, block tables, q, split partials)
 // out of L2. Measured on the u8 kernel at batch 8: 64.4 -> 60.5 us per layer.
