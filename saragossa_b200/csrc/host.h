@@ -233,12 +233,12 @@ struct Batch {
   float* d_part2_ml = nullptr;
   int32_t* d_group_counters = nullptr;
   int uniform_splits = 1;
-  int resident_per_sm = -1, resident_stages = 0;   // blocks of the attention kernel an SM holds at once
+  // What the attention kernel's instances fit at once, with queried_stages stages (asked once each, -1: not yet; 0 stages:
+  // nothing asked): blocks per SM [sinks][peers], and clusters on the device [sinks][blocks of a cluster]
+  int queried_stages = 0;
+  int resident_per_sm[2][2], max_clusters[2][17];
   const PeerTarget* peer_target = nullptr;   // not null: the launch being enqueued sends its outputs to the peers too
   bool peer_target_fused = false;            // set by enqueue_attention when the launch did take the peers
-  int max_clusters[17] = {-1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1, -1};   // per split count: clusters of
-                                                     // that many blocks the device holds at once (asked once)
-  int cluster_stages = 0;
   int max_splits = 1;
   int max_groups = 1;
   int splits_override = 0;

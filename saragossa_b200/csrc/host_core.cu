@@ -625,6 +625,13 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       a.trace_gt = 1;
     }
 #endif
+    const int sinks = a.sink_rows > 0;   // (launches with and without have kernel instances of their own)
+    if (queried_stages != a.n_stages) {
+      for (auto& row : resident_per_sm) row[0] = row[1] = -1;
+      for (auto& row : max_clusters)
+        for (int& c : row) c = -1;
+      queried_stages = a.n_stages;
+    }
     // When every block of the launch is resident at once, all blocks of a (sequence, KV head)
     // can merge a slice each after waiting for one another; otherwise (several waves, uneven
     // batches) the last arriver of a group merges, which needs nobody to wait. Blocks that wait
@@ -632,12 +639,12 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     // merge levels (more than 12 splits); below that, measured, the last arriver alone is faster.
     static const bool shared_merge_off = std::getenv("SGK_NO_SHARED_MERGE") != nullptr;
     if (!shared_merge_off && a.pages_per_split == 0 && a.splits > 12 && a.splits <= 160) {
-      if (resident_per_sm < 0 || resident_stages != a.n_stages)   // asked once per batch
-        resident_per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim, q_heads / pool->kv_heads)
-                          : kernel == 3 ? attention_u8_resident_blocks(pool->head_dim, a.n_stages)
-                                      : attention_mma_resident_blocks(pool->head_dim, a.n_stages),
-        resident_stages = a.n_stages;
-      const int per_sm = resident_per_sm;
+      // the instance that will be launched is asked, once per batch: each has registers of its own
+      int& per_sm = resident_per_sm[sinks][peer_target != nullptr];
+      if (per_sm < 0)
+        per_sm = kernel == 4   ? attention_u4_resident_blocks(pool->head_dim, q_heads / pool->kv_heads, peer_target != nullptr)
+                 : kernel == 3 ? attention_u8_resident_blocks(pool->head_dim, a.n_stages, peer_target != nullptr, sinks)
+                               : attention_mma_resident_blocks(pool->head_dim, a.n_stages, peer_target != nullptr, sinks);
       const int64_t blocks = int64_t(a.splits) * pool->kv_heads * n();
       // Blocks that wait for each other must all be resident. A cooperative launch guarantees it
       // next to launches of other streams too, and costs about 2 us per launch inside a graph; when
@@ -660,15 +667,12 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     // with three blocks and leave others one (8 sequences of 32768 rows, 4 heads of 128, 9 splits: 64.6 us, without 51.2).
     static const bool cluster_merge_off = std::getenv("SGK_NO_CLUSTER_MERGE") != nullptr;
     if (!cluster_merge_off && a.pages_per_split == 0 && a.splits >= 2 && a.splits <= (kernel == 4 ? 8 : 16)) {
-      if (cluster_stages != a.n_stages) {
-        for (int& c : max_clusters) c = -1;
-        cluster_stages = a.n_stages;
-      }
-      if (max_clusters[a.splits] < 0)
-        max_clusters[a.splits] = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, q_heads / pool->kv_heads, a.splits)
-                                 : kernel == 3 ? attention_u8_max_clusters(pool->head_dim, a.n_stages, a.splits)
-                                             : attention_mma_max_clusters(pool->head_dim, a.n_stages, a.splits);
-      a.cluster_merge = int64_t(pool->kv_heads) * n() <= max_clusters[a.splits];
+      int& clusters = max_clusters[sinks][a.splits];
+      if (clusters < 0)
+        clusters = kernel == 4   ? attention_u4_max_clusters(pool->head_dim, q_heads / pool->kv_heads, a.splits)
+                   : kernel == 3 ? attention_u8_max_clusters(pool->head_dim, a.n_stages, a.splits, sinks)
+                                 : attention_mma_max_clusters(pool->head_dim, a.n_stages, a.splits, sinks);
+      a.cluster_merge = int64_t(pool->kv_heads) * n() <= clusters;
     }
     // Several GPUs share the sequence: the launch sends its outputs to the peers itself and its last
     // block exchanges flags with them, when every block of the launch reaches its end (even splits)

@@ -123,21 +123,21 @@ cudaError_t attention_mma_configure();
 cudaError_t launch_wait_timeout_selftest(int32_t* status, cudaStream_t stream);
 int attention_mma_max_stages(int head_dim);
 // Blocks of the kernel one SM holds at once with `n_stages` stages (0 when the query fails).
-int attention_mma_resident_blocks(int head_dim, int n_stages);
-int attention_mma_max_clusters(int head_dim, int n_stages, int splits);
+int attention_mma_resident_blocks(int head_dim, int n_stages, bool peers, bool sinks);
+int attention_mma_max_clusters(int head_dim, int n_stages, int splits, bool sinks);
 // Tensor-core paged kernel for u8 group-32 pages: head_dim 128 or 256, q_heads/kv_heads <= 8.
 bool attention_u8_supported(int dtype, int head_dim, int gqa);
 cudaError_t launch_attention_u8(const AttnArgs& a, int n_seq, cudaStream_t stream);
 cudaError_t attention_u8_configure();
 int attention_u8_max_stages(int head_dim);
-int attention_u8_resident_blocks(int head_dim, int n_stages);
-int attention_u8_max_clusters(int head_dim, int n_stages, int splits);
+int attention_u8_resident_blocks(int head_dim, int n_stages, bool peers, bool sinks);
+int attention_u8_max_clusters(int head_dim, int n_stages, int splits, bool sinks);
 // The same for u4 group-32 pages.
 bool attention_u4_supported(int dtype, int head_dim, int gqa);
 cudaError_t launch_attention_u4(const AttnArgs& a, int n_seq, cudaStream_t stream);
 cudaError_t attention_u4_configure();
 int attention_u4_blocks_per_sm(int head_dim);
-int attention_u4_resident_blocks(int head_dim, int gqa);
+int attention_u4_resident_blocks(int head_dim, int gqa, bool peers);
 int attention_u4_max_clusters(int head_dim, int gqa, int splits);
 
 // Gather rows [row0, row0+n) of one layer into contiguous [n, kv_dim] arrays.

@@ -495,18 +495,26 @@ int attention_mma_max_stages(int head_dim) {
   return n / MMA_CONSUMERS * MMA_CONSUMERS;
 }
 
-int attention_mma_resident_blocks(int head_dim, int n_stages) {
+using Kernel = void (*)(AttnArgs);
+static Kernel kernel_for(int head_dim, bool cluster, bool peers, bool sinks) {
+  // [head_dim][sinks][plain, cluster, peers]
+  static const Kernel kernels[2][2][3] = {
+      {{attention_mma_kernel<128, false, false, false>, attention_mma_kernel<128, true, false, false>, attention_mma_kernel<128, false, true, false>},
+       {attention_mma_kernel<128, false, false, true>, attention_mma_kernel<128, true, false, true>, attention_mma_kernel<128, false, true, true>}},
+      {{attention_mma_kernel<256, false, false, false>, attention_mma_kernel<256, true, false, false>, attention_mma_kernel<256, false, true, false>},
+       {attention_mma_kernel<256, false, false, true>, attention_mma_kernel<256, true, false, true>, attention_mma_kernel<256, false, true, true>}}};
+  return kernels[head_dim == 256][sinks][peers ? 2 : cluster ? 1 : 0];
+}
+
+int attention_mma_resident_blocks(int head_dim, int n_stages, bool peers, bool sinks) {
   int blocks = 0;
-  cudaError_t e = head_dim == 128
-                      ? cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, attention_mma_kernel<128, false, false>, MMA_THREADS,
-                                                                      MmaSmem<128>::total(n_stages))
-                      : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, attention_mma_kernel<256, false, false>, MMA_THREADS,
-                                                                      MmaSmem<256>::total(n_stages));
+  const size_t smem = head_dim == 128 ? MmaSmem<128>::total(n_stages) : MmaSmem<256>::total(n_stages);
+  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel_for(head_dim, false, peers, sinks), MMA_THREADS, smem);
   return e == cudaSuccess ? blocks : 0;
 }
 
 // How many clusters of `splits` blocks the device can hold at once (0: such a launch would fail).
-int attention_mma_max_clusters(int head_dim, int n_stages, int splits) {
+int attention_mma_max_clusters(int head_dim, int n_stages, int splits, bool sinks) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, 1, 1);
   cfg.blockDim = dim3(MMA_THREADS);
@@ -519,24 +527,12 @@ int attention_mma_max_clusters(int head_dim, int n_stages, int splits) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  cudaError_t e = head_dim == 128 ? cudaOccupancyMaxActiveClusters(&n, attention_mma_kernel<128, true, false>, &cfg)
-                                  : cudaOccupancyMaxActiveClusters(&n, attention_mma_kernel<256, true, false>, &cfg);
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel_for(head_dim, true, false, sinks), &cfg);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
   return n;
-}
-
-using Kernel = void (*)(AttnArgs);
-static Kernel kernel_for(int head_dim, bool cluster, bool peers, bool sinks) {
-  // [head_dim][sinks][plain, cluster, peers]
-  static const Kernel kernels[2][2][3] = {
-      {{attention_mma_kernel<128, false, false, false>, attention_mma_kernel<128, true, false, false>, attention_mma_kernel<128, false, true, false>},
-       {attention_mma_kernel<128, false, false, true>, attention_mma_kernel<128, true, false, true>, attention_mma_kernel<128, false, true, true>}},
-      {{attention_mma_kernel<256, false, false, false>, attention_mma_kernel<256, true, false, false>, attention_mma_kernel<256, false, true, false>},
-       {attention_mma_kernel<256, false, false, true>, attention_mma_kernel<256, true, false, true>, attention_mma_kernel<256, false, true, true>}}};
-  return kernels[head_dim == 256][sinks][peers ? 2 : cluster ? 1 : 0];
 }
 
 cudaError_t attention_mma_configure() {

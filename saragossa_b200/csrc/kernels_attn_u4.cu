@@ -858,10 +858,10 @@ static U4Instance u4_instance(int head_dim, int gqa) {
 
 int attention_u4_blocks_per_sm(int head_dim) { return u4_instance(head_dim, 8).blocks_per_sm; }
 
-int attention_u4_resident_blocks(int head_dim, int gqa) {
+int attention_u4_resident_blocks(int head_dim, int gqa, bool peers) {
   const U4Instance x = u4_instance(head_dim, gqa);
   int blocks = 0;
-  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, x.kernels[0], x.threads, x.smem) == cudaSuccess ? blocks : 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, x.kernels[peers ? 2 : 0], x.threads, x.smem) == cudaSuccess ? blocks : 0;
 }
 
 // How many clusters of `splits` blocks the device can hold at once (0: such a launch would fail).
