@@ -197,14 +197,19 @@ int Seq::release_between(int64_t first_row, int64_t row) {
     upto = std::max(upto, released_pages);
   }
   if (upto > first && (first != released_first || upto != released_pages)) {
-    for (int64_t i = first; i < upto; ++i) {
-      if (pages[i] >= 0) pool->release(pages[i]);
-      pages[i] = -1;
-    }
+    // only the ends that are new: a long stream calls this page by page
+    const bool some = released_pages > released_first;
+    const int64_t from[2] = {first, some ? released_pages : upto}, to[2] = {some ? released_first : upto, upto};
     new_epoch();
     released_first = first;
     released_pages = upto;
-    SGK_TRY(publish(first, upto - first));
+    for (int end = 0; end < 2; ++end) {
+      for (int64_t i = from[end]; i < to[end]; ++i) {
+        if (pages[i] >= 0) pool->release(pages[i]);
+        pages[i] = -1;
+      }
+      SGK_TRY(publish(from[end], to[end] - from[end]));
+    }
   }
   if (!pool->host_only()) SGK_TRY(pool->flush_scrub(pool->st->stream));
   return SGK_OK;
