@@ -14,6 +14,7 @@
 #include <memory>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/sgk.h"
@@ -224,6 +225,7 @@ struct Batch {
   State* st = nullptr;
   Pool* pool = nullptr;
   std::vector<Kv*> kvs;
+  std::vector<std::pair<int, int>> same_sequence;   // (first member, later member) that are one sequence
   int layer = 0, q_heads = 0;
   int32_t* d_slots = nullptr;
   int32_t* d_counters = nullptr;  // [n*max(q_heads,kv_heads)] head, [n] seq, [n] append-done

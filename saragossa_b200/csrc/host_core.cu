@@ -309,11 +309,14 @@ int create_batch(State* st, Kv** kvs, int n, Batch** out) {
   b->q_heads = kvs[0]->q_heads;
   if (b->pool->host_only()) return fail(SGK_ERR_BACKEND, "batch over a bookkeeping-only pool");
   std::vector<int32_t> slots;
+  std::unordered_map<const Seq*, int> first_of;
   for (int i = 0; i < n; ++i) {
     if (kvs[i]->pool() != b->pool || kvs[i]->layer != b->layer || kvs[i]->q_heads != b->q_heads)
       return fail(SGK_ERR_CONFIG, "batch members must share pool, layer and q_heads");
     b->kvs.push_back(kvs[i]);
     slots.push_back(kvs[i]->seq->slot);
+    const auto first = first_of.emplace(kvs[i]->seq, i);
+    if (!first.second) b->same_sequence.emplace_back(first.first->second, i);
   }
   const int heads = std::max(b->q_heads, b->pool->kv_heads);
   // Splits never need to exceed about two blocks per SM for the whole launch.
@@ -484,11 +487,10 @@ int Batch::enqueue_truncate(cudaStream_t stream, const int64_t* lens) {
   for (int i = 0; i < n(); ++i)
     if (lens[i] < 0 || lens[i] > kvs[i]->seq->capacity)
       return fail(SGK_ERR_DIMENSION, "truncate KV %lld > capacity %lld", (long long)lens[i], (long long)kvs[i]->seq->capacity);
-  for (int i = 0; i < n(); ++i)
-    for (int j = 0; j < i; ++j)
-      if (kvs[i]->seq == kvs[j]->seq && lens[i] != lens[j])
-        return fail(SGK_ERR_DIMENSION, "truncate: members %d and %d are one sequence, with lengths %lld and %lld", j, i,
-                    (long long)lens[j], (long long)lens[i]);
+  for (const auto& [j, i] : same_sequence)
+    if (lens[i] != lens[j])
+      return fail(SGK_ERR_DIMENSION, "truncate: members %d and %d are one sequence, with lengths %lld and %lld", j, i,
+                  (long long)lens[j], (long long)lens[i]);
   for (int i = 0; i < n(); ++i) SGK_TRY(kvs[i]->seq->reserve(lens[i]));
   SetLensArgs a{};
   a.lens = pool->d_lens;

@@ -41,3 +41,37 @@ def test_either_end_of_what_was_returned():
     assert pool.free_pages == 16
     seq.close()
     pool.close()
+
+
+@pytest.mark.gpu
+def test_truncating_a_large_batch():
+    """The host's part of a batched truncation grows with the members, not with their pairs."""
+    st = sg.DecodeResidentState(0)
+    most, took = 6000, {}
+    pool = st.pool(1, 1, 32, sg.KV_U4G32, most, most, 16)
+    seqs = [pool.sequence(16) for _ in range(most)]
+    kvs = [s.layer(0, 1) for s in seqs]
+    for n in (600, most):
+        batch = sg.Batch(st, kvs[:n])
+        lens = [i % 16 for i in range(n)]
+        batch.enqueue_truncate(lens)
+        st.sync()
+        times = []
+        for _ in range(30):
+            times.append(_time(lambda: batch.enqueue_truncate(lens)))
+            st.sync()
+        took[n] = min(times)
+        batch.close()
+    assert [kv.len() for kv in kvs] == lens
+    # ten times the members, ten times the work (launches of 512 members among it); their pairs would be a hundred times as many
+    assert took[most] < 30 * took[600], took
+    both = sg.Batch(st, [kvs[3], kvs[5], kvs[3], kvs[7], kvs[3]])
+    for bad in ([1, 2, 1, 3, 4], [1, 2, 4, 3, 1], [4, 2, 1, 3, 1]):
+        with pytest.raises(sg.InferError) as e:
+            both.enqueue_truncate(bad)
+        assert e.value.kind == "Dimension"
+    both.enqueue_truncate([9, 2, 9, 3, 9])
+    st.sync()
+    assert [kvs[i].len() for i in (3, 5, 7)] == [9, 2, 3]
+    for x in (both, *seqs, pool, st):
+        x.close()
