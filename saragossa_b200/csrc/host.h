@@ -226,6 +226,7 @@ struct Batch {
   Pool* pool = nullptr;
   std::vector<Kv*> kvs;
   std::vector<std::pair<int, int>> same_sequence;   // (first member, later member) that are one sequence
+  std::vector<int64_t> pages_of;   // scratch of an uneven batch's launch over u4 pages; its memory stays
   int layer = 0, q_heads = 0;
   int32_t* d_slots = nullptr;
   int32_t* d_counters = nullptr;  // [n*max(q_heads,kv_heads)] head, [n] seq, [n] append-done

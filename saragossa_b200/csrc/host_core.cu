@@ -565,14 +565,14 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     // would make the launch as long as its longest block. Cut every sequence into pieces of the
     // same size instead, about three waves of blocks in all, and let the scheduler balance them.
     int64_t lo = INT64_MAX, hi = 0, total = 0;
-    std::vector<int64_t> pages_of;
+    pages_of.clear();
     for (Kv* kv : kvs) {
       int64_t rows = kv->len() + (fused ? 1 : 0);
       if (sliding_window > 0) rows = std::min<int64_t>(rows, std::min(sliding_window, rows) + PAGE_TOKENS + sink_rows);
       else rows -= std::min<int64_t>(rows, window_start) - SinkSpan(sink_rows, std::min<int64_t>(rows, window_start)).rows;
       const int64_t pages = (rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
       lo = std::min(lo, pages), hi = std::max(hi, pages), total += pages;
-      pages_of.push_back(pages);
+      if (kernel == 4) pages_of.push_back(pages);
     }
     if (hi * 4 > lo * 5 && hi >= 32) {
       const int64_t slots = int64_t(st->sm_count) * (kernel == 4 ? attention_u4_blocks_per_sm(pool->head_dim) : 2);
