@@ -482,7 +482,7 @@ int32_t sgk_kv_append_rows_f32(sgk_kv* kv, const float* k, size_t k_len, const f
   if (!kv) return fail(SGK_ERR_BACKEND, "null KV state");
   // LayerKvCache::append_batch (src/decoder/attention_cache.rs:47-58): seq > 0
   if (n_rows <= 0) return fail(SGK_ERR_DIMENSION, "append_batch needs at least one row");
-  if (kv->len() + n_rows > kv->seq->capacity)
+  if (n_rows > kv->seq->capacity - kv->len())
     return fail(SGK_ERR_DIMENSION, "append KV: capacity %lld reached (overflow)", (long long)kv->seq->capacity);
   return append_rows_host(kv, k, k_len, v, v_len, n_rows, false);
 }
@@ -496,6 +496,8 @@ int32_t sgk_kv_enqueue_append(sgk_kv* kv, void* stream, const float* d_k, const 
 int32_t sgk_kv_enqueue_append_rows(sgk_kv* kv, void* stream, const float* d_k, const float* d_v, int64_t n_rows) {
   if (!kv) return fail(SGK_ERR_BACKEND, "null KV state");
   if (n_rows <= 0) return fail(SGK_ERR_DIMENSION, "append_batch needs at least one row");
+  if (n_rows > kv->seq->capacity - kv->len())   // (before the count becomes an int)
+    return fail(SGK_ERR_DIMENSION, "append KV: capacity %lld reached (overflow)", (long long)kv->seq->capacity);
   SGK_TRY(kv->ensure_self_batch());
   return kv->self_batch->enqueue_append(kv->st->pick(stream), d_k, d_v, static_cast<int>(n_rows), nullptr, nullptr);
 }
@@ -627,8 +629,8 @@ static int32_t gather_impl(sgk_kv* kv, int64_t row0, int64_t n, int mode, void* 
                            uint16_t* kb, uint16_t* vs, uint16_t* vb) {
   if (!kv) return fail(SGK_ERR_BACKEND, "null KV state");
   if (!k_out || !v_out) return fail(SGK_ERR_BACKEND, "null host pointer");
-  if (row0 < 0 || n < 0 || row0 + n > kv->len())
-    return fail(SGK_ERR_DIMENSION, "gather rows [%lld,%lld) outside len %lld", (long long)row0, (long long)(row0 + n),
+  if (row0 < 0 || n < 0 || row0 > kv->len() || n > kv->len() - row0)
+    return fail(SGK_ERR_DIMENSION, "gather of %lld rows from row %lld outside len %lld", (long long)n, (long long)row0,
                 (long long)kv->len());
   if (n == 0) return SGK_OK;
   if (kv->seq->released(row0 / PAGE_TOKENS, (row0 + n + PAGE_TOKENS - 1) / PAGE_TOKENS))
