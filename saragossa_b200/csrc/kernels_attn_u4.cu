@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
     }
   }
   __syncthreads();
-  finish_block<HD, CLUSTER, PEERS, THREADS, 1, WARPS, true>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
+  finish_block<HD, CLUSTER, PEERS, THREADS, 1, WARPS>(a, o_s, ml_s, S::OPAD, flags, seq, kvh, split, gqa, do_append, len_ptr, len, tid,
                                    splits, recv_s);
   if (PEERS) peers_finish(a, tid, flags);
 }

@@ -282,10 +282,7 @@ __device__ __forceinline__ void peers_finish(const AttnArgs& a, int tid, int* fl
 // reduced with shuffles. The tail of the launch is then one wait and one L2 round trip instead of
 // two merge levels done by single blocks. Returns false when the wait ran out.
 constexpr int SHARED_MERGE_MAX_SPLITS = 160;   // five partials per lane
-// WIDE (up to 32 splits): a warp takes 32 neighbouring cells, a lane per cell, and walks the partials with coalesced loads
-// and no shuffles, in a different order of additions than the lane-per-partial form. Together with
-// taking the query's sums where its fragments are made it took 4 to 7 % off the calls of one or two sequences over 4-bit pages.
-template <int HD, int NT, bool PEERS = false, bool WIDE = false>
+template <int HD, int NT, bool PEERS = false>
 __device__ __forceinline__ bool shared_merge(const AttnArgs& a, int splits, int split, int gqa, int64_t qh0,
                                              int32_t* arrive_counter, int32_t* depart_counter, int* flags, int tid) {
   volatile int* abort_flag = flags;
@@ -306,31 +303,7 @@ __device__ __forceinline__ bool shared_merge(const AttnArgs& a, int splits, int 
     const int lane = tid & 31;
     const int warps = NT / 32;
     const int cells = gqa * (HD / 4);
-    if (WIDE && splits <= 32) {
-      for (int cell = (split * warps + (tid >> 5)) * 32 + lane; cell < cells; cell += splits * warps * 32) {
-        const int h = cell / (HD / 4), d = (cell % (HD / 4)) * 4;
-        const float* pm = a.part.ml + (qh0 + h) * a.splits * 2;
-        const float* po = a.part.o + (qh0 + h) * a.splits * HD + d;
-        float m = -1.0e30f;
-#pragma unroll 8
-        for (int p = 0; p < splits; ++p) m = fmaxf(m, __ldcg(pm + 2 * p));
-        float l = 0.0f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int p = 0; p < splits; ++p) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(pm + 2 * p));
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(po + int64_t(p) * HD));
-          const float w = exp2f(ml.x - m);
-          l += ml.y * w;
-          acc.x += v.x * w;
-          acc.y += v.y * w;
-          acc.z += v.z * w;
-          acc.w += v.w * w;
-        }
-        const float inv = 1.0f / l;
-        store_out<PEERS>(a, (qh0 + h) * HD + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      }
-    } else if (splits <= 32) {
+    if (splits <= 32) {
       // One partial per lane. With few splits a block owns many cells (29 at 18 splits, head_dim
       // 256): four cells per pass, all their loads issued before the first reduction, so the
       // block pays a quarter of the L2 round trips.
@@ -612,8 +585,7 @@ __device__ __forceinline__ void merge_block(const AttnArgs& a, const Partials& s
 // shared memory). A separate instance, so that the other one is compiled without a trace of that path:
 // with both in one kernel the page loop of the long-stream case lost 1.3 % (register allocation).
 // WARPS: warps whose states are in o_s and ml_s; the area behind ml_s holds WARPS * 24 + 16 floats in all.
-template <int HD, bool CLUSTER, bool PEERS = false, int NT = MMA_THREADS, int CELLS = (NT >= 256 ? 1 : 2), int WARPS = MMA_CONSUMERS,
-          bool WIDE = false>
+template <int HD, bool CLUSTER, bool PEERS = false, int NT = MMA_THREADS, int CELLS = (NT >= 256 ? 1 : 2), int WARPS = MMA_CONSUMERS>
 __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s, const float* ml_s, int opad,
                                              int* flags, int seq, int kvh, int split, int gqa, bool do_append,
                                              int32_t* len_ptr, int64_t len, int tid, int splits, float* recv) {
@@ -691,7 +663,7 @@ __device__ __forceinline__ void finish_block(const AttnArgs& a, const float* o_s
           a.seq_counters[seq] = 0;
         }
       }
-      shared_merge<HD, NT, PEERS, WIDE>(a, splits, split, gqa, qh0, head_counter, group_counter - group, flags, tid);
+      shared_merge<HD, NT, PEERS>(a, splits, split, gqa, qh0, head_counter, group_counter - group, flags, tid);
       if (tid == 0) SGK_TP(7);
       return;
     }
