@@ -370,7 +370,7 @@ int Batch::choose_splits(int kernel, int64_t max_rows) const {
     // keeps a few pages of work.
     const int heads = kernel >= 2 ? pool->kv_heads : q_heads;
     // (Over u4 pages two blocks per SM are as fast as the three or four that fit, with fewer partials to merge: one
-    // sequence of 32768 rows, 4 heads of 128, 16.4 us against 18.4; eight of them 51.5 against 53.3.)
+    // sequence of 32768 rows, 4 heads of 128, 16.4 us against 18.4.)
     const int64_t slots = int64_t(st->sm_count) * (kernel >= 2 ? 2 : 8);
     const int64_t units = int64_t(heads) * n();
     const int64_t pages = (max_rows + PAGE_TOKENS - 1) / PAGE_TOKENS;
@@ -389,8 +389,10 @@ int Batch::choose_splits(int kernel, int64_t max_rows) const {
       }
       if (eff >= 0.985) break;
     }
-    // Nine to twelve splits over u4 pages neither merge as a cluster (up to 8) nor all together (from 13 on), and are no
-    // faster than eight that do: 8 sequences, 4 heads of 128, 2048 rows 12.3 us against 10.3, 8192 rows 21.6 against 18.8.
+    // Nine to twelve splits over u4 pages neither merge as a cluster (up to 8) nor all together (from 13 on); eight that do, with
+    // and without this rule: 8 sequences, 4 heads of 128, 2048 rows 10.9 and 13.3 us, 8192 rows 19.1 and 22.1; 16 of 4096 rows, 2
+    // heads of 128, 14.4 and 17.0; 14 of 3000 rows, 2 heads of 64, 10.8 and 11.6; it loses where pages are long: 12 of 6000
+    // rows, 2 heads of 256, 22.1 and 21.1.
     if (kernel == 4 && best > 8 && best <= 12) best = 8;
     s = best;
   }
@@ -578,11 +580,13 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
       const int64_t slots = int64_t(st->sm_count) * (kernel == 4 ? attention_u4_blocks_per_sm(pool->head_dim) : 2);
       int64_t pps = (total * pool->kv_heads + slots * 3 - 1) / (slots * 3);
       if (kernel == 4 && int64_t(n()) * pool->kv_heads * 2 <= slots) {
-        // Over u4 pages the multiplications are the bound, not the stream, and what a block spends on its start and its
-        // merge counts for more: pieces just large enough for one wave (24 sequences of 200 to 20000 rows, 8 heads of 128:
-        // pieces of 149 pages 41.0 us, of 100 to 130, which need a second wave, 48.7 to 50.5, of 185 47.1).
-        // A sequence of at most half a piece counts half: two such blocks share a place one after the other (40.9 us against
-        // 44.6 where each counts as a block).
+        // Over u4 pages the stream is not the bound, and what a block spends on its start and its merge counts for more: pieces
+        // just large enough for one wave. With and without this rule: 24 sequences of 200 to 20000 rows, 8 heads of 128, 42.6
+        // and 52.5 us; 16 of 3000 to 30000, 4 heads of 128, 43.7 and 50.5; 32 of 450 to 9000, 2 heads of 256, 31.8 and 40.6; 10 of
+        // 8000 to 16000, 8 heads of 128, 43.6 and 55.5; 40 of 360 to 12000, 2 heads of 64, 19.2 and 23.2; 8 of 800 to 40000, 2
+        // heads of 128, 31.4 and 31.3.
+        // A sequence of at most half a piece counts half: two such blocks share a place one after the other (the first of
+        // these 42.6 against 45.8 where each counts as a block, the others as they are).
         pps = std::max<int64_t>(1, total * pool->kv_heads / slots);
         const auto half_blocks = [&] {
           int64_t sum = 0;
@@ -671,7 +675,7 @@ int Batch::enqueue_attention(cudaStream_t stream, const float* d_q, float* d_out
     // no partial goes through L2 and no device-wide atomic sits between the last page and the output.
     // Only when every cluster of the launch is resident at once: a launch that would fit one wave of
     // blocks must not get a second one from the placement of clusters. Over u4 pages up to 8: larger clusters fill some SMs
-    // with three blocks and leave others one (8 sequences of 32768 rows, 4 heads of 128, 9 splits: 64.6 us, without 51.2).
+    // with three blocks and leave others one (8 sequences of 32768 rows, 4 heads of 128, 9 splits: 64.6 us, 8 splits 51.2).
     static const bool cluster_merge_off = std::getenv("SGK_NO_CLUSTER_MERGE") != nullptr;
     if (!cluster_merge_off && a.pages_per_split == 0 && a.splits >= 2 && a.splits <= (kernel == 4 ? 8 : 16)) {
       int& clusters = max_clusters[sinks][a.splits];

@@ -29,10 +29,13 @@
 // would lose those digits.
 //
 // B200, one call after another on one stream, f32 queries, 32 query heads over 4 KV heads of 128: 8 sequences of 32768 rows
-// 51.5 us = 3.3 TB/s of page bytes (50 % of the copy rate; DRAM reads 1.013 of the page bytes), one sequence 16.4 us; 24 uneven
-// sequences of 200 to 20000 rows, 32 over 8 heads, 41.0 us = 3.4 TB/s; 64 windows of 2000 rows, 16 over 2 heads of 256, 30.8 us =
-// 2.8 TB/s. Not memory bounds it but the warps' instruction stream (364 instructions per page and KV head with start and
-// merge, 0.46 issued per scheduler and cycle, tensor pipe 34 %, ALU 29 %) and, below about 10 MB, start and merge.
+// 53.2 us = 3.2 TB/s of page bytes (48 % of the copy rate; DRAM reads 1.013 of the page bytes), one sequence 16.7 us; 24 uneven
+// sequences of 200 to 20000 rows, 32 over 8 heads, 41.0 us = 3.4 TB/s; 64 windows of 2000 rows, 16 over 2 heads of 256, 32.2 us =
+// 2.6 TB/s. No unit is full (8 x 32768: tensor pipe 33 %, ALU 27 %, DRAM 48 %; 0.43 instructions issued per scheduler and cycle,
+// 346 per page and KV head): with two warps per scheduler the bound is latency, first the fixed latencies between
+// dependent instructions (1.24 warps waiting per issue), then, below about 10 MB, start and merge.
+// With V rows 10^6 times the others': one of them, or the first four rows a hundredth of the others, nothing; one in 64, 91 us;
+// every second one, 107 us.
 //
 // The reference's KV has no 4-bit form; this kernel computes cached_attention_one
 // (src/decoder/attention_ops.rs:889-974) over the rows' values code * scale + bias.
@@ -208,7 +211,8 @@ __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park
 // PP: pages a warp works on at once. Two (head_dim 128) give the chains of matrix instructions twice the
 // independent work and share the query's fragments and the bookkeeping; with head_dim 256 one page fills the registers.
 // PAIRED (up to four query heads per KV head): the matrix instruction has eight columns, so column h + 4 takes the lo parts
-// of head h's query and weights beside the hi parts in column h: half the products and half their chains.
+// of head h's query and weights beside the hi parts in column h: half the products and half their chains (32/8 heads of 128: 24
+// uneven sequences 47.0 -> 42.5 us, 16 of 12000 rows 74.2 -> 67.3).
 // (Even batches place two blocks per SM: the cluster instance, which only they use, is compiled for no more than that. At three
 // it spilled, and 8 sequences of 32768 rows, 32/4 heads of 128, took 55.3 us instead of 53.2.)
 template <int HD, bool CLUSTER, bool PEERS, bool PAIRED>
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
   const int64_t head_off = int64_t(a.layer) * a.pool.layer_bytes + int64_t(kvh) * 2 * a.pool.tile_bytes;
   const bool owns_append = do_append && pe == n_pages && my_pages > 0;   // the new row lies in the last page
 
-  // Every warp owns every fourth stage of the ring and fetches its own pages: its n-th page has ordinal pb + warp + 4 n
+  // Every warp owns SLOTS neighbouring stages of the ring and fetches its own pages: its n-th page has ordinal pb + warp + 4 n
   // and goes to its stage n % SLOTS, one bulk copy per page, completion on the stage's barrier. A stage is refilled by the
   // warp itself as soon as it has used it up, so no second barrier and no producer stand between the two (a producer warp
   // needed about 640 cycles per page, waiting for the consumers' releases one by one).

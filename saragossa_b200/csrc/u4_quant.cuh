@@ -11,7 +11,7 @@
 // The floor 2^(e-16) lets V keep step / 2^e as an fp16 number without loss.
 //
 // Each rounding is of the exact value, although everything runs in f32: a difference a - b comes with
-// its rounding error (two-difference), multiples of a bf16 step by a number below 16 and of a 9-bit
+// its rounding error (Knuth's two-sum, for a difference), multiples of a bf16 step by a number below 16 and of a 9-bit
 // midpoint by 15 are exact, and so are the remainders they leave. A division that is rounded to f32
 // first and to bf16 afterwards picks the wrong neighbour about once in 2^15 groups.
 //
