@@ -29,12 +29,12 @@
 // would lose those digits.
 //
 // B200, one call after another on one stream, f32 queries, 32 query heads over 4 KV heads of 128: 8 sequences of 32768 rows
-// 53.2 us = 3.2 TB/s of page bytes (48 % of the copy rate; DRAM reads 1.013 of the page bytes), one sequence 16.7 us; 24 uneven
+// 51.5 us = 3.3 TB/s of page bytes (50 % of the copy rate; DRAM reads 1.013 of the page bytes), one sequence 16.7 us; 24 uneven
 // sequences of 200 to 20000 rows, 32 over 8 heads, 41.0 us = 3.4 TB/s; 64 windows of 2000 rows, 16 over 2 heads of 256, 32.2 us =
-// 2.6 TB/s. No unit is full (8 x 32768: tensor pipe 33 %, ALU 27 %, DRAM 48 %; 0.43 instructions issued per scheduler and cycle,
-// 346 per page and KV head): with two warps per scheduler the bound is latency, first the fixed latencies between
-// dependent instructions (1.24 warps waiting per issue), then, below about 10 MB, start and merge.
-// With V rows 10^6 times the others': one of them, or the first four rows a hundredth of the others, nothing; one in 64, 91 us;
+// 2.6 TB/s. No unit is full (8 x 32768: tensor pipe 33 %, ALU 27 %, DRAM 50 %; 0.44 instructions issued per scheduler and cycle,
+// 345 per page and KV head): with two warps per scheduler the bound is latency, first the fixed latencies between
+// dependent instructions (1.25 warps waiting per issue), then, below about 10 MB, start and merge.
+// With V rows 10^6 times the others': one of them, or the first four rows a hundredth of the others, 54 us; one in 64, 91 us;
 // every second one, 107 us.
 //
 // The reference's KV has no 4-bit form; this kernel computes cached_attention_one
@@ -214,7 +214,7 @@ __device__ __forceinline__ void u4_place_row(uint8_t* ktile, const uint8_t* park
 // of head h's query and weights beside the hi parts in column h: half the products and half their chains (32/8 heads of 128: 24
 // uneven sequences 47.0 -> 42.5 us, 16 of 12000 rows 74.2 -> 67.3).
 // (Even batches place two blocks per SM: the cluster instance, which only they use, is compiled for no more than that. At three
-// it spilled, and 8 sequences of 32768 rows, 32/4 heads of 128, took 55.3 us instead of 53.2.)
+// it spilled, and 8 sequences of 32768 rows, 32/4 heads of 128, took 54.2 us instead of 51.6.)
 template <int HD, bool CLUSTER, bool PEERS, bool PAIRED>
 __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD>::BLOCKS == 3 ? 2 : U4Shape<HD>::BLOCKS)
     attention_u4_kernel(AttnArgs a) {
@@ -452,6 +452,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
       o_lo[grp][0] = o_lo[grp][1] = o_lo[grp][2] = o_lo[grp][3] = 0.0f;
       o_b[0][grp] = o_b[1][grp] = 0.0f;
     }
+    float top0 = -1.0e30f, top1 = -1.0e30f;   // m0, m1 + U4_LIMIT
     float m0 = -1.0e30f, m1 = -1.0e30f, l0 = 0.0f, l1 = 0.0f;
     // The references are for rows with 2^-e <= back_limit (0: for none yet). While an iteration's rows are worked on class by class
     // back_limit is negative, and rows with 2^-e <= taken are done.
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
           mx0 = fmaxf(mx0, fmaxf(z[PP - 1][0], z[PP - 1][2])), mx1 = fmaxf(mx1, fmaxf(z[PP - 1][1], z[PP - 1][3]));
           most_back = fmaxf(most_back, fmaxf(back[PP - 1][0], back[PP - 1][1]));
         }
-        over = mx0 > m0 + U4_LIMIT || mx1 > m1 + U4_LIMIT || most_back > back_limit;
+        over = mx0 > top0 || mx1 > top1 || most_back > back_limit;
         if (__any_sync(0xffffffffu, over)) {
           // The class of this pass: the rows left with the largest powers of two, down to 1 / U4_SPREAD of the largest.
           float least = INFINITY;
@@ -693,6 +694,7 @@ __global__ void __launch_bounds__(U4Shape<HD>::WARPS * 32, CLUSTER && U4Shape<HD
           }
           m0 = mn0;
           m1 = mn1;
+          top0 = mn0 + U4_LIMIT, top1 = mn1 + U4_LIMIT;
         }
         // ---- weights ----
         uint32_t ph[PP][2], pl[PP][2];
