@@ -60,13 +60,16 @@ struct MmaSmem {
 };
 
 // A row that is not seen weighs nothing, whatever its bytes say: the staged V rows before `first` and from `last` on become
-// zeros (a weight of zero times a NaN left there is a NaN). One warp, for the page in which a window starts and the last
-// page. Not inlined: the page loop keeps its registers.
+// zeros (a weight of zero times a NaN left there is a NaN). One warp, two lanes per row, for the page in which a window
+// starts and the last page: it stands between that page's arrival and its products, 0.05 us of a token chain's 15.8 per layer.
 template <int HD>
-__device__ __noinline__ void blank_v_rows(uint8_t* vtile, int first, int last, int lane) {
-  for (int i = lane; i < PAGE_TOKENS * (HD / 8); i += 32) {
-    const int r = i / (HD / 8);
-    if (r < first || r >= last) *reinterpret_cast<uint4*>(vtile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+__device__ __forceinline__ void blank_v_rows(uint8_t* vtile, int first, int last, int lane) {
+  constexpr int CHUNKS = HD / 16;   // 16-byte pieces of half a row
+  const int r = lane >> 1;
+  if (r < first || r >= last) {
+    uint4* half = reinterpret_cast<uint4*>(vtile + r * (HD * 2)) + (lane & 1) * CHUNKS;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) half[(i + r) & (CHUNKS - 1)] = make_uint4(0u, 0u, 0u, 0u);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the copy that refills the stage
   __syncwarp();
